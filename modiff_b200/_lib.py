@@ -55,8 +55,16 @@ class GemmBf16Desc(C.Structure):
                 ("scale", C.c_float), ("b_rows", C.c_int32)]
 
 
+class Kv4CacheStruct(C.Structure):
+    """Mirror of `modiff_kv4_cache`."""
+    _fields_ = [("k_codes", C.c_void_p), ("v_codes", C.c_void_p), ("k_params", C.c_void_p),
+                ("v_params", C.c_void_p), ("pages", C.c_int32), ("heads", C.c_int32),
+                ("page_size", C.c_int32), ("dim", C.c_int32)]
+
+
 _P = C.c_void_p
 _G = C.POINTER(ConvGeom)
+_KV4 = C.POINTER(Kv4CacheStruct)
 
 # name -> (restype, argtypes); one entry per declaration of include/modiff_b200.h
 SIGNATURES = {
@@ -144,6 +152,20 @@ SIGNATURES = {
     "modiff_igemm_conv_packed4": (C.c_int, [_P, _P, _P, _P, _P, _P, C.c_int, _G, _P, _P, _P]),
     "modiff_adaround_fake_quant": (C.c_int, [_P, _P, _P, _P, _P, C.c_int64, C.c_int64, C.c_int,
                                              C.c_int, _P]),
+    "modiff_fp8_quantize": (C.c_int, [_P, C.c_int64, C.c_int64, C.c_int, C.c_int, _P, C.c_int64, _P,
+                                      C.c_int64, _P]),
+    "modiff_fp8_pack_weight": (C.c_int, [_P, C.c_int64, C.c_int, C.c_int, C.c_int, _P, C.c_int64, _P,
+                                         C.c_int64, _P]),
+    "modiff_fp8_linear": (C.c_int, [_P, C.c_int64, _P, C.c_int64, _P, C.c_int64, _P, C.c_int64, _P, _P,
+                                    C.c_int64, C.c_int, C.c_int, C.c_int, C.c_int, _P]),
+    "modiff_qk_norm_rope": (C.c_int, [_P, _P, _P, _P, C.c_int, _P, _P, _P, _P, C.c_int, _P, _P, _P, _P,
+                                      C.c_int64, _P, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int,
+                                      C.c_float, C.c_int, _P]),
+    "modiff_kv4_append": (C.c_int, [_KV4, _P, _P, _P, _P, _P, _P, C.c_int, C.c_int, C.c_int, C.c_int, _P]),
+    "modiff_kv4_read": (C.c_int, [_KV4, _P, _P, C.c_int, C.c_int, C.c_int, _P, _P, C.c_int, _P]),
+    "modiff_kv4_attention_bytes": (C.c_int64, [_KV4] + [C.c_int] * 6),
+    "modiff_kv4_attention": (C.c_int, [_P, _P, _KV4, _P, _P, _P, C.c_int, C.c_int, C.c_int, C.c_int,
+                                       C.c_float, C.c_int, C.c_int, C.c_int, C.c_int, _P, _P]),
     "modiff_attn_codes_bytes": (C.c_int64, [C.c_int] * 5),
     "modiff_attn_quantize": (C.c_int, [_P, _P, _P] + [C.c_int] * 5 + [_P, _P, C.c_int, _P, _P, _P,
                                                                    _P, _P, _P]),
@@ -181,6 +203,8 @@ KERNELS_PER_CALL = {
     "modiff_attn_quantize": 2, "modiff_attention_i8": 1, "modiff_adaround_fake_quant": 1,
     "modiff_pack_weights_int4": 1, "modiff_igemm_conv_packed4": 1,
     "modiff_f32_split_weights": 1, "modiff_f32_split": 1, "modiff_conv_f32_tc": 1,
+    "modiff_fp8_quantize": 1, "modiff_fp8_pack_weight": 1, "modiff_fp8_linear": 1,
+    "modiff_qk_norm_rope": 1, "modiff_kv4_append": 1, "modiff_kv4_read": 1, "modiff_kv4_attention": 1,
 }
 LAUNCHES = [0]        # kernels launched through `call` since import
 # Bumped whenever a layer allocates or replaces a device buffer that kernels address directly

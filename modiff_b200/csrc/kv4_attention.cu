@@ -1,0 +1,624 @@
+// Attention over a paged cache of keys and values held in 4 bits (layout: kv4_cache.cu):
+//   out = sum_t p_t (s_v[t] code_v[t] + m_v[t]) / sum_t p_t,
+//   p_t = exp(scale * q . (s_k[t] code_k[t] + m_k[t])) over the tokens that the query sees.
+//
+// The codes go into the tensor cores as they are.  A nibble n in the low bits of an fp16 word is the
+// subnormal number n 2^-24, in bits 4 - 7 it is 16 n 2^-24, both exact, so one AND (and a shift for the
+// upper byte) makes a pair of MMA operands out of eight packed codes' word; the factors 2^24 and 16 are
+// taken out of q and of the results.  Scale and minimum of a token leave the products:
+//   q . k_t = s_k (q . code) + m_k sum(q)            sum_t p_t v_t = sum_t (p_t s_v) code + sum_t p_t m_v
+// Queries are brought to fp16 by a power of two per row (exact for 16-bit types; fp32 queries and
+// weights travel as two fp16 planes, hi + lo, 22 bits).  p_t s_v is held in fp16 relative to the running
+// maximum of (score + exponent of s_v), so that it lies in [0, 2) 2^14 whatever the scales are.  Sums,
+// maxima and the output stay in fp32.
+//
+// mma.m16n8k16 with the tokens (scores) or the channels (output) as the 16 rows and eight query rows as
+// the columns: S^T = K Q^T, O^T = V^T P^T.  One step of a conversation has as many query rows per
+// key head as query heads share it, mostly 1 to 8, which fills the narrow side.  All operands come
+// straight from global memory into the registers of the thread that multiplies them: which channel is
+// which column of an MMA is free as long as both operands agree, so a thread takes consecutive bytes.
+//
+// Bound: HBM (d + 8 bytes per cached token and head) for single tokens.  The cache of one sequence
+// and head is split over `splits` blocks and the warps of each; partial results (numerator, sum,
+// maximum) are joined by kv4_join_kernel in a fixed order.
+#include <float.h>
+
+#include "kv4.cuh"
+
+namespace modiff {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kTile = 64;                 // tokens a warp takes at a time
+constexpr int kSub = kTile / 16;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct AttnParams {
+  const void* q;
+  int64_t qb, qt, qh;                     // element strides: sequence, token, head
+  void* out;                              // [batch][count][heads][dim]
+  float* part;                            // [splits][rows][dim], then sums and maxima [splits][rows] each
+  Kv4Pages c;
+  const int32_t* table;
+  const int32_t* lengths;
+  int batch, count, heads, group, max_pages, splits, row_tiles;
+  int causal, window, sinks;
+  float scale2;                           // scale * log2(e)
+  int64_t rows;                           // batch * count * heads
+};
+
+__device__ inline void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                               uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// transpose of an 8 x 8 matrix of 16-bit values held by the warp as an MMA fragment
+__device__ inline uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ inline float exp2_fast(float x) {   // hardware exp2, relative error about 2^-22
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ inline uint32_t half_pair(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ inline float2 half_values(uint32_t h) { return __half22float2(*reinterpret_cast<const __half2*>(&h)); }
+
+template <int BYTES>
+__device__ inline void load_words(const uint8_t* src, uint32_t (&w)[BYTES / 4]) {
+  if constexpr (BYTES % 16 == 0) {
+#pragma unroll
+    for (int i = 0; i < BYTES / 16; ++i) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + i);
+      w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+    }
+  } else if constexpr (BYTES % 8 == 0) {
+#pragma unroll
+    for (int i = 0; i < BYTES / 8; ++i) {
+      const uint2 v = __ldg(reinterpret_cast<const uint2*>(src) + i);
+      w[2 * i] = v.x; w[2 * i + 1] = v.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < BYTES / 4; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(src) + i);
+  }
+}
+
+// Tiles of kTile tokens that rows at positions [p_lo, p_hi] see any of: `first` tiles from 0 on (the
+// sinks), the others from tile `start` on.
+struct TileRange {
+  int first, start, count;
+  __device__ int tile(int i) const { return i < first ? i : start + (i - first); }
+};
+__device__ inline TileRange tiles_of(const AttnParams& p, int length, int p_lo, int p_hi) {
+  TileRange r;
+  const int end = p.causal ? min(length, p_hi + 1) : length;
+  int lo = 0, sink_end = 0;
+  if (p.window > 0) {
+    lo = max(0, p_lo - p.window + 1);
+    sink_end = min(min(p.sinks, lo), max(end, 0));
+  }
+  r.first = (sink_end + kTile - 1) / kTile;
+  r.start = max(lo / kTile, r.first);
+  const int last = end > 0 ? (end + kTile - 1) / kTile : 0;
+  r.count = r.first + max(0, last - r.start);
+  return r;
+}
+
+template <typename T, int D, int NT>
+constexpr int smem_bytes() {
+  constexpr int planes = sizeof(T) == 4 ? 2 : 1;
+  const int q = NT * (D / 16) * 32 * 8 * planes;               // query fragments
+  const int o = kWarps * NT * 8 * (D + 4) * 4;                 // the warps' outputs, joined at the end
+  return q > o ? q : o;
+}
+
+// One block: 8 * NT query rows (query, head of the group) of one sequence and key head, one part of
+// the tokens.
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kThreads)
+kv4_attention_kernel(const AttnParams p) {
+  constexpr int P = sizeof(T) == 4 ? 2 : 1;       // fp16 planes of q and of the weights
+  constexpr int R = 8 * NT;
+  constexpr int KW = D / 32;                      // words of a key row that a thread holds
+  constexpr int VW = D / 64;                      // words of a value row that a thread holds
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ float row_a[R], row_b[R];            // factors of (q . code) and of m_k
+  __shared__ float join_m[kWarps][R], join_l[kWarps][R], join_s[kWarps][R];
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, j = lane & 3;
+  int id = blockIdx.x;
+  const int split = id % p.splits;
+  id /= p.splits;
+  const int rt = id % p.row_tiles;
+  id /= p.row_tiles;
+  const int head = id % p.c.heads, b = id / p.c.heads;
+  const int row0 = rt * R;
+  const int rows_here = min(R, p.count * p.group - row0);
+  const int32_t* table = p.table + (int64_t)b * p.max_pages;
+  const int length = min(max(__ldg(p.lengths + b), 0), p.max_pages * p.c.page_size);
+
+  // ---- queries: one warp per row, brought to fp16 by a power of two, laid out as MMA fragments
+  uint32_t* q_frag = reinterpret_cast<uint32_t*>(smem);       // [plane][nt][k step][lane][2]
+  for (int r = warp; r < R; r += kWarps) {
+    float x[D / 32];
+    float top = 0.0f, sum = 0.0f;
+    const int rr = row0 + r;
+    const bool real = r < rows_here;
+    const T* src = static_cast<const T*>(p.q) + (int64_t)b * p.qb + (int64_t)(rr / p.group) * p.qt +
+                   (int64_t)(head * p.group + rr % p.group) * p.qh;
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) {
+      x[e] = real ? to_f32<T>(src[lane + 32 * e]) : 0.0f;
+      top = fmaxf(top, fabsf(x[e]));
+      sum += x[e];
+    }
+    for (int o = 16; o > 0; o >>= 1) {
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    }
+    // power of two that brings the largest element to [2^14, 2^15); in two factors, for fp32's range
+    int e2 = 0;
+    if (top > 0.0f && top < INFINITY) { frexpf(top, &e2); e2 = 15 - e2; }
+    const float f1 = ldexpf(1.0f, e2 / 2), f2 = ldexpf(1.0f, e2 - e2 / 2);
+    if (lane == 0) {
+      row_a[r] = ((p.scale2 * 16777216.0f) / f1) / f2;
+      row_b[r] = p.scale2 * sum;
+    }
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) {
+      const int ch = lane + 32 * e;
+      // thread j of an MMA holds channels [j D/4, (j + 1) D/4): word w, nibble n of them
+      const int tj = ch / (D / 4), w = ch % (D / 4) / 8, n = ch % 8;
+      const int step = 2 * w + ((n >> 1) & 1), reg = n & 1, half_at = n >> 2;
+      float v = x[e] * f1 * f2;
+      if (n & 1) v *= 0.0625f;
+      __half* dst = reinterpret_cast<__half*>(
+          &q_frag[(((r >> 3) * (D / 16) + step) * 32 + ((r & 7) * 4 + tj)) * 2 + reg]) + half_at;
+      const __half hi = __float2half_rn(v);
+      *dst = hi;
+      if (P == 2) dst[NT * (D / 16) * 32 * 2 * 2] = __float2half_rn(v - __half2float(hi));
+    }
+  }
+  __syncthreads();
+
+  const int pos_lo = length - p.count + row0 / p.group;
+  const int pos_hi = length - p.count + (row0 + rows_here - 1) / p.group;
+  const TileRange range = tiles_of(p, length, pos_lo, pos_hi);
+  const int t_begin = (int)((int64_t)range.count * split / p.splits);
+  const int t_end = (int)((int64_t)range.count * (split + 1) / p.splits);
+
+  float o[D / 16][NT][4];
+  float m_run[NT][2], l_run[NT][2], s_run[NT][2], ra[NT][2], rb[NT][2];
+  int pos[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][nt][e] = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = 8 * nt + 2 * j + e;
+      m_run[nt][e] = -INFINITY;
+      l_run[nt][e] = s_run[nt][e] = 0.0f;
+      ra[nt][e] = row_a[r];
+      rb[nt][e] = row_b[r];
+      pos[nt][e] = length - p.count + (row0 + r) / p.group;
+    }
+  }
+  const int64_t row_bytes = D / 2;
+  const __half2* k_par = reinterpret_cast<const __half2*>(p.c.k_params);
+  const __half2* v_par = reinterpret_cast<const __half2*>(p.c.v_params);
+
+  for (int ti = t_begin + warp; ti < t_end; ti += kWarps) {
+    const int t0 = range.tile(ti) * kTile;
+    // rows of the cache where the four pieces of 16 tokens begin; -1: not there
+    int64_t base[kSub];
+    bool whole = true;
+#pragma unroll
+    for (int u = 0; u < kSub; ++u) {
+      base[u] = t0 + 16 * u < length ? kv4_place(p.c, table, p.max_pages, t0 + 16 * u, head) : -1;
+      whole &= base[u] >= 0;
+    }
+    // does every row see every token?
+    whole &= t0 + kTile <= length;
+    if (p.causal) whole &= t0 + kTile <= pos_lo + 1;
+    if (p.window > 0) whole &= t0 > pos_hi - p.window || t0 + kTile <= p.sinks;
+
+    // ---- scores
+    float s[kSub][NT][4];
+    float2 kp[kSub][2], vp[kSub][2];
+    uint32_t kw[kSub][2][KW];
+#pragma unroll
+    for (int u = 0; u < kSub; ++u)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int64_t at = base[u] + g + 8 * e;
+        if (base[u] >= 0) {
+          load_words<4 * KW>(p.c.k_codes + at * row_bytes + j * (D / 8), kw[u][e]);
+        } else {
+#pragma unroll
+          for (int w = 0; w < KW; ++w) kw[u][e][w] = 0;
+        }
+      }
+#pragma unroll
+    for (int u = 0; u < kSub; ++u)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int64_t at = base[u] + g + 8 * e;
+        kp[u][e] = vp[u][e] = make_float2(0.0f, 0.0f);
+        if (base[u] >= 0 && t0 + 16 * u + g + 8 * e < length) {   // beyond the last token: whatever was there
+          kp[u][e] = __half22float2(__ldg(k_par + at));
+          vp[u][e] = __half22float2(__ldg(v_par + at));
+        }
+      }
+#pragma unroll
+    for (int u = 0; u < kSub; ++u) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[u][nt][e] = 0.0f;
+    }
+#pragma unroll
+    for (int w = 0; w < KW; ++w)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint2 qf[P][NT];
+#pragma unroll
+        for (int pl = 0; pl < P; ++pl)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            qf[pl][nt] = *reinterpret_cast<const uint2*>(
+                &q_frag[(((pl * NT + nt) * (D / 16) + 2 * w + h) * 32 + lane) * 2]);
+#pragma unroll
+        for (int u = 0; u < kSub; ++u) {
+          const uint32_t w0 = h ? kw[u][0][w] >> 8 : kw[u][0][w];
+          const uint32_t w1 = h ? kw[u][1][w] >> 8 : kw[u][1][w];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int pl = 0; pl < P; ++pl)
+              mma_f16(s[u][nt], w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u,
+                      qf[pl][nt].x, qf[pl][nt].y);
+        }
+      }
+
+    // ---- value codes of the first piece are on their way while the softmax runs
+    uint32_t vw[4][VW];
+    auto load_values = [&](int u) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int64_t at = base[u] + 2 * j + (e & 1) + 8 * (e >> 1);
+        if (base[u] >= 0) {
+          load_words<4 * VW>(p.c.v_codes + at * row_bytes + g * (D / 16), vw[e]);
+        } else {
+#pragma unroll
+          for (int w = 0; w < VW; ++w) vw[e][w] = 0;
+        }
+      }
+    };
+    load_values(0);
+
+    // ---- softmax: scores in units of log2, reference = running maximum of score + exponent of s_v
+    float ev[kSub][2];
+#pragma unroll
+    for (int u = 0; u < kSub; ++u)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        ev[u][e] = (float)max((int)((__float_as_uint(vp[u][e].x) >> 23) & 255u) - 127, -24);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < kSub; ++u)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float x = fmaf(kp[u][e].x, s[u][nt][2 * e + c] * ra[nt][c], kp[u][e].y * rb[nt][c]);
+            if (!whole) {
+              const int t = t0 + 16 * u + g + 8 * e;
+              bool sees = base[u] >= 0 && t < length;
+              if (p.causal) sees &= t <= pos[nt][c];
+              if (p.window > 0) sees &= t > pos[nt][c] - p.window || t < p.sinks;
+              if (!sees) x = -INFINITY;
+            }
+            s[u][nt][2 * e + c] = x;
+            top = fmaxf(top, x + ev[u][e]);
+          }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+        if (top > m_run[nt][c]) {
+          const float alpha = exp2_fast(m_run[nt][c] - top);      // 0 while nothing was seen
+          m_run[nt][c] = top;
+          l_run[nt][c] *= alpha;
+          s_run[nt][c] *= alpha;
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            o[i][nt][c] *= alpha;
+            o[i][nt][2 + c] *= alpha;
+          }
+        }
+        const float ref = m_run[nt][c] == -INFINITY ? 0.0f : m_run[nt][c];
+#pragma unroll
+        for (int u = 0; u < kSub; ++u)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float x = s[u][nt][2 * e + c];
+            const float w = exp2_fast(x - ref);
+            l_run[nt][c] += w;
+            // a hidden token's scale and minimum may be anything: its weight of 0 must not meet them
+            s_run[nt][c] += x == -INFINITY ? 0.0f : w * vp[u][e].y;
+            s[u][nt][2 * e + c] = x == -INFINITY ? 0.0f : w * vp[u][e].x * 16384.0f;
+          }
+      }
+
+    // ---- output
+#pragma unroll
+    for (int u = 0; u < kSub; ++u) {
+      if (u > 0) load_values(u);
+      uint32_t b0[P][NT], b1[P][NT];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float* x = s[u][nt];
+        const uint32_t h0 = half_pair(x[0], x[1]), h1 = half_pair(x[2], x[3]);
+        b0[0][nt] = transpose8(h0);
+        b1[0][nt] = transpose8(h1);
+        if (P == 2) {
+          const float2 f0 = half_values(h0), f1 = half_values(h1);
+          b0[P - 1][nt] = transpose8(half_pair(x[0] - f0.x, x[1] - f0.y));
+          b1[P - 1][nt] = transpose8(half_pair(x[2] - f1.x, x[3] - f1.y));
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < VW; ++w)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t z0 = __byte_perm(vw[0][w], vw[1][w], h ? 0x7632 : 0x5410);
+          const uint32_t z1 = __byte_perm(vw[2][w], vw[3][w], h ? 0x7632 : 0x5410);
+#pragma unroll
+          for (int h2 = 0; h2 < 2; ++h2) {
+            const uint32_t y0 = h2 ? z0 >> 8 : z0, y1 = h2 ? z1 >> 8 : z1;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int pl = 0; pl < P; ++pl)
+                mma_f16(o[4 * w + 2 * h + h2][nt], y0 & 0x000f000fu, y0 & 0x00f000f0u, y1 & 0x000f000fu,
+                        y1 & 0x00f000f0u, b0[pl][nt], b1[pl][nt]);
+          }
+        }
+    }
+  }
+
+  // ---- the warps' results joined: numerators in units of 2^m
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int sh = 4; sh < 32; sh <<= 1) {
+        l_run[nt][c] += __shfl_xor_sync(0xffffffffu, l_run[nt][c], sh);
+        s_run[nt][c] += __shfl_xor_sync(0xffffffffu, s_run[nt][c], sh);
+      }
+  if (g == 0) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        join_m[warp][8 * nt + 2 * j + c] = m_run[nt][c];
+        join_l[warp][8 * nt + 2 * j + c] = l_run[nt][c];
+        join_s[warp][8 * nt + 2 * j + c] = s_run[nt][c];
+      }
+  }
+  __syncthreads();                                            // also: the query fragments are read
+  float* o_sh = reinterpret_cast<float*>(smem);               // [warp][row][D + 4]
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float* dst = o_sh + (size_t)(warp * R + 8 * nt + 2 * j + c) * (D + 4) + g * (D / 8) + 2 * i;
+        dst[0] = o[i][nt][c] * 1024.0f;                       // 2^24 / 2^14
+        dst[1] = o[i][nt][2 + c] * 64.0f;                     // codes of odd channels stood for 16 n
+      }
+  __syncthreads();
+  for (int idx = threadIdx.x; idx < rows_here * (D / 4); idx += kThreads) {
+    const int r = idx / (D / 4), c4 = idx % (D / 4) * 4;
+    float m = join_m[0][r];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) m = fmaxf(m, join_m[w][r]);
+    float l = 0.0f, acc[4] = {};
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = join_m[w][r] == -INFINITY ? 0.0f : exp2_fast(join_m[w][r] - m);
+      const float4 v = *reinterpret_cast<const float4*>(o_sh + (size_t)(w * R + r) * (D + 4) + c4);
+      const float ms = join_s[w][r];
+      l = fmaf(f, join_l[w][r], l);
+      acc[0] = fmaf(f, v.x + ms, acc[0]);
+      acc[1] = fmaf(f, v.y + ms, acc[1]);
+      acc[2] = fmaf(f, v.z + ms, acc[2]);
+      acc[3] = fmaf(f, v.w + ms, acc[3]);
+    }
+    const int rr = row0 + r;
+    const int64_t out_row = ((int64_t)b * p.count + rr / p.group) * p.heads + head * p.group + rr % p.group;
+    if (p.splits == 1) {
+      const float inv = l != 0.0f ? 1.0f / l : 0.0f;          // a row that sees nothing is 0
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] *= inv;
+      store_f32<T, 4>(static_cast<T*>(p.out) + out_row * D + c4, acc);
+    } else {
+      const int64_t at = split * p.rows + out_row;
+      store_f32<float, 4>(p.part + at * D + c4, acc);
+      if (c4 == 0) {
+        float* lm = p.part + (int64_t)p.splits * p.rows * D;
+        lm[at] = l;
+        lm[(int64_t)p.splits * p.rows + at] = m;
+      }
+    }
+  }
+}
+
+// The splits' partial results joined, in order; a thread owns four channels of a row.
+template <typename T>
+__global__ void __launch_bounds__(256)
+kv4_join_kernel(const float* __restrict__ part, T* __restrict__ out, int64_t rows, int dim, int splits) {
+  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int chunks = dim / 4;
+  if (idx >= rows * chunks) return;
+  const int64_t row = idx / chunks;
+  const int c4 = (int)(idx % chunks) * 4;
+  const float* l_at = part + (int64_t)splits * rows * dim + row;
+  const float* m_at = l_at + (int64_t)splits * rows;
+  float m = -INFINITY;
+  for (int s = 0; s < splits; ++s) m = fmaxf(m, m_at[s * rows]);
+  float l = 0.0f, acc[4] = {};
+  for (int s = 0; s < splits; ++s) {
+    const float ms = m_at[s * rows];
+    if (ms == -INFINITY) {
+      // nothing seen, or only scores that are not numbers: the sum says which
+      l += l_at[s * rows];
+      continue;
+    }
+    const float f = exp2_fast(ms - m);
+    float v[4];
+    load_f32<float, 4>(part + (s * rows + row) * dim + c4, v);
+    l = fmaf(f, l_at[s * rows], l);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] = fmaf(f, v[e], acc[e]);
+  }
+  const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) acc[e] *= inv;
+  store_f32<T, 4>(out + row * dim + c4, acc);
+}
+
+// Blocks per sequence and key head: enough to give every SM several, at least two tiles of a block's
+// warps each.  The lengths are on the device, so the table's width stands for the longest.
+int splits_for(int64_t blocks, int max_tokens) {
+  const int64_t want = ceil_div64(4ll * device_sms(), blocks);
+  const int64_t most = ceil_div64(max_tokens, 2 * kTile * kWarps);
+  const int64_t s = want < most ? want : most;
+  return (int)(s < 1 ? 1 : (s > 64 ? 64 : s));
+}
+
+int row_block(int rows, int dim) { return rows <= 8 ? 1 : (rows <= 16 || dim > 128 ? 2 : 4); }
+
+struct Plan {
+  int nt, row_tiles, splits;
+  int64_t blocks;
+};
+Plan plan_of(const modiff_kv4_cache* c, int batch, int count, int heads, int max_pages, int window, int sinks) {
+  Plan pl;
+  const int rows = count * (heads / c->heads);
+  pl.nt = row_block(rows, c->dim);
+  pl.row_tiles = ceil_div(rows, 8 * pl.nt);
+  const int64_t units = (int64_t)batch * c->heads * pl.row_tiles;
+  int64_t tokens = (int64_t)max_pages * c->page_size;
+  if (window > 0 && (int64_t)window + sinks + 8 * pl.nt < tokens) tokens = (int64_t)window + sinks + 8 * pl.nt;
+  pl.splits = splits_for(units, (int)tokens);
+  pl.blocks = units * pl.splits;
+  return pl;
+}
+
+template <typename T, int D, int NT>
+int launch_attention(const AttnParams& p, int64_t blocks, cudaStream_t s) {
+  constexpr int smem = smem_bytes<T, D, NT>();
+  static SmemLimit limit;
+  MODIFF_CUDA(raise_smem_limit(kv4_attention_kernel<T, D, NT>, smem, limit));
+  kv4_attention_kernel<T, D, NT><<<(unsigned)blocks, kThreads, smem, s>>>(p);
+  MODIFF_LAUNCH_CHECK("kv4_attention_kernel");
+  if (p.splits > 1) {
+    const int64_t n = ceil_div64(p.rows * (D / 4), 256);
+    kv4_join_kernel<T><<<(unsigned)n, 256, 0, s>>>(p.part, static_cast<T*>(p.out), p.rows, D, p.splits);
+    MODIFF_LAUNCH_CHECK("kv4_join_kernel");
+  }
+  return MODIFF_OK;
+}
+
+template <typename T, int D>
+int by_rows(const AttnParams& p, const Plan& pl, cudaStream_t s) {
+  if (pl.nt == 1) return launch_attention<T, D, 1>(p, pl.blocks, s);
+  if (pl.nt == 2) return launch_attention<T, D, 2>(p, pl.blocks, s);
+  if constexpr (D <= 128) return launch_attention<T, D, 4>(p, pl.blocks, s);
+  return MODIFF_ERR_INVALID;
+}
+
+int check_shape(const modiff_kv4_cache* c, int batch, int count, int heads) {
+  MODIFF_CHECK_ARG(batch >= 0 && count >= 0 && heads > 0, "bad shape");
+  MODIFF_CHECK_ARG(heads % c->heads == 0, "%d query heads for %d key heads", heads, c->heads);
+  MODIFF_CHECK_ARG((int64_t)count * heads <= 0x3fffffff, "too many query rows");
+  return MODIFF_OK;
+}
+
+}  // namespace
+}  // namespace modiff
+
+using namespace modiff;
+
+extern "C" int64_t modiff_kv4_attention_bytes(const modiff_kv4_cache* cache, int batch, int count, int heads,
+                                              int max_pages, int window, int sinks) {
+  if (!cache || cache->heads <= 0 || batch <= 0 || count <= 0 || check_shape(cache, batch, count, heads)) return 0;
+  const Plan pl = plan_of(cache, batch, count, heads, max_pages, window, sinks);
+  if (pl.splits == 1) return 0;
+  return 4ll * pl.splits * batch * count * heads * (cache->dim + 2);
+}
+
+extern "C" int modiff_kv4_attention(const void* q, const int64_t* q_strides, const modiff_kv4_cache* cache,
+                                    const int32_t* table, const int32_t* lengths, void* out, int batch, int count,
+                                    int heads, int max_pages, float scale, int causal, int window, int sinks,
+                                    int dtype, void* workspace, void* stream) {
+  int rc = kv4_check(cache, table, lengths, batch, max_pages);
+  if (rc) return rc;
+  rc = check_shape(cache, batch, count, heads);
+  if (rc) return rc;
+  MODIFF_CHECK_ARG(dtype_ok(dtype), "unknown element type %d", dtype);
+  MODIFF_CHECK_ARG(window >= 0 && sinks >= 0, "negative window or sinks");
+  MODIFF_CHECK_ARG(causal || window == 0, "a window needs causal positions");
+  if (batch == 0 || count == 0) return MODIFF_OK;
+  MODIFF_CHECK_ARG(q && q_strides && out, "NULL pointer argument");
+  const int size = dtype_bytes(dtype);
+  MODIFF_CHECK_ARG((uintptr_t)q % size == 0 && (uintptr_t)out % 16 == 0, "misaligned tensor");
+  const Plan pl = plan_of(cache, batch, count, heads, max_pages, window, sinks);
+  MODIFF_CHECK_ARG(pl.blocks <= 0x7fffffff, "too many query rows");
+  MODIFF_CHECK_ARG(pl.splits == 1 || (workspace && (uintptr_t)workspace % 16 == 0), "NULL or misaligned workspace");
+  AttnParams p;
+  p.q = q;
+  p.qb = q_strides[0]; p.qt = q_strides[1]; p.qh = q_strides[2];
+  p.out = out;
+  p.part = static_cast<float*>(workspace);
+  p.c = kv4_pages(cache);
+  p.table = table; p.lengths = lengths;
+  p.batch = batch; p.count = count; p.heads = heads; p.group = heads / cache->heads;
+  p.max_pages = max_pages;
+  p.splits = pl.splits; p.row_tiles = pl.row_tiles;
+  // positions and windows are subtracted in 32 bits; none of the cache's tokens is 2^30 back
+  constexpr int kFar = 1 << 30;
+  p.causal = causal;
+  p.window = window < kFar ? window : kFar;
+  p.sinks = sinks < kFar ? sinks : kFar;
+  p.scale2 = scale * kLog2e;
+  p.rows = (int64_t)batch * count * heads;
+  cudaStream_t st = (cudaStream_t)stream;
+  return with_dtype(dtype, [&](auto tag) {
+    using T = decltype(tag);
+    switch (cache->dim) {
+      case 64: return by_rows<T, 64>(p, pl, st);
+      case 128: return by_rows<T, 128>(p, pl, st);
+      case 192: return by_rows<T, 192>(p, pl, st);
+      default: return by_rows<T, 256>(p, pl, st);
+    }
+  });
+}

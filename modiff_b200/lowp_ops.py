@@ -1,0 +1,364 @@
+"""Operators of a transformer served in low precision: linear layers in 8-bit floating point with one
+scale per block of 128, norms of queries and keys with the rotation of their positions, and attention
+over a paged cache of keys and values held in 4 bits.
+
+Tensors are CUDA tensors of fp32, fp16 or bf16, all of a call on one device; a call is enqueued on that
+device's current stream.  Sums, statistics and softmax are fp32, the result is rounded once.  There is no
+backward pass: inputs that ask for gradients are refused while gradients are recorded.
+"""
+import ctypes as C
+from typing import NamedTuple
+
+import torch
+
+from . import _lib
+from ._lib import ModiffError
+
+FP8_BLOCK = 128
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _check(name, x, *others):
+    """`x` and `others` (None allowed) are CUDA tensors of one device, none of which needs gradients."""
+    for t in (x,) + others:
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise ModiffError(f"{name}: every tensor must be a CUDA tensor (there is no CPU fallback)")
+        if t.device != x.device:
+            raise ModiffError(f"{name}: tensors on {x.device} and {t.device}")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ModiffError(f"{name} has no backward pass: call it under torch.no_grad() or detach its inputs")
+
+
+def _dtype(name, x):
+    if x.dtype not in _DTYPES:
+        raise ModiffError(f"{name}: fp32, fp16 or bf16 tensors, got {x.dtype}")
+    return _DTYPES[x.dtype]
+
+
+def _call(device, entry, *args, **kw):
+    """One entry point on `device`'s current stream, whatever the current device is."""
+    if device.index == torch.cuda.current_device():
+        _lib.call(entry, *args, torch.cuda.current_stream(device).cuda_stream, **kw)
+    else:
+        with torch.cuda.device(device):
+            _lib.call(entry, *args, torch.cuda.current_stream(device).cuda_stream, **kw)
+
+
+def _i64(*v):
+    return (C.c_int64 * len(v))(*v)
+
+
+# ------------------------------------------------------------------------------- 8-bit linear layers
+class Fp8Rows(NamedTuple):
+    """Rows quantised by `fp8_quantize`: e4m3 codes [..., k] (row pitch a multiple of 16), fp32 scales
+    [..., ceil(k / 128)] and the type of the rows, which is the type of the layers' outputs."""
+    codes: torch.Tensor
+    scale: torch.Tensor
+    dtype: torch.dtype
+
+
+def fp8_quantize(x):
+    """x [..., k] -> `Fp8Rows`: per row and block of 128 channels scale = max|x| / 448 (1 where that is
+    0) and codes e4m3(x / scale).  Quantise once what several layers read."""
+    _check("fp8_quantize", x)
+    dt = _dtype("fp8_quantize", x)
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ModiffError(f"fp8_quantize: rows of at least one channel, got shape {tuple(x.shape)}")
+    k = x.shape[-1]
+    rows = x.numel() // k
+    x2 = x.reshape(rows, k)
+    if x2.stride(1) != 1 and k > 1:
+        x2 = x2.contiguous()
+    blocks = -(-k // FP8_BLOCK)
+    kp = -(-k // 16) * 16
+    lead = tuple(x.shape[:-1])
+    codes = torch.empty(lead + (kp,), dtype=torch.float8_e4m3fn, device=x.device)
+    scale = torch.empty(lead + (blocks,), dtype=torch.float32, device=x.device)
+    if rows:
+        _call(x.device, 'modiff_fp8_quantize', x2.data_ptr(), x2.stride(0), rows, k, dt, codes.data_ptr(), kp,
+              scale.data_ptr(), blocks, nbytes=rows * (k * x.element_size() + kp + 4 * blocks))
+    return Fp8Rows(codes[..., :k], scale, x.dtype)
+
+
+def fp8_pack_weight(w):
+    """A weight matrix [n, k] -> (e4m3 codes [n, k] with a row pitch of a multiple of 16, fp32 scales
+    [ceil(n / 128), ceil(k / 128)]), one scale per 128 x 128 block.  Once per weight version."""
+    _check("fp8_pack_weight", w.detach() if isinstance(w, torch.Tensor) else w)
+    dt = _dtype("fp8_pack_weight", w)
+    if w.dim() != 2 or w.numel() == 0:
+        raise ModiffError(f"fp8_pack_weight: a matrix [n, k], got shape {tuple(w.shape)}")
+    w = w.detach()
+    n, k = w.shape
+    if w.stride(1) != 1 and k > 1:
+        w = w.contiguous()
+    kp = -(-k // 16) * 16
+    codes = torch.empty((n, kp), dtype=torch.float8_e4m3fn, device=w.device)
+    scale = torch.empty((-(-n // FP8_BLOCK), -(-k // FP8_BLOCK)), dtype=torch.float32, device=w.device)
+    _call(w.device, 'modiff_fp8_pack_weight', w.data_ptr(), w.stride(0), n, k, dt, codes.data_ptr(), kp,
+          scale.data_ptr(), scale.shape[1], nbytes=n * (k * w.element_size() + kp))
+    return codes[:, :k], scale
+
+
+def _fp8_weight(w, w_scale, device):
+    if w.dtype != torch.float8_e4m3fn or w.dim() != 2 or w.numel() == 0:
+        raise ModiffError("fp8_linear: weight codes are a float8_e4m3fn matrix [n, k] (fp8_pack_weight)")
+    n, k = w.shape
+    pitch = w.stride(0) if n > 1 else -(-k // 16) * 16
+    if (w.stride(1) != 1 and k > 1) or pitch % 16 or pitch < k or w.data_ptr() % 16:
+        raise ModiffError("fp8_linear: weight rows start at multiples of 16 bytes (fp8_pack_weight lays them "
+                          f"out so); got strides {tuple(w.stride())} for {k} channels")
+    want = (-(-n // FP8_BLOCK), -(-k // FP8_BLOCK))
+    if w_scale.dtype != torch.float32 or tuple(w_scale.shape) != want:
+        raise ModiffError(f"fp8_linear: fp32 weight scales of shape {want}, got {w_scale.dtype} "
+                          f"{tuple(w_scale.shape)}")
+    if not w_scale.is_contiguous():
+        w_scale = w_scale.contiguous()
+    return n, k, pitch, w_scale
+
+
+def fp8_linear(x, w, w_scale, bias=None):
+    """y = x w^T (+ bias) with x (a tensor [..., k], or `Fp8Rows`) and w (`fp8_pack_weight`) as 8-bit
+    floating-point codes with one scale per block of 128 channels (and 128 weight rows).  y [..., n] and
+    bias have the type of x."""
+    if not isinstance(x, Fp8Rows):
+        _check("fp8_linear", x, w, w_scale, bias)
+        if x.dim() < 1 or x.shape[-1] != w.shape[-1]:
+            raise ModiffError(f"fp8_linear: rows of shape {tuple(x.shape)} for weights {tuple(w.shape)}")
+        x = fp8_quantize(x)
+    else:
+        _check("fp8_linear", x.codes, x.scale, w, w_scale, bias)
+    codes, scale, dtype = x
+    n, k, w_pitch, w_scale = _fp8_weight(w, w_scale, codes.device)
+    if codes.dtype != torch.float8_e4m3fn or codes.shape[-1] != k:
+        raise ModiffError(f"fp8_linear: rows of {codes.shape[-1]} channels for weights {tuple(w.shape)}")
+    dt = _DTYPES.get(dtype)
+    if dt is None:
+        raise ModiffError(f"fp8_linear: outputs of fp32, fp16 or bf16, got {dtype}")
+    if bias is not None and (bias.dtype != dtype or tuple(bias.shape) != (n,)):
+        raise ModiffError(f"fp8_linear: bias of {n} values of {dtype}, got {tuple(bias.shape)} {bias.dtype}")
+    lead = codes.shape[:-1]
+    rows = lead.numel()
+    blocks = -(-k // FP8_BLOCK)
+    kp = -(-k // 16) * 16
+    if scale.dtype != torch.float32 or tuple(scale.shape) != tuple(lead) + (blocks,):
+        raise ModiffError(f"fp8_linear: fp32 scales of shape {tuple(lead) + (blocks,)}, got {tuple(scale.shape)}")
+    if rows and (codes.data_ptr() % 16 or not scale.is_contiguous() or not _pitched(codes, kp)):
+        raise ModiffError("fp8_linear: rows of codes as fp8_quantize lays them out")
+    y = torch.empty(tuple(lead) + (n,), dtype=dtype, device=codes.device)
+    if rows > 0x7fffffff:
+        raise ModiffError("fp8_linear: too many rows")
+    if rows:
+        if bias is not None and n > 1 and bias.stride(0) != 1:
+            bias = bias.contiguous()
+        _call(codes.device, 'modiff_fp8_linear', codes.data_ptr(), kp, scale.data_ptr(), blocks, w.data_ptr(), w_pitch,
+              w_scale.data_ptr(), blocks, _lib.ptr(bias), y.data_ptr(), n, rows, k, n, dt,
+              nbytes=rows * kp + n * k + y.numel() * y.element_size(), nops=2 * rows * n * k)
+    return y
+
+
+def _pitched(codes, pitch):
+    """Whether the leading dimensions of `codes` walk rows of `pitch` bytes without a gap."""
+    want = pitch
+    if codes.shape[-1] > 1 and codes.stride(-1) != 1:
+        return False
+    for d in range(codes.dim() - 2, -1, -1):
+        if codes.shape[d] > 1 and codes.stride(d) != want:
+            return False
+        want *= codes.shape[d]
+    return True
+
+
+# --------------------------------------------------------------------- norms of queries and keys
+def _tokens(name, x):
+    """[..., heads, d] as [tokens, heads, d] with the channels contiguous (a copy only if it must be)."""
+    if x.dim() < 3:
+        raise ModiffError(f"{name}: tensors [..., heads, d], got shape {tuple(x.shape)}")
+    x = x if x.dim() == 3 else x.flatten(0, -3)
+    return x if x.stride(2) == 1 or x.shape[2] == 1 else x.contiguous()
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6, interleaved=False, out=None):
+    """Root-mean-square norm of every head of q [..., heads, d] and k [..., kv_heads, d] (k may be None),
+    times the weights fp32 [d] (None: ones), and the rotation of the first 2 * cos.shape[1] channels by
+    the angles in row `positions` (int32 / int64, one per token; None: the token's own number) of the
+    fp32 tables cos and sin, one pass over both.  Pairs are (i, half + i), or (2i, 2i + 1) with
+    `interleaved`.  q and k may be slices of one projection; `out` = (q, k) writes in place.  A position
+    outside the tables gives a row of NaN.  Returns (q', k')."""
+    name = "qk_norm_rope"
+    _check(name, q, k, q_weight, k_weight, cos, sin, positions, *(out or ()))
+    dt = _dtype(name, q)
+    d = q.shape[-1]
+    if k is not None and (k.dtype != q.dtype or k.shape[-1] != d or k.shape[:-2] != q.shape[:-2]):
+        raise ModiffError(f"{name}: q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} differ in more "
+                          "than their heads")
+    if d % 2 or not 2 <= d <= 256:
+        raise ModiffError(f"{name}: heads of an even number of channels up to 256, got {d}")
+    for w in (q_weight, k_weight):
+        if w is not None and (w.dtype != torch.float32 or tuple(w.shape) != (d,) or not w.is_contiguous()):
+            raise ModiffError(f"{name}: contiguous fp32 weights of {d} values, got {tuple(w.shape)} {w.dtype}")
+    if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2 or cos.shape != sin.shape
+            or 2 * cos.shape[1] > d):
+        raise ModiffError(f"{name}: fp32 tables [rows, at most {d // 2}], got {tuple(cos.shape)} and "
+                          f"{tuple(sin.shape)}")
+    cos, sin = cos.contiguous(), sin.contiguous()
+    q3 = _tokens(name, q)
+    k3 = None if k is None else _tokens(name, k)
+    n = q3.shape[0]
+    wide = 0
+    if positions is not None:
+        if positions.dtype not in (torch.int32, torch.int64) or positions.numel() != n:
+            raise ModiffError(f"{name}: {n} positions of int32 or int64, got {tuple(positions.shape)} "
+                              f"{positions.dtype}")
+        positions = positions.contiguous()
+        wide = int(positions.dtype == torch.int64)
+    elif cos.shape[1] and cos.shape[0] < n:
+        raise ModiffError(f"{name}: tables of {cos.shape[0]} rows for {n} tokens")
+    if out is None:
+        outs = (torch.empty(q.shape, dtype=q.dtype, device=q.device),
+                None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device))
+    else:
+        outs = tuple(out)
+        if len(outs) != 2 or (outs[1] is None) != (k is None):
+            raise ModiffError(f"{name}: out is a pair like (q, k)")
+        for o, x in zip(outs, (q, k)):
+            if o is not None and (o.shape != x.shape or o.dtype != x.dtype):
+                raise ModiffError(f"{name}: out {tuple(o.shape)} {o.dtype} for {tuple(x.shape)} {x.dtype}")
+    flat = []
+    for o in outs:
+        if o is None:
+            flat.append(None)
+            continue
+        f = o if o.dim() == 3 else o.flatten(0, -3)
+        if (f.stride(2) != 1 and d > 1) or f.data_ptr() != o.data_ptr():
+            raise ModiffError(f"{name}: out needs contiguous channels and leading dimensions that merge")
+        flat.append(f)
+    if n:
+        args = []
+        for x, o in ((q3, flat[0]), (k3, flat[1])):
+            if x is None:
+                args += [None, None, None, None, 0]
+            else:
+                args += [x.data_ptr(), _i64(x.stride(0), x.stride(1)), o.data_ptr(), _i64(o.stride(0), o.stride(1)),
+                         x.shape[1]]
+        heads = q3.shape[1] + (0 if k3 is None else k3.shape[1])
+        _call(q.device, 'modiff_qk_norm_rope', *args, _lib.ptr(q_weight), _lib.ptr(k_weight), cos.data_ptr(),
+              sin.data_ptr(), cos.shape[0], _lib.ptr(positions), wide, n, d, 2 * cos.shape[1], int(bool(interleaved)),
+              float(eps), dt, nbytes=2 * n * heads * d * q.element_size())
+    return outs
+
+
+# ------------------------------------------------------------------------------ the 4-bit cache
+class KV4Cache(NamedTuple):
+    """A paged cache of keys and values in 4 bits (`kv4_cache` makes an empty one): codes uint8 [pages,
+    kv_heads, page_size, d / 2], channel 2i in the low half of byte i, and fp16 (scale, minimum) [pages,
+    kv_heads, page_size, 2].  A token's value of channel c is scale * code[c] + minimum."""
+    k_codes: torch.Tensor
+    k_params: torch.Tensor
+    v_codes: torch.Tensor
+    v_params: torch.Tensor
+
+
+def kv4_cache(pages, kv_heads, page_size, head_dim, device):
+    """An empty `KV4Cache`.  page_size is a multiple of 16, head_dim 64, 128, 192 or 256; a token takes
+    head_dim + 8 bytes per head."""
+    if pages < 1 or kv_heads < 1 or page_size < 16 or page_size % 16 or head_dim not in (64, 128, 192, 256):
+        raise ModiffError(f"kv4_cache: {pages} pages of {page_size} tokens (a multiple of 16), {kv_heads} heads of "
+                          f"{head_dim} channels (64, 128, 192 or 256)")
+    shape = (pages, kv_heads, page_size)
+    codes = [torch.zeros(shape + (head_dim // 2,), dtype=torch.uint8, device=device) for _ in range(2)]
+    params = [torch.zeros(shape + (2,), dtype=torch.float16, device=device) for _ in range(2)]
+    return KV4Cache(codes[0], params[0], codes[1], params[1])
+
+
+def _cache(name, cache, table, lengths):
+    kc, kp, vc, vp = cache
+    if (kc.dim() != 4 or kc.dtype != torch.uint8 or vc.dtype != torch.uint8 or kc.shape != vc.shape
+            or kp.dtype != torch.float16 or vp.dtype != torch.float16 or kp.shape != vp.shape
+            or kp.shape != kc.shape[:3] + (2,)
+            or not (kc.is_contiguous() and vc.is_contiguous() and kp.is_contiguous() and vp.is_contiguous())):
+        raise ModiffError(f"{name}: a cache is contiguous uint8 codes [pages, heads, page_size, d / 2] and fp16 "
+                          f"[pages, heads, page_size, 2], got {tuple(kc.shape)} {kc.dtype}, {tuple(kp.shape)} {kp.dtype}")
+    if (table.dim() != 2 or table.dtype != torch.int32 or lengths.dtype != torch.int32
+            or tuple(lengths.shape) != (table.shape[0],) or table.shape[1] == 0):
+        raise ModiffError(f"{name}: int32 table [batch, pages] and lengths [batch], got {tuple(table.shape)} "
+                          f"{table.dtype} and {tuple(lengths.shape)} {lengths.dtype}")
+    pages, heads, size, half = kc.shape
+    return (_lib.Kv4CacheStruct(kc.data_ptr(), vc.data_ptr(), kp.data_ptr(), vp.data_ptr(), pages, heads, size,
+                                2 * half), table.contiguous(), lengths.contiguous())
+
+
+def kv4_append(cache, k, v, table, lengths):
+    """Writes k and v [batch, n, kv_heads, d] as the last n positions of every sequence: token i of
+    sequence b at position lengths[b] - n + i, i.e. at that offset of the pages `table`[b] names.
+    `lengths` counts the new tokens; positions below 0 (shorter sequences of a padded batch) and page
+    numbers outside the cache are skipped.  No two sequences may name the same place."""
+    name = "kv4_append"
+    _check(name, k, v, table, lengths, *cache)
+    c, table, lengths = _cache(name, cache, table, lengths)
+    dt = _dtype(name, k)
+    b = table.shape[0]
+    if (k.dim() != 4 or k.shape != v.shape or v.dtype != k.dtype or k.shape[0] != b or k.shape[2] != c.heads
+            or k.shape[3] != c.dim):
+        raise ModiffError(f"{name}: k and v [{b}, n, {c.heads}, {c.dim}] of one type, got {tuple(k.shape)} {k.dtype} "
+                          f"and {tuple(v.shape)} {v.dtype}")
+    if k.stride(3) != 1:
+        k = k.contiguous()
+    if v.stride(3) != 1:
+        v = v.contiguous()
+    if k.numel():
+        _call(k.device, 'modiff_kv4_append', C.byref(c), k.data_ptr(), _i64(*k.stride()[:3]), v.data_ptr(),
+              _i64(*v.stride()[:3]), table.data_ptr(), lengths.data_ptr(), b, k.shape[1], table.shape[1], dt,
+              nbytes=2 * k.numel() * k.element_size() + k.numel() // c.dim * 2 * (c.dim // 2 + 4))
+
+
+def kv4_read(cache, table, lengths, n, dtype=torch.float32):
+    """The last n positions of every sequence as values: (k, v) [batch, n, kv_heads, d], zeros for
+    positions below 0 and pages outside the cache."""
+    name = "kv4_read"
+    _check(name, table, lengths, *cache)
+    c, table, lengths = _cache(name, cache, table, lengths)
+    if dtype not in _DTYPES or n < 0:
+        raise ModiffError(f"{name}: n >= 0 tokens as fp32, fp16 or bf16, got {n} and {dtype}")
+    b = table.shape[0]
+    k = torch.empty((b, n, c.heads, c.dim), dtype=dtype, device=table.device)
+    v = torch.empty_like(k)
+    if k.numel():
+        _call(table.device, 'modiff_kv4_read', C.byref(c), table.data_ptr(), lengths.data_ptr(), b, n, table.shape[1],
+              k.data_ptr(), v.data_ptr(), _DTYPES[dtype],
+              nbytes=2 * k.numel() * k.element_size() + k.numel() // c.dim * 2 * (c.dim // 2 + 4))
+    return k, v
+
+
+def kv4_attention(q, cache, table, lengths, scale=None, causal=True, window=0, sinks=0):
+    """Attention of q [batch, n, heads, d] over the cached tokens of every sequence:
+    out[b, i, h] = sum_t softmax_t(scale * q[b, i, h] . k_t) v_t; `heads` is a multiple of the cache's
+    heads, which consecutive query heads share.  Query i of sequence b stands at position
+    lengths[b] - n + i and sees the positions up to its own; with `window` > 0 only the last `window` of
+    them and the first `sinks` of the sequence (tokens outside are not read).  causal=False: every query
+    sees all lengths[b] tokens.  A row that sees nothing is 0.  scale defaults to d ** -0.5."""
+    name = "kv4_attention"
+    _check(name, q, table, lengths, *cache)
+    c, table, lengths = _cache(name, cache, table, lengths)
+    dt = _dtype(name, q)
+    b = table.shape[0]
+    if q.dim() != 4 or q.shape[0] != b or q.shape[3] != c.dim or q.shape[2] == 0 or q.shape[2] % c.heads:
+        raise ModiffError(f"{name}: q [{b}, n, a multiple of {c.heads}, {c.dim}], got {tuple(q.shape)}")
+    window, sinks = int(window), int(sinks)
+    if window < 0 or sinks < 0 or (window and not causal) or (sinks and not window):
+        raise ModiffError(f"{name}: window {window} and sinks {sinks}: a window needs causal positions, sinks need "
+                          "a window")
+    if q.stride(3) != 1:
+        q = q.contiguous()
+    n, heads = q.shape[1], q.shape[2]
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if out.numel():
+        window, sinks = min(window, 1 << 30), min(sinks, 1 << 30)
+        size = _lib.lib().modiff_kv4_attention_bytes(C.byref(c), b, n, heads, table.shape[1], window, sinks)
+        work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+        scale = float(scale) if scale is not None else c.dim ** -0.5
+        _call(q.device, 'modiff_kv4_attention', q.data_ptr(), _i64(*q.stride()[:3]), C.byref(c), table.data_ptr(),
+              lengths.data_ptr(), out.data_ptr(), b, n, heads, table.shape[1], scale, int(bool(causal)), window, sinks,
+              dt, _lib.ptr(work))
+    return out

@@ -553,3 +553,8 @@ def int8_attention_bits(quantizer, what):
         raise ModiffError(f"int8 attention needs symmetric per-tensor {what} quantisers "
                           "(build the model with symmetric activation parameters, --a_sym)")
     return int(quantizer.n_bits)
+
+
+# operators of a transformer served in low precision
+from .lowp_ops import (Fp8Rows, KV4Cache, fp8_linear, fp8_pack_weight, fp8_quantize,  # noqa: E402,F401
+                       kv4_append, kv4_attention, kv4_cache, kv4_read, qk_norm_rope)
