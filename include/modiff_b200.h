@@ -643,10 +643,13 @@ int modiff_attention_i8(const int8_t* q_codes, const int8_t* k_codes, const int8
 
 /* Linear layer in 8-bit floating point (e4m3), one fp32 scale per block of 128 channels:
  *   modiff_fp8_quantize     rows x [rows][k] -> codes [rows][code_pitch] (zeros from k to the pitch),
- *                           scale [rows][scale_pitch >= ceil(k / 128)] = max|x| / 448 of the block, 1
- *                           where that is 0; code = e4m3(x / scale).  code_pitch a multiple of 16
+ *                           scale [ceil(k / 128)][scale_pitch >= rows, a multiple of 4] = max|x| * (1.0f / 448.0f) of the
+ *                           block, 1 where that is 0; code = e4m3(x / scale).  code_pitch a multiple of 16
  *   modiff_fp8_pack_weight  w [n][k] -> codes [n][round_up(k, 16)], scale [ceil(n/128)][ceil(k/128)]
- *   modiff_fp8_linear       y[m][n] = sum over blocks of scale[m][b] * w_scale[n / 128][b] *
+ *   modiff_fp8_linear_x     quantises rows x of type dtype and multiplies them: one launch for a few
+ *                           rows, else through `workspace` (modiff_fp8_linear_bytes; NULL if that is
+ *                           0), which calls that overlap must not share
+ *   modiff_fp8_linear       y[m][n] = sum over blocks of scale[b][m] * w_scale[n / 128][b] *
  *                           sum(code * w code) + bias[n]; bias (NULL: none) and y of type dtype */
 int modiff_fp8_quantize(const void* x, int64_t x_pitch, int64_t rows, int k, int dtype, uint8_t* codes,
                         int64_t code_pitch, float* scale, int64_t scale_pitch, void* stream);
@@ -657,20 +660,25 @@ int modiff_fp8_linear(const uint8_t* codes, int64_t code_pitch, const float* sca
                       const void* bias, void* y, int64_t y_pitch, int rows, int k, int n, int dtype,
                       void* stream);
 
+int64_t modiff_fp8_linear_bytes(int rows, int k, int n);
+int modiff_fp8_linear_x(const void* x, int64_t x_pitch, const uint8_t* w, int64_t w_pitch,
+                        const float* w_scale, int64_t w_scale_pitch, const void* bias, void* y,
+                        int64_t y_pitch, int rows, int k, int n, int dtype, void* workspace, void* stream);
+
 /* Root-mean-square norm of every head of q and k (weights fp32 [d], NULL: ones) and the rotation of the
  * first `rot` channels by row `positions[token]` (NULL: `token`) of cos / sin fp32 [table_rows][rot / 2],
  * in one pass.  Pairs are (i, rot / 2 + i), or (2i, 2i + 1) if `interleaved`.  q, k and the outputs are
- * addressed as x[token * s0 + head * s1 + channel] (strides: two int64 on the host); an output may be its
+ * addressed as x[token * s0 + head * s1 + channel] with the two strides behind each pointer; an output may be its
  * input.  A position outside the tables gives a row of NaN.  d even, at most 256. */
-int modiff_qk_norm_rope(const void* q, const int64_t* q_strides, void* q_out, const int64_t* q_out_strides,
-                        int q_heads, const void* k, const int64_t* k_strides, void* k_out,
-                        const int64_t* k_out_strides, int k_heads, const float* q_weight,
-                        const float* k_weight, const float* cos, const float* sin, int64_t table_rows,
+int modiff_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, void* q_out, int64_t q_out_token,
+                        int64_t q_out_head, int q_heads, const void* k, int64_t k_token, int64_t k_head,
+                        void* k_out, int64_t k_out_token, int64_t k_out_head, int k_heads,
+                        const float* q_weight, const float* k_weight, const float* cos, const float* sin, int64_t table_rows,
                         const void* positions, int positions64, int64_t tokens, int d, int rot,
                         int interleaved, float eps, int dtype, void* stream);
 
 /* Cache of keys and values in 4 bits, in pages.  A token's channels of one head have m = fp16(min),
- * s = fp16((max - min) / 15) and the codes round((x - m) / s) in 0 .. 15.
+ * s = fp16((max - min) * (1.0f / 15.0f)) and the codes round((x - m) / s) in 0 .. 15.
  *   codes   uint8 [pages][heads][page_size][dim / 2], channel 2i in the low half of byte i
  *   params  fp16 [pages][heads][page_size][2] = (s, m)
  * page_size a multiple of 16; dim 64, 128, 192 or 256.  Position t of sequence b is at offset
@@ -690,15 +698,16 @@ typedef struct modiff_kv4_cache {
   uint16_t *k_params, *v_params;
   int32_t pages, heads, page_size, dim;
 } modiff_kv4_cache;
-int modiff_kv4_append(const modiff_kv4_cache* cache, const void* k, const int64_t* k_strides, const void* v,
-                      const int64_t* v_strides, const int32_t* table, const int32_t* lengths, int batch,
-                      int count, int max_pages, int dtype, void* stream);
+int modiff_kv4_append(const modiff_kv4_cache* cache, const void* k, int64_t k_seq, int64_t k_token,
+                      int64_t k_head, const void* v, int64_t v_seq, int64_t v_token, int64_t v_head,
+                      const int32_t* table, const int32_t* lengths, int batch, int count, int max_pages,
+                      int dtype, void* stream);
 int modiff_kv4_read(const modiff_kv4_cache* cache, const int32_t* table, const int32_t* lengths, int batch,
                     int count, int max_pages, void* k, void* v, int dtype, void* stream);
 int64_t modiff_kv4_attention_bytes(const modiff_kv4_cache* cache, int batch, int count, int heads,
                                    int max_pages, int window, int sinks);
-int modiff_kv4_attention(const void* q, const int64_t* q_strides, const modiff_kv4_cache* cache,
-                         const int32_t* table, const int32_t* lengths, void* out, int batch, int count,
+int modiff_kv4_attention(const void* q, int64_t q_seq, int64_t q_token, int64_t q_head,
+                         const modiff_kv4_cache* cache, const int32_t* table, const int32_t* lengths, void* out, int batch, int count,
                          int heads, int max_pages, float scale, int causal, int window, int sinks,
                          int dtype, void* workspace, void* stream);
 

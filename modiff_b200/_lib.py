@@ -158,13 +158,18 @@ SIGNATURES = {
                                          C.c_int64, _P]),
     "modiff_fp8_linear": (C.c_int, [_P, C.c_int64, _P, C.c_int64, _P, C.c_int64, _P, C.c_int64, _P, _P,
                                     C.c_int64, C.c_int, C.c_int, C.c_int, C.c_int, _P]),
-    "modiff_qk_norm_rope": (C.c_int, [_P, _P, _P, _P, C.c_int, _P, _P, _P, _P, C.c_int, _P, _P, _P, _P,
-                                      C.c_int64, _P, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int,
+    "modiff_fp8_linear_bytes": (C.c_int64, [C.c_int] * 3),
+    "modiff_fp8_linear_x": (C.c_int, [_P, C.c_int64, _P, C.c_int64, _P, C.c_int64, _P, _P, C.c_int64,
+                                      C.c_int, C.c_int, C.c_int, C.c_int, _P, _P]),
+    "modiff_qk_norm_rope": (C.c_int, [_P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64, C.c_int] * 2 +
+                            [_P, _P, _P, _P, C.c_int64, _P, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int,
                                       C.c_float, C.c_int, _P]),
-    "modiff_kv4_append": (C.c_int, [_KV4, _P, _P, _P, _P, _P, _P, C.c_int, C.c_int, C.c_int, C.c_int, _P]),
+    "modiff_kv4_append": (C.c_int, [_KV4] + [_P, C.c_int64, C.c_int64, C.c_int64] * 2 + [_P, _P] +
+                          [C.c_int] * 4 + [_P]),
     "modiff_kv4_read": (C.c_int, [_KV4, _P, _P, C.c_int, C.c_int, C.c_int, _P, _P, C.c_int, _P]),
     "modiff_kv4_attention_bytes": (C.c_int64, [_KV4] + [C.c_int] * 6),
-    "modiff_kv4_attention": (C.c_int, [_P, _P, _KV4, _P, _P, _P, C.c_int, C.c_int, C.c_int, C.c_int,
+    "modiff_kv4_attention": (C.c_int, [_P, C.c_int64, C.c_int64, C.c_int64, _KV4, _P, _P, _P, C.c_int,
+                                       C.c_int, C.c_int, C.c_int,
                                        C.c_float, C.c_int, C.c_int, C.c_int, C.c_int, _P, _P]),
     "modiff_attn_codes_bytes": (C.c_int64, [C.c_int] * 5),
     "modiff_attn_quantize": (C.c_int, [_P, _P, _P] + [C.c_int] * 5 + [_P, _P, C.c_int, _P, _P, _P,
@@ -203,7 +208,7 @@ KERNELS_PER_CALL = {
     "modiff_attn_quantize": 2, "modiff_attention_i8": 1, "modiff_adaround_fake_quant": 1,
     "modiff_pack_weights_int4": 1, "modiff_igemm_conv_packed4": 1,
     "modiff_f32_split_weights": 1, "modiff_f32_split": 1, "modiff_conv_f32_tc": 1,
-    "modiff_fp8_quantize": 1, "modiff_fp8_pack_weight": 1, "modiff_fp8_linear": 1,
+    "modiff_fp8_quantize": 1, "modiff_fp8_pack_weight": 1, "modiff_fp8_linear": 1, "modiff_fp8_linear_x": 1,
     "modiff_qk_norm_rope": 1, "modiff_kv4_append": 1, "modiff_kv4_read": 1, "modiff_kv4_attention": 1,
 }
 LAUNCHES = [0]        # kernels launched through `call` since import

@@ -842,6 +842,7 @@ int read_device_status_pair(int* status, int reset);        // igemm_pair.cu
 int read_device_status_attention_i8(int* status, int reset);   // attention_i8.cu
 int read_device_status_conv_f32(int* status, int reset);       // conv_f32_tc.cu
 int read_device_status_fp8(int* status, int reset);            // fp8_linear.cu
+int read_device_status_fp8_pair(int* status, int reset);       // fp8_linear_pair.cu
 bool pair_supported(const modiff_conv_geom* g, int with_sum_rows, int per_sample, const float* bias,
                     const int32_t* acc_out, const float* o_hat);
 int launch_igemm_pair(const int8_t* codes, const int8_t* wcodes, int with_sum_rows,
@@ -900,7 +901,10 @@ int read_device_status(int* status, int reset) {
   int f8 = 0;
   rc = read_device_status_fp8(&f8, reset);
   if (rc) return rc;
-  *status = a | b | c | d | e | f | h | i8 | f32 | f8;
+  int f8p = 0;
+  rc = read_device_status_fp8_pair(&f8p, reset);
+  if (rc) return rc;
+  *status = a | b | c | d | e | f | h | i8 | f32 | f8 | f8p;
   return MODIFF_OK;
 }
 

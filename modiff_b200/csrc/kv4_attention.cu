@@ -576,8 +576,8 @@ extern "C" int64_t modiff_kv4_attention_bytes(const modiff_kv4_cache* cache, int
   return 4ll * pl.splits * batch * count * heads * (cache->dim + 2);
 }
 
-extern "C" int modiff_kv4_attention(const void* q, const int64_t* q_strides, const modiff_kv4_cache* cache,
-                                    const int32_t* table, const int32_t* lengths, void* out, int batch, int count,
+extern "C" int modiff_kv4_attention(const void* q, int64_t q_seq, int64_t q_token, int64_t q_head,
+                                    const modiff_kv4_cache* cache, const int32_t* table, const int32_t* lengths, void* out, int batch, int count,
                                     int heads, int max_pages, float scale, int causal, int window, int sinks,
                                     int dtype, void* workspace, void* stream) {
   int rc = kv4_check(cache, table, lengths, batch, max_pages);
@@ -588,7 +588,7 @@ extern "C" int modiff_kv4_attention(const void* q, const int64_t* q_strides, con
   MODIFF_CHECK_ARG(window >= 0 && sinks >= 0, "negative window or sinks");
   MODIFF_CHECK_ARG(causal || window == 0, "a window needs causal positions");
   if (batch == 0 || count == 0) return MODIFF_OK;
-  MODIFF_CHECK_ARG(q && q_strides && out, "NULL pointer argument");
+  MODIFF_CHECK_ARG(q && out, "NULL pointer argument");
   const int size = dtype_bytes(dtype);
   MODIFF_CHECK_ARG((uintptr_t)q % size == 0 && (uintptr_t)out % 16 == 0, "misaligned tensor");
   const Plan pl = plan_of(cache, batch, count, heads, max_pages, window, sinks);
@@ -596,7 +596,7 @@ extern "C" int modiff_kv4_attention(const void* q, const int64_t* q_strides, con
   MODIFF_CHECK_ARG(pl.splits == 1 || (workspace && (uintptr_t)workspace % 16 == 0), "NULL or misaligned workspace");
   AttnParams p;
   p.q = q;
-  p.qb = q_strides[0]; p.qt = q_strides[1]; p.qh = q_strides[2];
+  p.qb = q_seq; p.qt = q_token; p.qh = q_head;
   p.out = out;
   p.part = static_cast<float*>(workspace);
   p.c = kv4_pages(cache);

@@ -1,7 +1,7 @@
 // Writing and reading back a paged cache of keys and values held in 4 bits.
 //
 // A token's d channels of one head x have, in fp32 and rounded to fp16,
-//   m = fp16(min x),  s = fp16((max x - min x) / 15)
+//   m = fp16(min x),  s = fp16((max x - min x) (1 / 15))      (a product with the fp32 number 1 / 15)
 // and the codes round((x - m) / s) in 0 .. 15 (all 0 where s is 0); values beyond +-65504 count as
 // +-65504, a NaN makes the whole row NaN.  Every step is one correctly rounded fp32 operation, so the
 // bits are those of the same formula written with tensor operations.
@@ -74,7 +74,7 @@ kv4_append_kernel(const AppendParams p) {
     any |= __shfl_xor_sync(0xffffffffu, any, o);
   }
   if (!mine) return;
-  const __half s = __float2half_rn(any ? __int_as_float(0x7fc00000) : __fdiv_rn(__fsub_rn(high, low), 15.0f));
+  const __half s = __float2half_rn(any ? __int_as_float(0x7fc00000) : __fmul_rn(__fsub_rn(high, low), 1.0f / 15.0f));
   const __half m = __float2half_rn(any ? __int_as_float(0x7fc00000) : low);
   const float sf = __half2float(s), mf = __half2float(m);
   uint32_t packed = 0;
@@ -173,20 +173,21 @@ Kv4Pages kv4_pages(const modiff_kv4_cache* c) {
 
 using namespace modiff;
 
-extern "C" int modiff_kv4_append(const modiff_kv4_cache* cache, const void* k, const int64_t* k_strides,
-                                 const void* v, const int64_t* v_strides, const int32_t* table,
+extern "C" int modiff_kv4_append(const modiff_kv4_cache* cache, const void* k, int64_t k_seq, int64_t k_token,
+                                 int64_t k_head, const void* v, int64_t v_seq, int64_t v_token, int64_t v_head,
+                                 const int32_t* table,
                                  const int32_t* lengths, int batch, int count, int max_pages, int dtype,
                                  void* stream) {
   int rc = kv4_check(cache, table, lengths, batch, max_pages);
   if (rc) return rc;
   MODIFF_CHECK_ARG(dtype_ok(dtype), "unknown element type %d", dtype);
-  MODIFF_CHECK_ARG(k && v && k_strides && v_strides, "NULL pointer argument");
+  MODIFF_CHECK_ARG(k && v, "NULL pointer argument");
   MODIFF_CHECK_ARG(count >= 0, "negative token count");
   if (batch == 0 || count == 0) return MODIFF_OK;
   AppendParams p;
   p.k = k; p.v = v;
-  p.kb = k_strides[0]; p.kt = k_strides[1]; p.kh = k_strides[2];
-  p.vb = v_strides[0]; p.vt = v_strides[1]; p.vh = v_strides[2];
+  p.kb = k_seq; p.kt = k_token; p.kh = k_head;
+  p.vb = v_seq; p.vt = v_token; p.vh = v_head;
   p.c = kv4_pages(cache);
   p.table = table; p.lengths = lengths;
   p.batch = batch; p.count = count; p.max_pages = max_pages;

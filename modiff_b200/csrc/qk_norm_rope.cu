@@ -199,10 +199,9 @@ int by_lanes(NormRopeParams& p, cudaStream_t s) {
 
 using namespace modiff;
 
-extern "C" int modiff_qk_norm_rope(const void* q, const int64_t* q_strides, void* q_out,
-                                   const int64_t* q_out_strides, int q_heads, const void* k,
-                                   const int64_t* k_strides, void* k_out, const int64_t* k_out_strides,
-                                   int k_heads, const float* q_weight, const float* k_weight,
+extern "C" int modiff_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, void* q_out, int64_t q_out_token,
+                                   int64_t q_out_head, int q_heads, const void* k, int64_t k_token,
+                                   int64_t k_head, void* k_out, int64_t k_out_token, int64_t k_out_head, int k_heads, const float* q_weight, const float* k_weight,
                                    const float* cos, const float* sin, int64_t table_rows,
                                    const void* positions, int positions64, int64_t tokens, int d,
                                    int rot, int interleaved, float eps, int dtype, void* stream) {
@@ -211,22 +210,15 @@ extern "C" int modiff_qk_norm_rope(const void* q, const int64_t* q_strides, void
   MODIFF_CHECK_ARG(d >= 2 && d <= 256 && d % 2 == 0, "head width %d: an even number up to 256 is served", d);
   MODIFF_CHECK_ARG(rot >= 0 && rot <= d && rot % 2 == 0, "rotated channels %d of %d", rot, d);
   MODIFF_CHECK_ARG(rot == 0 || (cos && sin), "NULL table");
-  MODIFF_CHECK_ARG(q_heads == 0 || (q && q_out && q_strides && q_out_strides), "NULL pointer argument");
-  MODIFF_CHECK_ARG(k_heads == 0 || (k && k_out && k_strides && k_out_strides), "NULL pointer argument");
+  MODIFF_CHECK_ARG(q_heads == 0 || (q && q_out), "NULL pointer argument");
+  MODIFF_CHECK_ARG(k_heads == 0 || (k && k_out), "NULL pointer argument");
   MODIFF_CHECK_ARG(positions || rot == 0 || table_rows >= tokens, "tables of %lld rows for %lld tokens",
                    (long long)table_rows, (long long)tokens);
   if (tokens == 0 || q_heads + k_heads == 0) return MODIFF_OK;
 
   NormRopeParams p = {};
-  auto side = [](NormRopeSide& s, const void* x, const int64_t* xs, void* y, const int64_t* ys, const float* w,
-                 int heads) {
-    s.heads = heads;
-    if (!heads) return;
-    s.x = x; s.y = y; s.w = w;
-    s.x_token = xs[0]; s.x_head = xs[1]; s.y_token = ys[0]; s.y_head = ys[1];
-  };
-  side(p.q, q, q_strides, q_out, q_out_strides, q_weight, q_heads);
-  side(p.k, k, k_strides, k_out, k_out_strides, k_weight, k_heads);
+  p.q = NormRopeSide{q, q_out, q_token, q_head, q_out_token, q_out_head, q_weight, q_heads, 0};
+  p.k = NormRopeSide{k, k_out, k_token, k_head, k_out_token, k_out_head, k_weight, k_heads, 0};
   p.cos = cos;
   p.sin = sin;
   p.positions = rot ? positions : nullptr;

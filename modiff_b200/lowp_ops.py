@@ -18,165 +18,210 @@ FP8_BLOCK = 128
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
-def _check(name, x, *others):
-    """`x` and `others` (None allowed) are CUDA tensors of one device, none of which needs gradients."""
-    for t in (x,) + others:
+_stream = torch._C._cuda_getCurrentRawStream       # what torch.cuda.current_stream(device).cuda_stream wraps
+
+
+def _device(name, *tensors):
+    """The device that all `tensors` (None allowed) are on; CUDA tensors, none of which needs gradients."""
+    device, grad = -1, torch.is_grad_enabled()
+    for t in tensors:
         if t is None:
             continue
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        if not isinstance(t, torch.Tensor) or t.get_device() < 0:
             raise ModiffError(f"{name}: every tensor must be a CUDA tensor (there is no CPU fallback)")
-        if t.device != x.device:
-            raise ModiffError(f"{name}: tensors on {x.device} and {t.device}")
-        if t.requires_grad and torch.is_grad_enabled():
+        if device < 0:
+            device = t.get_device()
+        elif t.get_device() != device:
+            raise ModiffError(f"{name}: tensors on cuda:{device} and {t.device}")
+        if grad and t.requires_grad:
             raise ModiffError(f"{name} has no backward pass: call it under torch.no_grad() or detach its inputs")
+    return device
 
 
 def _dtype(name, x):
-    if x.dtype not in _DTYPES:
+    dt = _DTYPES.get(x.dtype)
+    if dt is None:
         raise ModiffError(f"{name}: fp32, fp16 or bf16 tensors, got {x.dtype}")
-    return _DTYPES[x.dtype]
+    return dt
 
 
-def _call(device, entry, *args, **kw):
-    """One entry point on `device`'s current stream, whatever the current device is."""
-    if device.index == torch.cuda.current_device():
-        _lib.call(entry, *args, torch.cuda.current_stream(device).cuda_stream, **kw)
+def _call(device, entry, *args, nbytes=0, nops=0, more=0):
+    """One entry point on `device`'s current stream, whatever the current device is; `more` kernels
+    beyond its first."""
+    if device == torch.cuda.current_device():
+        _lib.call(entry, *args, _stream(device), nbytes=nbytes, nops=nops)
     else:
         with torch.cuda.device(device):
-            _lib.call(entry, *args, torch.cuda.current_stream(device).cuda_stream, **kw)
-
-
-def _i64(*v):
-    return (C.c_int64 * len(v))(*v)
+            _lib.call(entry, *args, _stream(device), nbytes=nbytes, nops=nops)
+    _lib.LAUNCHES[0] += more
 
 
 # ------------------------------------------------------------------------------- 8-bit linear layers
 class Fp8Rows(NamedTuple):
     """Rows quantised by `fp8_quantize`: e4m3 codes [..., k] (row pitch a multiple of 16), fp32 scales
-    [..., ceil(k / 128)] and the type of the rows, which is the type of the layers' outputs."""
+    [..., ceil(k / 128)] (in memory block by block, the rows of a block next to each other) and the type
+    of the rows, which is the type of the layers' outputs."""
     codes: torch.Tensor
     scale: torch.Tensor
     dtype: torch.dtype
 
 
-def fp8_quantize(x):
-    """x [..., k] -> `Fp8Rows`: per row and block of 128 channels scale = max|x| / 448 (1 where that is
-    0) and codes e4m3(x / scale).  Quantise once what several layers read."""
-    _check("fp8_quantize", x)
-    dt = _dtype("fp8_quantize", x)
+def _rows(name, x):
+    """[..., k] as (address, row pitch, rows, k, the tensor that holds them); a copy only if it must be."""
     if x.dim() < 1 or x.shape[-1] == 0:
-        raise ModiffError(f"fp8_quantize: rows of at least one channel, got shape {tuple(x.shape)}")
+        raise ModiffError(f"{name}: rows of at least one channel, got shape {tuple(x.shape)}")
     k = x.shape[-1]
-    rows = x.numel() // k
-    x2 = x.reshape(rows, k)
-    if x2.stride(1) != 1 and k > 1:
-        x2 = x2.contiguous()
-    blocks = -(-k // FP8_BLOCK)
-    kp = -(-k // 16) * 16
+    if x.dim() != 2:
+        x = x.reshape(-1, k)
+    if k > 1 and x.stride(1) != 1:
+        x = x.contiguous()
+    return x.data_ptr(), x.stride(0), x.shape[0], k, x
+
+
+def fp8_quantize(x):
+    """x [..., k] -> `Fp8Rows`: per row and block of 128 channels scale = max|x| / 448 (as a product with
+    the fp32 number 1 / 448; 1 where it is 0) and codes e4m3(x / scale).  Quantise once what several
+    layers read."""
+    device = _device("fp8_quantize", x)
+    dt = _dtype("fp8_quantize", x)
+    at, pitch, rows, k, keep = _rows("fp8_quantize", x)
+    blocks, kp = -(-k // FP8_BLOCK), -(-k // 16) * 16
     lead = tuple(x.shape[:-1])
     codes = torch.empty(lead + (kp,), dtype=torch.float8_e4m3fn, device=x.device)
-    scale = torch.empty(lead + (blocks,), dtype=torch.float32, device=x.device)
+    row4 = -(-rows // 4) * 4
+    scale = torch.empty((blocks, row4), dtype=torch.float32, device=x.device)
     if rows:
-        _call(x.device, 'modiff_fp8_quantize', x2.data_ptr(), x2.stride(0), rows, k, dt, codes.data_ptr(), kp,
-              scale.data_ptr(), blocks, nbytes=rows * (k * x.element_size() + kp + 4 * blocks))
-    return Fp8Rows(codes[..., :k], scale, x.dtype)
+        _call(device, 'modiff_fp8_quantize', at, pitch, rows, k, dt, codes.data_ptr(), kp, scale.data_ptr(), row4,
+              nbytes=rows * (k * x.element_size() + kp + 4 * blocks))
+    scale = scale[:, :rows].t()
+    return Fp8Rows(codes[..., :k], scale if len(lead) == 1 else scale.view(lead + (blocks,)), x.dtype)
 
 
 def fp8_pack_weight(w):
     """A weight matrix [n, k] -> (e4m3 codes [n, k] with a row pitch of a multiple of 16, fp32 scales
     [ceil(n / 128), ceil(k / 128)]), one scale per 128 x 128 block.  Once per weight version."""
-    _check("fp8_pack_weight", w.detach() if isinstance(w, torch.Tensor) else w)
+    if isinstance(w, torch.Tensor):
+        w = w.detach()
+    device = _device("fp8_pack_weight", w)
     dt = _dtype("fp8_pack_weight", w)
     if w.dim() != 2 or w.numel() == 0:
         raise ModiffError(f"fp8_pack_weight: a matrix [n, k], got shape {tuple(w.shape)}")
-    w = w.detach()
-    n, k = w.shape
-    if w.stride(1) != 1 and k > 1:
-        w = w.contiguous()
+    at, pitch, n, k, keep = _rows("fp8_pack_weight", w)
     kp = -(-k // 16) * 16
     codes = torch.empty((n, kp), dtype=torch.float8_e4m3fn, device=w.device)
     scale = torch.empty((-(-n // FP8_BLOCK), -(-k // FP8_BLOCK)), dtype=torch.float32, device=w.device)
-    _call(w.device, 'modiff_fp8_pack_weight', w.data_ptr(), w.stride(0), n, k, dt, codes.data_ptr(), kp,
-          scale.data_ptr(), scale.shape[1], nbytes=n * (k * w.element_size() + kp))
+    _call(device, 'modiff_fp8_pack_weight', at, pitch, n, k, dt, codes.data_ptr(), kp, scale.data_ptr(),
+          scale.shape[1], nbytes=n * (k * w.element_size() + kp))
     return codes[:, :k], scale
-
-
-def _fp8_weight(w, w_scale, device):
-    if w.dtype != torch.float8_e4m3fn or w.dim() != 2 or w.numel() == 0:
-        raise ModiffError("fp8_linear: weight codes are a float8_e4m3fn matrix [n, k] (fp8_pack_weight)")
-    n, k = w.shape
-    pitch = w.stride(0) if n > 1 else -(-k // 16) * 16
-    if (w.stride(1) != 1 and k > 1) or pitch % 16 or pitch < k or w.data_ptr() % 16:
-        raise ModiffError("fp8_linear: weight rows start at multiples of 16 bytes (fp8_pack_weight lays them "
-                          f"out so); got strides {tuple(w.stride())} for {k} channels")
-    want = (-(-n // FP8_BLOCK), -(-k // FP8_BLOCK))
-    if w_scale.dtype != torch.float32 or tuple(w_scale.shape) != want:
-        raise ModiffError(f"fp8_linear: fp32 weight scales of shape {want}, got {w_scale.dtype} "
-                          f"{tuple(w_scale.shape)}")
-    if not w_scale.is_contiguous():
-        w_scale = w_scale.contiguous()
-    return n, k, pitch, w_scale
 
 
 def fp8_linear(x, w, w_scale, bias=None):
     """y = x w^T (+ bias) with x (a tensor [..., k], or `Fp8Rows`) and w (`fp8_pack_weight`) as 8-bit
     floating-point codes with one scale per block of 128 channels (and 128 weight rows).  y [..., n] and
     bias have the type of x."""
-    if not isinstance(x, Fp8Rows):
-        _check("fp8_linear", x, w, w_scale, bias)
-        if x.dim() < 1 or x.shape[-1] != w.shape[-1]:
-            raise ModiffError(f"fp8_linear: rows of shape {tuple(x.shape)} for weights {tuple(w.shape)}")
-        x = fp8_quantize(x)
-    else:
-        _check("fp8_linear", x.codes, x.scale, w, w_scale, bias)
-    codes, scale, dtype = x
-    n, k, w_pitch, w_scale = _fp8_weight(w, w_scale, codes.device)
-    if codes.dtype != torch.float8_e4m3fn or codes.shape[-1] != k:
-        raise ModiffError(f"fp8_linear: rows of {codes.shape[-1]} channels for weights {tuple(w.shape)}")
+    ready = isinstance(x, Fp8Rows)
+    src = x.codes if ready else x
+    device = _device("fp8_linear", src, w, w_scale, bias)
+    if w.dtype != torch.float8_e4m3fn or w.dim() != 2 or w.numel() == 0:
+        raise ModiffError("fp8_linear: weight codes are a float8_e4m3fn matrix [n, k] (fp8_pack_weight)")
+    n, k = w.shape
+    w_pitch, step = w.stride()
+    if n == 1:
+        w_pitch = -(-k // 16) * 16
+    if (k > 1 and step != 1) or w_pitch % 16 or w_pitch < k or w.data_ptr() % 16:
+        raise ModiffError("fp8_linear: weight rows start at multiples of 16 bytes (fp8_pack_weight lays them "
+                          f"out so); got strides {w.stride()} for {k} channels")
+    blocks = -(-k // FP8_BLOCK)
+    if w_scale.dtype != torch.float32 or w_scale.shape != (-(-n // FP8_BLOCK), blocks):
+        raise ModiffError(f"fp8_linear: fp32 weight scales of shape {(-(-n // FP8_BLOCK), blocks)}, got "
+                          f"{w_scale.dtype} {tuple(w_scale.shape)}")
+    if not w_scale.is_contiguous():
+        w_scale = w_scale.contiguous()
+    dtype = x.dtype
     dt = _DTYPES.get(dtype)
     if dt is None:
-        raise ModiffError(f"fp8_linear: outputs of fp32, fp16 or bf16, got {dtype}")
-    if bias is not None and (bias.dtype != dtype or tuple(bias.shape) != (n,)):
-        raise ModiffError(f"fp8_linear: bias of {n} values of {dtype}, got {tuple(bias.shape)} {bias.dtype}")
-    lead = codes.shape[:-1]
-    rows = lead.numel()
-    blocks = -(-k // FP8_BLOCK)
-    kp = -(-k // 16) * 16
-    if scale.dtype != torch.float32 or tuple(scale.shape) != tuple(lead) + (blocks,):
-        raise ModiffError(f"fp8_linear: fp32 scales of shape {tuple(lead) + (blocks,)}, got {tuple(scale.shape)}")
-    if rows and (codes.data_ptr() % 16 or not scale.is_contiguous() or not _pitched(codes, kp)):
-        raise ModiffError("fp8_linear: rows of codes as fp8_quantize lays them out")
-    y = torch.empty(tuple(lead) + (n,), dtype=dtype, device=codes.device)
-    if rows > 0x7fffffff:
-        raise ModiffError("fp8_linear: too many rows")
-    if rows:
-        if bias is not None and n > 1 and bias.stride(0) != 1:
-            bias = bias.contiguous()
-        _call(codes.device, 'modiff_fp8_linear', codes.data_ptr(), kp, scale.data_ptr(), blocks, w.data_ptr(), w_pitch,
+        raise ModiffError(f"fp8_linear: fp32, fp16 or bf16 rows, got {dtype}")
+    if src.dim() < 1 or src.shape[-1] != k:
+        raise ModiffError(f"fp8_linear: rows of shape {tuple(src.shape)} for weights {tuple(w.shape)}")
+    if bias is not None:
+        if bias.dtype != dtype or bias.shape != (n,):
+            raise ModiffError(f"fp8_linear: bias of {n} values of {dtype}, got {tuple(bias.shape)} {bias.dtype}")
+        bias = bias.contiguous()
+    lead = tuple(src.shape[:-1])
+    y = torch.empty(lead + (n,), dtype=dtype, device=src.device)
+    if y.numel() == 0:
+        return y
+    if ready:
+        kp = -(-k // 16) * 16
+        rows = lead[0] if len(lead) == 1 else y.numel() // n
+        if rows > 0x7fffffff:
+            raise ModiffError("fp8_linear: too many rows")
+        _device("fp8_linear", src, x.scale)
+        if x.scale.dtype != torch.float32 or tuple(x.scale.shape) != lead + (blocks,):
+            raise ModiffError(f"fp8_linear: fp32 scales of shape {lead + (blocks,)}, got {tuple(x.scale.shape)}")
+        row4 = -(-rows // 4) * 4
+        if (src.dtype != torch.float8_e4m3fn or src.data_ptr() % 16 or not _pitched(src, kp, 1)
+                or x.scale.data_ptr() % 16 or not _pitched(x.scale, 1, row4)):
+            raise ModiffError("fp8_linear: rows of codes as fp8_quantize lays them out")
+        _call(device, 'modiff_fp8_linear', src.data_ptr(), kp, x.scale.data_ptr(), row4, w.data_ptr(), w_pitch,
               w_scale.data_ptr(), blocks, _lib.ptr(bias), y.data_ptr(), n, rows, k, n, dt,
               nbytes=rows * kp + n * k + y.numel() * y.element_size(), nops=2 * rows * n * k)
+        return y
+    at, pitch, rows, _, keep = _rows("fp8_linear", x)
+    if rows > 0x7fffffff:
+        raise ModiffError("fp8_linear: too many rows")
+    size = _lib.lib().modiff_fp8_linear_bytes(rows, k, n)
+    work = torch.empty(size, dtype=torch.uint8, device=src.device) if size else None
+    _call(device, 'modiff_fp8_linear_x', at, pitch, w.data_ptr(), w_pitch, w_scale.data_ptr(), blocks, _lib.ptr(bias),
+          y.data_ptr(), n, rows, k, n, dt, _lib.ptr(work),
+          nbytes=(rows * k + y.numel()) * y.element_size() + n * k, nops=2 * rows * n * k, more=int(size > 0))
     return y
 
 
-def _pitched(codes, pitch):
-    """Whether the leading dimensions of `codes` walk rows of `pitch` bytes without a gap."""
-    want = pitch
-    if codes.shape[-1] > 1 and codes.stride(-1) != 1:
+def _pitched(t, pitch, step):
+    """Whether the leading dimensions of `t` walk rows `pitch` apart without a gap, its last one `step`."""
+    if t.shape[-1] > 1 and t.stride(-1) != step:
         return False
-    for d in range(codes.dim() - 2, -1, -1):
-        if codes.shape[d] > 1 and codes.stride(d) != want:
+    for d in range(t.dim() - 2, -1, -1):
+        if t.shape[d] > 1 and t.stride(d) != pitch:
             return False
-        want *= codes.shape[d]
+        pitch *= t.shape[d]
     return True
 
 
 # --------------------------------------------------------------------- norms of queries and keys
 def _tokens(name, x):
     """[..., heads, d] as [tokens, heads, d] with the channels contiguous (a copy only if it must be)."""
-    if x.dim() < 3:
-        raise ModiffError(f"{name}: tensors [..., heads, d], got shape {tuple(x.shape)}")
-    x = x if x.dim() == 3 else x.flatten(0, -3)
+    if x.dim() != 3:
+        if x.dim() < 3:
+            raise ModiffError(f"{name}: tensors [..., heads, d], got shape {tuple(x.shape)}")
+        x = x.flatten(0, -3)
     return x if x.stride(2) == 1 or x.shape[2] == 1 else x.contiguous()
+
+
+def _norm_weight(name, w, d):
+    if w is None:
+        return None
+    if w.dtype != torch.float32 or w.shape != (d,):
+        raise ModiffError(f"{name}: fp32 weights of {d} values, got {tuple(w.shape)} {w.dtype}")
+    return w.contiguous()
+
+
+def _norm_out(name, x, out):
+    """Where the result of `x` goes: a new tensor, or `out`, as the caller sees it and as [tokens, heads, d]."""
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    elif out.shape != x.shape or out.dtype != x.dtype:
+        raise ModiffError(f"{name}: out {tuple(out.shape)} {out.dtype} for {tuple(x.shape)} {x.dtype}")
+    flat = out
+    if out.dim() != 3:
+        try:
+            flat = out.view(-1, *out.shape[-2:]) if out.numel() else out.flatten(0, -3)
+        except RuntimeError:
+            raise ModiffError(f"{name}: out needs leading dimensions that merge, got strides {out.stride()}") from None
+    if flat.stride(2) != 1:
+        raise ModiffError(f"{name}: out needs contiguous channels, got strides {out.stride()}")
+    return out, flat
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6, interleaved=False, out=None):
@@ -184,69 +229,55 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6, i
     times the weights fp32 [d] (None: ones), and the rotation of the first 2 * cos.shape[1] channels by
     the angles in row `positions` (int32 / int64, one per token; None: the token's own number) of the
     fp32 tables cos and sin, one pass over both.  Pairs are (i, half + i), or (2i, 2i + 1) with
-    `interleaved`.  q and k may be slices of one projection; `out` = (q, k) writes in place.  A position
-    outside the tables gives a row of NaN.  Returns (q', k')."""
+    `interleaved`.  q and k may be slices of one projection; `out` = (q, k) writes in place (`out` may
+    be the inputs or apart from them, not overlap them otherwise).  A position outside the tables gives a
+    row of NaN.  Returns (q', k')."""
     name = "qk_norm_rope"
-    _check(name, q, k, q_weight, k_weight, cos, sin, positions, *(out or ()))
+    if out is not None and (len(out) != 2 or (out[1] is None) != (k is None)):
+        raise ModiffError(f"{name}: out is a pair like (q, k)")
+    device = _device(name, q, k, q_weight, k_weight, cos, sin, positions, *(out or ()))
     dt = _dtype(name, q)
-    d = q.shape[-1]
+    d = q.shape[-1] if q.dim() else 0
     if k is not None and (k.dtype != q.dtype or k.shape[-1] != d or k.shape[:-2] != q.shape[:-2]):
         raise ModiffError(f"{name}: q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} differ in more "
                           "than their heads")
     if d % 2 or not 2 <= d <= 256:
         raise ModiffError(f"{name}: heads of an even number of channels up to 256, got {d}")
-    for w in (q_weight, k_weight):
-        if w is not None and (w.dtype != torch.float32 or tuple(w.shape) != (d,) or not w.is_contiguous()):
-            raise ModiffError(f"{name}: contiguous fp32 weights of {d} values, got {tuple(w.shape)} {w.dtype}")
+    q_weight, k_weight = _norm_weight(name, q_weight, d), _norm_weight(name, k_weight, d)
     if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2 or cos.shape != sin.shape
             or 2 * cos.shape[1] > d):
         raise ModiffError(f"{name}: fp32 tables [rows, at most {d // 2}], got {tuple(cos.shape)} and "
                           f"{tuple(sin.shape)}")
     cos, sin = cos.contiguous(), sin.contiguous()
+    rows, half = cos.shape
     q3 = _tokens(name, q)
-    k3 = None if k is None else _tokens(name, k)
     n = q3.shape[0]
-    wide = 0
+    wide, at = 0, None
     if positions is not None:
-        if positions.dtype not in (torch.int32, torch.int64) or positions.numel() != n:
+        wide = int(positions.dtype == torch.int64)
+        if not (wide or positions.dtype == torch.int32) or positions.numel() != n:
             raise ModiffError(f"{name}: {n} positions of int32 or int64, got {tuple(positions.shape)} "
                               f"{positions.dtype}")
         positions = positions.contiguous()
-        wide = int(positions.dtype == torch.int64)
-    elif cos.shape[1] and cos.shape[0] < n:
-        raise ModiffError(f"{name}: tables of {cos.shape[0]} rows for {n} tokens")
-    if out is None:
-        outs = (torch.empty(q.shape, dtype=q.dtype, device=q.device),
-                None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device))
+        at = positions.data_ptr()
+    elif half and rows < n:
+        raise ModiffError(f"{name}: tables of {rows} rows for {n} tokens")
+    q_out, qo = _norm_out(name, q, None if out is None else out[0])
+    heads = q3.shape[1]
+    args = [q3.data_ptr(), q3.stride(0), q3.stride(1), qo.data_ptr(), qo.stride(0), qo.stride(1), heads]
+    k_out = None
+    if k is None:
+        args += [None, 0, 0, None, 0, 0, 0]
     else:
-        outs = tuple(out)
-        if len(outs) != 2 or (outs[1] is None) != (k is None):
-            raise ModiffError(f"{name}: out is a pair like (q, k)")
-        for o, x in zip(outs, (q, k)):
-            if o is not None and (o.shape != x.shape or o.dtype != x.dtype):
-                raise ModiffError(f"{name}: out {tuple(o.shape)} {o.dtype} for {tuple(x.shape)} {x.dtype}")
-    flat = []
-    for o in outs:
-        if o is None:
-            flat.append(None)
-            continue
-        f = o if o.dim() == 3 else o.flatten(0, -3)
-        if (f.stride(2) != 1 and d > 1) or f.data_ptr() != o.data_ptr():
-            raise ModiffError(f"{name}: out needs contiguous channels and leading dimensions that merge")
-        flat.append(f)
+        k3 = _tokens(name, k)
+        k_out, ko = _norm_out(name, k, None if out is None else out[1])
+        args += [k3.data_ptr(), k3.stride(0), k3.stride(1), ko.data_ptr(), ko.stride(0), ko.stride(1), k3.shape[1]]
+        heads += k3.shape[1]
     if n:
-        args = []
-        for x, o in ((q3, flat[0]), (k3, flat[1])):
-            if x is None:
-                args += [None, None, None, None, 0]
-            else:
-                args += [x.data_ptr(), _i64(x.stride(0), x.stride(1)), o.data_ptr(), _i64(o.stride(0), o.stride(1)),
-                         x.shape[1]]
-        heads = q3.shape[1] + (0 if k3 is None else k3.shape[1])
-        _call(q.device, 'modiff_qk_norm_rope', *args, _lib.ptr(q_weight), _lib.ptr(k_weight), cos.data_ptr(),
-              sin.data_ptr(), cos.shape[0], _lib.ptr(positions), wide, n, d, 2 * cos.shape[1], int(bool(interleaved)),
-              float(eps), dt, nbytes=2 * n * heads * d * q.element_size())
-    return outs
+        _call(device, 'modiff_qk_norm_rope', *args, _lib.ptr(q_weight), _lib.ptr(k_weight), cos.data_ptr(),
+              sin.data_ptr(), rows, at, wide, n, d, 2 * half, int(bool(interleaved)), float(eps), dt,
+              nbytes=2 * n * heads * d * q.element_size())
+    return q_out, k_out
 
 
 # ------------------------------------------------------------------------------ the 4-bit cache
@@ -274,17 +305,18 @@ def kv4_cache(pages, kv_heads, page_size, head_dim, device):
 
 def _cache(name, cache, table, lengths):
     kc, kp, vc, vp = cache
-    if (kc.dim() != 4 or kc.dtype != torch.uint8 or vc.dtype != torch.uint8 or kc.shape != vc.shape
-            or kp.dtype != torch.float16 or vp.dtype != torch.float16 or kp.shape != vp.shape
-            or kp.shape != kc.shape[:3] + (2,)
+    shape = kc.shape
+    if (len(shape) != 4 or kc.dtype != torch.uint8 or vc.dtype != torch.uint8 or vc.shape != shape
+            or kp.dtype != torch.float16 or vp.dtype != torch.float16 or kp.shape != shape[:3] + (2,)
+            or vp.shape != kp.shape
             or not (kc.is_contiguous() and vc.is_contiguous() and kp.is_contiguous() and vp.is_contiguous())):
         raise ModiffError(f"{name}: a cache is contiguous uint8 codes [pages, heads, page_size, d / 2] and fp16 "
                           f"[pages, heads, page_size, 2], got {tuple(kc.shape)} {kc.dtype}, {tuple(kp.shape)} {kp.dtype}")
     if (table.dim() != 2 or table.dtype != torch.int32 or lengths.dtype != torch.int32
-            or tuple(lengths.shape) != (table.shape[0],) or table.shape[1] == 0):
+            or lengths.shape != table.shape[:1] or table.shape[1] == 0):
         raise ModiffError(f"{name}: int32 table [batch, pages] and lengths [batch], got {tuple(table.shape)} "
                           f"{table.dtype} and {tuple(lengths.shape)} {lengths.dtype}")
-    pages, heads, size, half = kc.shape
+    pages, heads, size, half = shape
     return (_lib.Kv4CacheStruct(kc.data_ptr(), vc.data_ptr(), kp.data_ptr(), vp.data_ptr(), pages, heads, size,
                                 2 * half), table.contiguous(), lengths.contiguous())
 
@@ -295,7 +327,7 @@ def kv4_append(cache, k, v, table, lengths):
     `lengths` counts the new tokens; positions below 0 (shorter sequences of a padded batch) and page
     numbers outside the cache are skipped.  No two sequences may name the same place."""
     name = "kv4_append"
-    _check(name, k, v, table, lengths, *cache)
+    device = _device(name, k, v, table, lengths, *cache)
     c, table, lengths = _cache(name, cache, table, lengths)
     dt = _dtype(name, k)
     b = table.shape[0]
@@ -308,8 +340,8 @@ def kv4_append(cache, k, v, table, lengths):
     if v.stride(3) != 1:
         v = v.contiguous()
     if k.numel():
-        _call(k.device, 'modiff_kv4_append', C.byref(c), k.data_ptr(), _i64(*k.stride()[:3]), v.data_ptr(),
-              _i64(*v.stride()[:3]), table.data_ptr(), lengths.data_ptr(), b, k.shape[1], table.shape[1], dt,
+        _call(device, 'modiff_kv4_append', C.byref(c), k.data_ptr(), *k.stride()[:3], v.data_ptr(),
+              *v.stride()[:3], table.data_ptr(), lengths.data_ptr(), b, k.shape[1], table.shape[1], dt,
               nbytes=2 * k.numel() * k.element_size() + k.numel() // c.dim * 2 * (c.dim // 2 + 4))
 
 
@@ -317,7 +349,7 @@ def kv4_read(cache, table, lengths, n, dtype=torch.float32):
     """The last n positions of every sequence as values: (k, v) [batch, n, kv_heads, d], zeros for
     positions below 0 and pages outside the cache."""
     name = "kv4_read"
-    _check(name, table, lengths, *cache)
+    device = _device(name, table, lengths, *cache)
     c, table, lengths = _cache(name, cache, table, lengths)
     if dtype not in _DTYPES or n < 0:
         raise ModiffError(f"{name}: n >= 0 tokens as fp32, fp16 or bf16, got {n} and {dtype}")
@@ -325,7 +357,7 @@ def kv4_read(cache, table, lengths, n, dtype=torch.float32):
     k = torch.empty((b, n, c.heads, c.dim), dtype=dtype, device=table.device)
     v = torch.empty_like(k)
     if k.numel():
-        _call(table.device, 'modiff_kv4_read', C.byref(c), table.data_ptr(), lengths.data_ptr(), b, n, table.shape[1],
+        _call(device, 'modiff_kv4_read', C.byref(c), table.data_ptr(), lengths.data_ptr(), b, n, table.shape[1],
               k.data_ptr(), v.data_ptr(), _DTYPES[dtype],
               nbytes=2 * k.numel() * k.element_size() + k.numel() // c.dim * 2 * (c.dim // 2 + 4))
     return k, v
@@ -339,7 +371,7 @@ def kv4_attention(q, cache, table, lengths, scale=None, causal=True, window=0, s
     them and the first `sinks` of the sequence (tokens outside are not read).  causal=False: every query
     sees all lengths[b] tokens.  A row that sees nothing is 0.  scale defaults to d ** -0.5."""
     name = "kv4_attention"
-    _check(name, q, table, lengths, *cache)
+    device = _device(name, q, table, lengths, *cache)
     c, table, lengths = _cache(name, cache, table, lengths)
     dt = _dtype(name, q)
     b = table.shape[0]
@@ -358,7 +390,7 @@ def kv4_attention(q, cache, table, lengths, scale=None, causal=True, window=0, s
         size = _lib.lib().modiff_kv4_attention_bytes(C.byref(c), b, n, heads, table.shape[1], window, sinks)
         work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
         scale = float(scale) if scale is not None else c.dim ** -0.5
-        _call(q.device, 'modiff_kv4_attention', q.data_ptr(), _i64(*q.stride()[:3]), C.byref(c), table.data_ptr(),
+        _call(device, 'modiff_kv4_attention', q.data_ptr(), *q.stride()[:3], C.byref(c), table.data_ptr(),
               lengths.data_ptr(), out.data_ptr(), b, n, heads, table.shape[1], scale, int(bool(causal)), window, sinks,
-              dt, _lib.ptr(work))
+              dt, _lib.ptr(work), more=int(size > 0))
     return out

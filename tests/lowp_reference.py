@@ -21,7 +21,8 @@ def e4m3_rows(x):
     xp[:, :k] = x.float().cpu()
     xb = xp.view(rows, kb, BLOCK)
     top = xb.abs().amax(-1)
-    s = torch.where(top == 0, torch.ones_like(top), top / 448.0)
+    s = top * torch.tensor(1.0 / 448.0)
+    s = torch.where(s == 0, torch.ones_like(s), s)
     codes = (xb / s[..., None]).clamp(-448.0, 448.0).to(torch.float8_e4m3fn).float()
     return codes.view(rows, -1)[:, :k], s
 
@@ -33,7 +34,8 @@ def e4m3_blocks(w):
     wp[:n, :k] = w.float().cpu()
     blocks = wp.view(nb, BLOCK, kb, BLOCK)
     top = blocks.abs().amax(dim=(1, 3))
-    s = torch.where(top == 0, torch.ones_like(top), top / 448.0)
+    s = top * torch.tensor(1.0 / 448.0)
+    s = torch.where(s == 0, torch.ones_like(s), s)
     codes = (blocks / s[:, None, :, None]).clamp(-448.0, 448.0).to(torch.float8_e4m3fn).float()
     return codes.view(nb * BLOCK, kb * BLOCK)[:n, :k], s
 
@@ -91,7 +93,7 @@ def norm_tolerance(y, size, d, dtype):
 def quantise_4bit(x):
     x = x.float().cpu().clamp(-65504.0, 65504.0)
     low, high = x.amin(-1, keepdim=True), x.amax(-1, keepdim=True)
-    s, m = ((high - low) / 15.0).half(), low.half()
+    s, m = ((high - low) * torch.tensor(1.0 / 15.0)).half(), low.half()
     sf = s.float()
     q = torch.where(sf > 0, (x - m.float()) / torch.where(sf > 0, sf, torch.ones_like(sf)), torch.zeros_like(x))
     q = torch.nan_to_num(q, 0.0).round().clamp(0, 15).to(torch.uint8)

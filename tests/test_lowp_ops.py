@@ -53,43 +53,48 @@ def test_entry_points_refuse_bad_arguments_without_a_device():
     """The C entry points check before they touch a device: made-up addresses are never followed."""
     lib = _lib.lib()
     a = 1 << 20                                            # an aligned address nobody reads
-    s2, s3 = (C.c_int64 * 2)(64, 64), (C.c_int64 * 3)(64, 64, 64)
+    s2, s3 = (64, 64), (64, 64, 64)
 
     def cache(pages=4, heads=2, size=16, dim=64, at=a):
         return C.byref(_lib.Kv4CacheStruct(at, a, a, a, pages, heads, size, dim))
 
     def attend(c, q=a, heads=4, count=1, pages=1, causal=1, window=0, sinks=0, dtype=0):
-        return lib.modiff_kv4_attention(q, s3, c, a, a, a, 1, count, heads, pages, 1.0, causal, window, sinks, dtype,
+        return lib.modiff_kv4_attention(q, *s3, c, a, a, a, 1, count, heads, pages, 1.0, causal, window, sinks, dtype,
                                         None, None)
 
     for rc in (attend(cache(size=24)), attend(cache(dim=96)), attend(cache(pages=0)), attend(cache(at=a + 8)),
                attend(cache(at=None)), attend(cache(), heads=3), attend(cache(), window=-1),
                attend(cache(), causal=0, window=4), attend(cache(), dtype=3), attend(cache(), q=None),
                attend(cache(), pages=0), attend(cache(), pages=1 << 28), attend(cache(), count=1 << 29),
-               lib.modiff_kv4_append(cache(), a, s3, a, s3, a, a, 1, -1, 1, 0, None),
-               lib.modiff_kv4_append(cache(), a + 1, s3, a, s3, a, a, 1, 1, 1, 0, None),
+               lib.modiff_kv4_append(cache(), a, *s3, a, *s3, a, a, 1, -1, 1, 0, None),
+               lib.modiff_kv4_append(cache(), a + 1, *s3, a, *s3, a, a, 1, 1, 1, 0, None),
                lib.modiff_kv4_read(cache(), a, a, 1, 1, 1, a + 4, a, 0, None),
-               lib.modiff_fp8_quantize(a, 64, 1, 0, 0, a, 64, a, 1, None),
-               lib.modiff_fp8_quantize(a, 64, 1, 64, 0, a, 72, a, 1, None),
-               lib.modiff_fp8_quantize(a, 64, 1, 64, 0, a, 48, a, 1, None),
-               lib.modiff_fp8_quantize(a, 64, 1, 200, 0, a, 208, a, 1, None),
+               lib.modiff_fp8_quantize(a, 64, 1, 0, 0, a, 64, a, 4, None),
+               lib.modiff_fp8_quantize(a, 64, 1, 64, 0, a, 72, a, 4, None),
+               lib.modiff_fp8_quantize(a, 64, 1, 64, 0, a, 48, a, 4, None),
+               lib.modiff_fp8_quantize(a, 64, 1, 64, 0, a, 64, a, 6, None),
+               lib.modiff_fp8_quantize(a, 64, 5, 64, 0, a, 64, a, 4, None),
                lib.modiff_fp8_pack_weight(a, 64, 1, 64, 0, a, 128, a, 1, None),
-               lib.modiff_fp8_linear(a, 64, a, 1, a, 72, a, 1, None, a, 8, 1, 64, 8, 0, None),
-               lib.modiff_fp8_linear(a, 64, a, 1, a, 64, a, 1, None, a, 7, 1, 64, 8, 0, None),
-               lib.modiff_fp8_linear(a + 8, 64, a, 1, a, 64, a, 1, None, a, 8, 1, 64, 8, 0, None),
-               lib.modiff_fp8_linear(a, 64, a, 1, a, 64, a, 1, None, a, 8, 1, 64, 8, 7, None),
-               lib.modiff_qk_norm_rope(a, s2, a, s2, 1, a, s2, a, s2, 1, None, None, a, a, 8, a, 0, 8, 63, 32, 0, 1e-6,
+               lib.modiff_fp8_linear(a, 64, a, 4, a, 72, a, 1, None, a, 8, 1, 64, 8, 0, None),
+               lib.modiff_fp8_linear(a, 64, a, 4, a, 64, a, 1, None, a, 7, 1, 64, 8, 0, None),
+               lib.modiff_fp8_linear(a + 8, 64, a, 4, a, 64, a, 1, None, a, 8, 1, 64, 8, 0, None),
+               lib.modiff_fp8_linear(a, 64, a, 4, a, 64, a, 1, None, a, 8, 1, 64, 8, 7, None),
+               lib.modiff_fp8_linear(a, 64, a, 5, a, 64, a, 1, None, a, 8, 1, 64, 8, 0, None),
+               lib.modiff_fp8_linear_x(a, 64, a, 64, a, 1, None, a, 8, 40, 64, 8, 0, None, None),
+               lib.modiff_fp8_linear_x(a, 64, a, 72, a, 1, None, a, 8, 40, 64, 8, 0, a, None),
+               lib.modiff_fp8_linear_x(None, 64, a, 64, a, 1, None, a, 8, 1, 64, 8, 0, a, None),
+               lib.modiff_qk_norm_rope(a, *s2, a, *s2, 1, a, *s2, a, *s2, 1, None, None, a, a, 8, a, 0, 8, 63, 32, 0, 1e-6,
                                        0, None),
-               lib.modiff_qk_norm_rope(a, s2, a, s2, 1, a, s2, a, s2, 1, None, None, a, a, 8, a, 0, 8, 64, 66, 0, 1e-6,
+               lib.modiff_qk_norm_rope(a, *s2, a, *s2, 1, a, *s2, a, *s2, 1, None, None, a, a, 8, a, 0, 8, 64, 66, 0, 1e-6,
                                        0, None),
-               lib.modiff_qk_norm_rope(a, s2, a, s2, 1, a, s2, a, s2, 1, None, None, a, a, 7, None, 0, 8, 64, 64, 0,
+               lib.modiff_qk_norm_rope(a, *s2, a, *s2, 1, a, *s2, a, *s2, 1, None, None, a, a, 7, None, 0, 8, 64, 64, 0,
                                        1e-6, 0, None),
-               lib.modiff_qk_norm_rope(a, s2, a, s2, 1, a, s2, a, s2, 1, None, None, None, a, 8, a, 0, 8, 64, 64, 0,
+               lib.modiff_qk_norm_rope(a, *s2, a, *s2, 1, a, *s2, a, *s2, 1, None, None, None, a, 8, a, 0, 8, 64, 64, 0,
                                        1e-6, 0, None)):
         assert rc == 1 and lib.modiff_last_error()
     # nothing to do is not an error, and touches nothing
     assert lib.modiff_fp8_quantize(None, 64, 0, 64, 0, None, 64, None, 1, None) == 0
-    assert lib.modiff_kv4_append(cache(), a, s3, a, s3, a, a, 1, 0, 1, 0, None) == 0
+    assert lib.modiff_kv4_append(cache(), a, *s3, a, *s3, a, a, 1, 0, 1, 0, None) == 0
 
 
 @gpu
