@@ -33,6 +33,7 @@ constexpr int kThreads = 32 * kWarps;
 constexpr int kTile = 64;                 // tokens a warp takes at a time
 constexpr int kSub = kTile / 16;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kMaxSplits = 256;
 
 struct AttnParams {
   const void* q;
@@ -72,6 +73,33 @@ __device__ inline uint32_t half_pair(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ inline float2 half_values(uint32_t h) { return __half22float2(*reinterpret_cast<const __half2*>(&h)); }
+
+// pairs of fp32 values, one instruction for both
+__device__ inline uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ inline float2 unpack2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ inline uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ inline uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ inline uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 
 template <int BYTES>
 __device__ inline void load_words(const uint8_t* src, uint32_t (&w)[BYTES / 4]) {
@@ -114,6 +142,11 @@ __device__ inline TileRange tiles_of(const AttnParams& p, int length, int p_lo, 
   return r;
 }
 
+__device__ inline bool sees(const AttnParams& p, int t, int pos) {
+  if (p.causal && t > pos) return false;
+  return p.window <= 0 || t > pos - p.window || t < p.sinks;
+}
+
 template <typename T, int D, int NT>
 constexpr int smem_bytes() {
   constexpr int planes = sizeof(T) == 4 ? 2 : 1;
@@ -131,10 +164,12 @@ kv4_attention_kernel(const AttnParams p) {
   constexpr int R = 8 * NT;
   constexpr int KW = D / 32;                      // words of a key row that a thread holds
   constexpr int VW = D / 64;                      // words of a value row that a thread holds
+  constexpr bool kAllValues = NT == 1 && D <= 128;  // registers for a whole tile's values
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float row_a[R], row_b[R];            // factors of (q . code) and of m_k
+  __shared__ float row_a[R], row_b[R];            // factor of a score, sum of the scaled query
   __shared__ float join_m[kWarps][R], join_l[kWarps][R], join_s[kWarps][R];
 
+  if (p.splits > 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, j = lane & 3;
   int id = blockIdx.x;
@@ -172,8 +207,9 @@ kv4_attention_kernel(const AttnParams p) {
     if (top > 0.0f && top < INFINITY) { frexpf(top, &e2); e2 = 15 - e2; }
     const float f1 = ldexpf(1.0f, e2 / 2), f2 = ldexpf(1.0f, e2 - e2 / 2);
     if (lane == 0) {
+      // score = a (s_k (q' . code') + m_k b) with q' the scaled query and code' = code 2^-24
       row_a[r] = ((p.scale2 * 16777216.0f) / f1) / f2;
-      row_b[r] = p.scale2 * sum;
+      row_b[r] = sum * f1 * f2 * 0x1p-24f;
     }
 #pragma unroll
     for (int e = 0; e < D / 32; ++e) {
@@ -199,7 +235,8 @@ kv4_attention_kernel(const AttnParams p) {
   const int t_end = (int)((int64_t)range.count * (split + 1) / p.splits);
 
   float o[D / 16][NT][4];
-  float m_run[NT][2], l_run[NT][2], s_run[NT][2], ra[NT][2], rb[NT][2];
+  float m_run[NT][2];
+  uint64_t l_run[NT], s_run[NT], ra[NT], rb[NT];   // pairs: query rows 2j and 2j + 1 of the eight
   int pos[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -207,69 +244,90 @@ kv4_attention_kernel(const AttnParams p) {
     for (int i = 0; i < D / 16; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[i][nt][e] = 0.0f;
+    const int r = 8 * nt + 2 * j;
+    l_run[nt] = s_run[nt] = 0ull;
+    ra[nt] = pack2(row_a[r], row_a[r + 1]);
+    rb[nt] = pack2(row_b[r], row_b[r + 1]);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int r = 8 * nt + 2 * j + e;
       m_run[nt][e] = -INFINITY;
-      l_run[nt][e] = s_run[nt][e] = 0.0f;
-      ra[nt][e] = row_a[r];
-      rb[nt][e] = row_b[r];
-      pos[nt][e] = length - p.count + (row0 + r) / p.group;
+      pos[nt][e] = length - p.count + (row0 + r + e) / p.group;
     }
   }
-  const int64_t row_bytes = D / 2;
-  const __half2* k_par = reinterpret_cast<const __half2*>(p.c.k_params);
-  const __half2* v_par = reinterpret_cast<const __half2*>(p.c.v_params);
+  constexpr int kRow = D / 2;                     // bytes of a token's codes
+  const uint8_t* k_lane = p.c.k_codes + g * kRow + j * (D / 8);
+  const uint8_t* v_lane = p.c.v_codes + 2 * j * kRow + g * (D / 16);
+  const uint32_t* kp_lane = reinterpret_cast<const uint32_t*>(p.c.k_params) + g;
+  const uint32_t* vp_lane = reinterpret_cast<const uint32_t*>(p.c.v_params) + g;
 
-  for (int ti = t_begin + warp; ti < t_end; ti += kWarps) {
-    const int t0 = range.tile(ti) * kTile;
-    // rows of the cache where the four pieces of 16 tokens begin; -1: not there
-    int64_t base[kSub];
-    bool whole = true;
+  // Rows of the cache where the four pieces of 16 tokens of a tile begin; -1: not there.  Pages of whole
+  // tiles are looked up once.
+  const bool whole_pages = p.c.page_size % kTile == 0;
+  auto place = [&](int t0, int64_t (&base)[kSub]) {
+    if (whole_pages) {
+      const int64_t first = kv4_place(p.c, table, p.max_pages, t0, head);
+#pragma unroll
+      for (int u = 0; u < kSub; ++u) base[u] = first >= 0 && t0 + 16 * u < length ? first + 16 * u : -1;
+    } else {
+#pragma unroll
+      for (int u = 0; u < kSub; ++u)
+        base[u] = t0 + 16 * u < length ? kv4_place(p.c, table, p.max_pages, t0 + 16 * u, head) : -1;
+    }
+  };
+  // Pieces that are not there are read from the cache's beginning, and masked.
+  uint32_t kw[kSub][2][KW], kp[kSub][2];
+  auto load_keys = [&](const int64_t (&base)[kSub]) {
 #pragma unroll
     for (int u = 0; u < kSub; ++u) {
-      base[u] = t0 + 16 * u < length ? kv4_place(p.c, table, p.max_pages, t0 + 16 * u, head) : -1;
-      whole &= base[u] >= 0;
+      const int64_t at = base[u] < 0 ? 0 : base[u];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        load_words<4 * KW>(k_lane + at * kRow + 8 * e * kRow, kw[u][e]);
+        kp[u][e] = __ldg(kp_lane + at + 8 * e);
+      }
     }
+  };
+
+  int64_t base[kSub];
+  int ti = t_begin + warp;
+  if (ti < t_end) {
+    place(range.tile(ti) * kTile, base);
+    load_keys(base);
+  }
+  for (; ti < t_end; ti += kWarps) {
+    const int t0 = range.tile(ti) * kTile;
+    bool whole = true;
+#pragma unroll
+    for (int u = 0; u < kSub; ++u) whole &= base[u] >= 0;
     // does every row see every token?
     whole &= t0 + kTile <= length;
     if (p.causal) whole &= t0 + kTile <= pos_lo + 1;
     if (p.window > 0) whole &= t0 > pos_hi - p.window || t0 + kTile <= p.sinks;
 
-    // ---- scores
-    float s[kSub][NT][4];
-    float2 kp[kSub][2], vp[kSub][2];
-    uint32_t kw[kSub][2][KW];
+    // ---- this tile's values are on their way while the scores are multiplied
+    uint32_t vw[kAllValues ? kSub : 1][4][VW], vp[kSub][2];
+    auto load_values = [&](int u) {
+      const int64_t at = base[u] < 0 ? 0 : base[u];
 #pragma unroll
-    for (int u = 0; u < kSub; ++u)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int64_t at = base[u] + g + 8 * e;
-        if (base[u] >= 0) {
-          load_words<4 * KW>(p.c.k_codes + at * row_bytes + j * (D / 8), kw[u][e]);
-        } else {
-#pragma unroll
-          for (int w = 0; w < KW; ++w) kw[u][e][w] = 0;
-        }
-      }
-#pragma unroll
-    for (int u = 0; u < kSub; ++u)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int64_t at = base[u] + g + 8 * e;
-        kp[u][e] = vp[u][e] = make_float2(0.0f, 0.0f);
-        if (base[u] >= 0 && t0 + 16 * u + g + 8 * e < length) {   // beyond the last token: whatever was there
-          kp[u][e] = __half22float2(__ldg(k_par + at));
-          vp[u][e] = __half22float2(__ldg(v_par + at));
-        }
-      }
+      for (int e = 0; e < 4; ++e)
+        load_words<4 * VW>(v_lane + at * kRow + ((e & 1) + 8 * (e >> 1)) * kRow, vw[kAllValues ? u : 0][e]);
+    };
 #pragma unroll
     for (int u = 0; u < kSub; ++u) {
+      const int64_t at = base[u] < 0 ? 0 : base[u];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) vp[u][e] = __ldg(vp_lane + at + 8 * e);
+      if (kAllValues) load_values(u);
+    }
+
+    // ---- scores, in units of 1 / a
+    float s[kSub][NT][4];
+#pragma unroll
+    for (int u = 0; u < kSub; ++u)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[u][nt][e] = 0.0f;
-    }
 #pragma unroll
     for (int w = 0; w < KW; ++w)
 #pragma unroll
@@ -293,101 +351,127 @@ kv4_attention_kernel(const AttnParams p) {
                       qf[pl][nt].x, qf[pl][nt].y);
         }
       }
-
-    // ---- value codes of the first piece are on their way while the softmax runs
-    uint32_t vw[4][VW];
-    auto load_values = [&](int u) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int64_t at = base[u] + 2 * j + (e & 1) + 8 * (e >> 1);
-        if (base[u] >= 0) {
-          load_words<4 * VW>(p.c.v_codes + at * row_bytes + g * (D / 16), vw[e]);
-        } else {
-#pragma unroll
-          for (int w = 0; w < VW; ++w) vw[e][w] = 0;
-        }
-      }
-    };
-    load_values(0);
-
-    // ---- softmax: scores in units of log2, reference = running maximum of score + exponent of s_v
-    float ev[kSub][2];
+    float2 kf[kSub][2], vf[kSub][2];
 #pragma unroll
     for (int u = 0; u < kSub; ++u)
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        ev[u][e] = (float)max((int)((__float_as_uint(vp[u][e].x) >> 23) & 255u) - 127, -24);
+      for (int e = 0; e < 2; ++e) {
+        kf[u][e] = half_values(kp[u][e]);
+        vf[u][e] = half_values(vp[u][e]);
+        if (!whole && (base[u] < 0 || t0 + 16 * u + g + 8 * e >= length))   // not there: whatever was read
+          kf[u][e] = vf[u][e] = make_float2(0.0f, 0.0f);
+      }
+
+    // ---- the next tile's keys
+    int64_t here[kSub];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int u = 0; u < kSub; ++u) here[u] = base[u];
+    if (ti + kWarps < t_end) {
+      place(range.tile(ti + kWarps) * kTile, base);
+      load_keys(base);
+    }
+
+    // ---- softmax: scores in units of log2, reference = running maximum of score + exponent of s_v
+    uint32_t pw[P][kSub][NT][2];                  // weights times s_v, fp16 pairs
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float top[2] = {-INFINITY, -INFINITY};
+      uint64_t x[kSub][2];
+#pragma unroll
+      for (int u = 0; u < kSub; ++u)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          x[u][e] = fma2(pack2(s[u][nt][2 * e], s[u][nt][2 * e + 1]), pack2(kf[u][e].x, kf[u][e].x),
+                         mul2(pack2(kf[u][e].y, kf[u][e].y), rb[nt]));
+          const float ev = (float)max((int)((__float_as_uint(vf[u][e].x) >> 23) & 255u) - 127, -24);
+          float2 r = unpack2(fma2(x[u][e], ra[nt], pack2(ev, ev)));
+          if (!whole) {
+            const int t = t0 + 16 * u + g + 8 * e;
+            const bool there = here[u] >= 0 && t < length;
+            if (!(there && sees(p, t, pos[nt][0]))) r.x = -INFINITY;
+            if (!(there && sees(p, t, pos[nt][1]))) r.y = -INFINITY;
+          }
+          top[0] = fmaxf(top[0], r.x);
+          top[1] = fmaxf(top[1], r.y);
+        }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        float top = -INFINITY;
+        top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 4));
+        top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 8));
+        top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 16));
+      }
+      if (top[0] > m_run[nt][0] || top[1] > m_run[nt][1]) {
+        float alpha[2];
 #pragma unroll
-        for (int u = 0; u < kSub; ++u)
+        for (int c = 0; c < 2; ++c) {
+          const bool more = top[c] > m_run[nt][c];
+          alpha[c] = more ? exp2_fast(m_run[nt][c] - top[c]) : 1.0f;      // 0 while nothing was seen
+          m_run[nt][c] = more ? top[c] : m_run[nt][c];
+        }
+        const uint64_t a2 = pack2(alpha[0], alpha[1]);
+        l_run[nt] = mul2(l_run[nt], a2);
+        s_run[nt] = mul2(s_run[nt], a2);
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float x = fmaf(kp[u][e].x, s[u][nt][2 * e + c] * ra[nt][c], kp[u][e].y * rb[nt][c]);
-            if (!whole) {
-              const int t = t0 + 16 * u + g + 8 * e;
-              bool sees = base[u] >= 0 && t < length;
-              if (p.causal) sees &= t <= pos[nt][c];
-              if (p.window > 0) sees &= t > pos[nt][c] - p.window || t < p.sinks;
-              if (!sees) x = -INFINITY;
-            }
-            s[u][nt][2 * e + c] = x;
-            top = fmaxf(top, x + ev[u][e]);
+        for (int i = 0; i < D / 16; ++i) {
+          o[i][nt][0] *= alpha[0];
+          o[i][nt][1] *= alpha[1];
+          o[i][nt][2] *= alpha[0];
+          o[i][nt][3] *= alpha[1];
+        }
+      }
+      const uint64_t ref = pack2(m_run[nt][0] == -INFINITY ? 0.0f : -m_run[nt][0],
+                                 m_run[nt][1] == -INFINITY ? 0.0f : -m_run[nt][1]);
+#pragma unroll
+      for (int u = 0; u < kSub; ++u)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float2 a = unpack2(fma2(x[u][e], ra[nt], ref));
+          float2 w = make_float2(exp2_fast(a.x), exp2_fast(a.y));
+          float vx = vf[u][e].x * 16384.0f, vx1 = vx, vy = vf[u][e].y, vy1 = vy;
+          if (!whole) {
+            // a hidden token's scale and minimum may be anything: its weight of 0 must not meet them
+            const int t = t0 + 16 * u + g + 8 * e;
+            const bool there = here[u] >= 0 && t < length;
+            if (!(there && sees(p, t, pos[nt][0]))) { w.x = 0.0f; vx = vy = 0.0f; }
+            if (!(there && sees(p, t, pos[nt][1]))) { w.y = 0.0f; vx1 = vy1 = 0.0f; }
           }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-        if (top > m_run[nt][c]) {
-          const float alpha = exp2_fast(m_run[nt][c] - top);      // 0 while nothing was seen
-          m_run[nt][c] = top;
-          l_run[nt][c] *= alpha;
-          s_run[nt][c] *= alpha;
-#pragma unroll
-          for (int i = 0; i < D / 16; ++i) {
-            o[i][nt][c] *= alpha;
-            o[i][nt][2 + c] *= alpha;
+          const uint64_t w2 = pack2(w.x, w.y);
+          l_run[nt] = add2(l_run[nt], w2);
+          s_run[nt] = fma2(w2, pack2(vy, vy1), s_run[nt]);
+          const float2 q = unpack2(mul2(w2, pack2(vx, vx1)));
+          const uint32_t h = half_pair(q.x, q.y);
+          pw[0][u][nt][e] = h;
+          if (P == 2) {
+            const float2 f = half_values(h);
+            pw[P - 1][u][nt][e] = half_pair(q.x - f.x, q.y - f.y);
           }
         }
-        const float ref = m_run[nt][c] == -INFINITY ? 0.0f : m_run[nt][c];
-#pragma unroll
-        for (int u = 0; u < kSub; ++u)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float x = s[u][nt][2 * e + c];
-            const float w = exp2_fast(x - ref);
-            l_run[nt][c] += w;
-            // a hidden token's scale and minimum may be anything: its weight of 0 must not meet them
-            s_run[nt][c] += x == -INFINITY ? 0.0f : w * vp[u][e].y;
-            s[u][nt][2 * e + c] = x == -INFINITY ? 0.0f : w * vp[u][e].x * 16384.0f;
-          }
-      }
+    }
 
     // ---- output
 #pragma unroll
     for (int u = 0; u < kSub; ++u) {
-      if (u > 0) load_values(u);
+      if (!kAllValues) {
+        const int64_t at = here[u] < 0 ? 0 : here[u];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          load_words<4 * VW>(v_lane + at * kRow + ((e & 1) + 8 * (e >> 1)) * kRow, vw[0][e]);
+      }
+      const auto& vu = vw[kAllValues ? u : 0];
       uint32_t b0[P][NT], b1[P][NT];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const float* x = s[u][nt];
-        const uint32_t h0 = half_pair(x[0], x[1]), h1 = half_pair(x[2], x[3]);
-        b0[0][nt] = transpose8(h0);
-        b1[0][nt] = transpose8(h1);
-        if (P == 2) {
-          const float2 f0 = half_values(h0), f1 = half_values(h1);
-          b0[P - 1][nt] = transpose8(half_pair(x[0] - f0.x, x[1] - f0.y));
-          b1[P - 1][nt] = transpose8(half_pair(x[2] - f1.x, x[3] - f1.y));
+      for (int pl = 0; pl < P; ++pl)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          b0[pl][nt] = transpose8(pw[pl][u][nt][0]);
+          b1[pl][nt] = transpose8(pw[pl][u][nt][1]);
         }
-      }
 #pragma unroll
       for (int w = 0; w < VW; ++w)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint32_t z0 = __byte_perm(vw[0][w], vw[1][w], h ? 0x7632 : 0x5410);
-          const uint32_t z1 = __byte_perm(vw[2][w], vw[3][w], h ? 0x7632 : 0x5410);
+          const uint32_t z0 = __byte_perm(vu[0][w], vu[1][w], h ? 0x7632 : 0x5410);
+          const uint32_t z1 = __byte_perm(vu[2][w], vu[3][w], h ? 0x7632 : 0x5410);
 #pragma unroll
           for (int h2 = 0; h2 < 2; ++h2) {
             const uint32_t y0 = h2 ? z0 >> 8 : z0, y1 = h2 ? z1 >> 8 : z1;
@@ -404,23 +488,22 @@ kv4_attention_kernel(const AttnParams p) {
 
   // ---- the warps' results joined: numerators in units of 2^m
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+  for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
-#pragma unroll
-      for (int sh = 4; sh < 32; sh <<= 1) {
-        l_run[nt][c] += __shfl_xor_sync(0xffffffffu, l_run[nt][c], sh);
-        s_run[nt][c] += __shfl_xor_sync(0xffffffffu, s_run[nt][c], sh);
-      }
-  if (g == 0) {
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        join_m[warp][8 * nt + 2 * j + c] = m_run[nt][c];
-        join_l[warp][8 * nt + 2 * j + c] = l_run[nt][c];
-        join_s[warp][8 * nt + 2 * j + c] = s_run[nt][c];
-      }
+    for (int sh = 4; sh < 32; sh <<= 1) {
+      l_run[nt] = add2(l_run[nt], __shfl_xor_sync(0xffffffffu, l_run[nt], sh));
+      s_run[nt] = add2(s_run[nt], __shfl_xor_sync(0xffffffffu, s_run[nt], sh));
+    }
+    if (g == 0) {
+      const int r = 8 * nt + 2 * j;
+      const float2 l = unpack2(l_run[nt]), sm = unpack2(s_run[nt]);
+      join_m[warp][r] = m_run[nt][0];
+      join_m[warp][r + 1] = m_run[nt][1];
+      join_l[warp][r] = l.x;
+      join_l[warp][r + 1] = l.y;
+      join_s[warp][r] = sm.x;
+      join_s[warp][r + 1] = sm.y;
+    }
   }
   __syncthreads();                                            // also: the query fragments are read
   float* o_sh = reinterpret_cast<float*>(smem);               // [warp][row][D + 4]
@@ -471,47 +554,74 @@ kv4_attention_kernel(const AttnParams p) {
   }
 }
 
-// The splits' partial results joined, in order; a thread owns four channels of a row.
-template <typename T>
-__global__ void __launch_bounds__(256)
-kv4_join_kernel(const float* __restrict__ part, T* __restrict__ out, int64_t rows, int dim, int splits) {
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int chunks = dim / 4;
-  if (idx >= rows * chunks) return;
-  const int64_t row = idx / chunks;
-  const int c4 = (int)(idx % chunks) * 4;
-  const float* l_at = part + (int64_t)splits * rows * dim + row;
+// The splits' partial results of one row joined: weights first, then the numerators, four channels a
+// thread, the splits dealt out to kGroups groups of threads whose sums are added in order.
+constexpr int kJoinThreads = 256;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinThreads)
+kv4_join_kernel(const float* __restrict__ part, T* __restrict__ out, int64_t rows, int splits) {
+  constexpr int kLanes = D / 4, kGroups = kJoinThreads / kLanes;
+  __shared__ float weight[kMaxSplits];
+  __shared__ float sh[32];
+  __shared__ float4 acc_sh[kGroups][kLanes];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int64_t row = blockIdx.x;
+  const float* l_at = part + (int64_t)splits * rows * D + row;
   const float* m_at = l_at + (int64_t)splits * rows;
-  float m = -INFINITY;
-  for (int s = 0; s < splits; ++s) m = fmaxf(m, m_at[s * rows]);
-  float l = 0.0f, acc[4] = {};
-  for (int s = 0; s < splits; ++s) {
-    const float ms = m_at[s * rows];
-    if (ms == -INFINITY) {
-      // nothing seen, or only scores that are not numbers: the sum says which
-      l += l_at[s * rows];
-      continue;
-    }
-    const float f = exp2_fast(ms - m);
-    float v[4];
-    load_f32<float, 4>(part + (s * rows + row) * dim + c4, v);
-    l = fmaf(f, l_at[s * rows], l);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] = fmaf(f, v[e], acc[e]);
+  float m = -INFINITY, ms = -INFINITY, l = 0.0f;
+  if (threadIdx.x < splits) {                          // splits <= kJoinThreads
+    m = ms = m_at[threadIdx.x * rows];
+    l = l_at[threadIdx.x * rows];
   }
-  const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = m;
+  __syncthreads();
 #pragma unroll
-  for (int e = 0; e < 4; ++e) acc[e] *= inv;
-  store_f32<T, 4>(out + row * dim + c4, acc);
+  for (int i = 0; i < kJoinThreads / 32; ++i) m = fmaxf(m, sh[i]);
+  // a part without a maximum saw nothing, or only scores that are not numbers: its sum says which
+  const float f = ms == -INFINITY ? 0.0f : exp2_fast(ms - m);
+  if (threadIdx.x < splits) weight[threadIdx.x] = f;
+  l = ms == -INFINITY ? l : f * l;
+  l = block_sum(l, sh);                                // a barrier inside: the weights are there
+  const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (group < kGroups) {
+#pragma unroll 4
+    for (int s = group; s < splits; s += kGroups) {
+      const float w = weight[s];
+      const float4 v = *reinterpret_cast<const float4*>(part + (s * rows + row) * D + 4 * lane);
+      acc.x = fmaf(w, v.x, acc.x);
+      acc.y = fmaf(w, v.y, acc.y);
+      acc.z = fmaf(w, v.z, acc.z);
+      acc.w = fmaf(w, v.w, acc.w);
+    }
+    acc_sh[group][lane] = acc;
+  }
+  __syncthreads();
+  if (threadIdx.x < kLanes) {
+    float v[4] = {};
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) {
+      const float4 a = acc_sh[i][threadIdx.x];
+      v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+    }
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] *= inv;
+    store_f32<T, 4>(out + row * D + 4 * threadIdx.x, v);
+  }
 }
 
-// Blocks per sequence and key head: enough to give every SM several, at least two tiles of a block's
-// warps each.  The lengths are on the device, so the table's width stands for the longest.
-int splits_for(int64_t blocks, int max_tokens) {
-  const int64_t want = ceil_div64(4ll * device_sms(), blocks);
-  const int64_t most = ceil_div64(max_tokens, 2 * kTile * kWarps);
+// Parts of the tokens of one sequence and key head: one round of blocks over all SMs if there are few of
+// them, else several, so that sequences of other lengths even out; every part at least one tile for each
+// warp.  The lengths are on the device, so the table's width stands for the longest.
+int splits_for(int64_t units, int max_tokens) {
+  const int64_t slots = 3ll * device_sms();            // three blocks of 168 registers a thread per SM
+  const int64_t want = 2 * units <= slots ? slots / units : ceil_div64(3 * slots, units);
+  const int64_t most = ceil_div64(max_tokens, kTile * kWarps);
   const int64_t s = want < most ? want : most;
-  return (int)(s < 1 ? 1 : (s > 64 ? 64 : s));
+  return (int)(s < 1 ? 1 : (s > kMaxSplits ? kMaxSplits : s));
 }
 
 int row_block(int rows, int dim) { return rows <= 8 ? 1 : (rows <= 16 || dim > 128 ? 2 : 4); }
@@ -541,9 +651,17 @@ int launch_attention(const AttnParams& p, int64_t blocks, cudaStream_t s) {
   kv4_attention_kernel<T, D, NT><<<(unsigned)blocks, kThreads, smem, s>>>(p);
   MODIFF_LAUNCH_CHECK("kv4_attention_kernel");
   if (p.splits > 1) {
-    const int64_t n = ceil_div64(p.rows * (D / 4), 256);
-    kv4_join_kernel<T><<<(unsigned)n, 256, 0, s>>>(p.part, static_cast<T*>(p.out), p.rows, D, p.splits);
-    MODIFF_LAUNCH_CHECK("kv4_join_kernel");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)p.rows);
+    cfg.blockDim = dim3(kJoinThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    MODIFF_CUDA(cudaLaunchKernelEx(&cfg, kv4_join_kernel<T, D>, (const float*)p.part, static_cast<T*>(p.out), p.rows,
+                                   p.splits));
   }
   return MODIFF_OK;
 }
