@@ -30,10 +30,12 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kTile = 64;                 // tokens a warp takes at a time
+constexpr int kTile = 32;                 // tokens a warp takes at a time
 constexpr int kSub = kTile / 16;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kExponentBias = 47.0f;    // of the exponents of s_v in the running maximum, see there
 constexpr int kMaxSplits = 256;
+constexpr int kBlocksPerSm = 4;           // of the single-token kernel: 128 registers a thread
 
 struct AttnParams {
   const void* q;
@@ -73,6 +75,20 @@ __device__ inline uint32_t half_pair(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ inline float2 half_values(uint32_t h) { return __half22float2(*reinterpret_cast<const __half2*>(&h)); }
+
+// Two channels of four codes out of a word: `even` the low halves of two bytes 16 bits apart, as n 2^-24,
+// `odd` the high halves, as 16 n 2^-24.  The even ones of the upper bytes come from a subtraction (exact),
+// because logic instructions, of half the rate of additions, are what this kernel has most of.
+__device__ inline void codes_lower(uint32_t w, uint32_t& even, uint32_t& odd) {
+  even = w & 0x000f000fu;
+  odd = w & 0x00f000f0u;
+}
+__device__ inline void codes_upper(uint32_t w, uint32_t& even, uint32_t& odd) {
+  const uint32_t t = __byte_perm(w, 0, 0x4341);
+  odd = t & 0x00f000f0u;
+  const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&t), *reinterpret_cast<const __half2*>(&odd));
+  even = *reinterpret_cast<const uint32_t*>(&d);
+}
 
 // pairs of fp32 values, one instruction for both
 __device__ inline uint64_t pack2(float a, float b) {
@@ -158,7 +174,7 @@ constexpr int smem_bytes() {
 // One block: 8 * NT query rows (query, head of the group) of one sequence and key head, one part of
 // the tokens.
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, NT > 1 || D > 128 ? 2 : kBlocksPerSm)
 kv4_attention_kernel(const AttnParams p) {
   constexpr int P = sizeof(T) == 4 ? 2 : 1;       // fp16 planes of q and of the weights
   constexpr int R = 8 * NT;
@@ -341,14 +357,19 @@ kv4_attention_kernel(const AttnParams p) {
                 &q_frag[(((pl * NT + nt) * (D / 16) + 2 * w + h) * 32 + lane) * 2]);
 #pragma unroll
         for (int u = 0; u < kSub; ++u) {
-          const uint32_t w0 = h ? kw[u][0][w] >> 8 : kw[u][0][w];
-          const uint32_t w1 = h ? kw[u][1][w] >> 8 : kw[u][1][w];
+          uint32_t e0, o0, e1, o1;
+          if (h) {
+            codes_upper(kw[u][0][w], e0, o0);
+            codes_upper(kw[u][1][w], e1, o1);
+          } else {
+            codes_lower(kw[u][0][w], e0, o0);
+            codes_lower(kw[u][1][w], e1, o1);
+          }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int pl = 0; pl < P; ++pl)
-              mma_f16(s[u][nt], w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u,
-                      qf[pl][nt].x, qf[pl][nt].y);
+              mma_f16(s[u][nt], e0, e1, o0, o1, qf[pl][nt].x, qf[pl][nt].y);
         }
       }
     float2 kf[kSub][2], vf[kSub][2];
@@ -383,7 +404,9 @@ kv4_attention_kernel(const AttnParams p) {
         for (int e = 0; e < 2; ++e) {
           x[u][e] = fma2(pack2(s[u][nt][2 * e], s[u][nt][2 * e + 1]), pack2(kf[u][e].x, kf[u][e].x),
                          mul2(pack2(kf[u][e].y, kf[u][e].y), rb[nt]));
-          const float ev = (float)max((int)((__float_as_uint(vf[u][e].x) >> 23) & 255u) - 127, -24);
+          // 32 + the exponent field of the fp16 scale, as a float: its true exponent + 47 (less for subnormal
+          // scales, which then only leave the weights some of their room)
+          const float ev = __uint_as_float(((vp[u][e] << 8) & 0x007c0000u) | 0x42000000u);
           float2 r = unpack2(fma2(x[u][e], ra[nt], pack2(ev, ev)));
           if (!whole) {
             const int t = t0 + 16 * u + g + 8 * e;
@@ -419,8 +442,8 @@ kv4_attention_kernel(const AttnParams p) {
           o[i][nt][3] *= alpha[1];
         }
       }
-      const uint64_t ref = pack2(m_run[nt][0] == -INFINITY ? 0.0f : -m_run[nt][0],
-                                 m_run[nt][1] == -INFINITY ? 0.0f : -m_run[nt][1]);
+      const uint64_t ref = pack2(m_run[nt][0] == -INFINITY ? 0.0f : kExponentBias - m_run[nt][0],
+                                 m_run[nt][1] == -INFINITY ? 0.0f : kExponentBias - m_run[nt][1]);
 #pragma unroll
       for (int u = 0; u < kSub; ++u)
 #pragma unroll
@@ -474,13 +497,19 @@ kv4_attention_kernel(const AttnParams p) {
           const uint32_t z1 = __byte_perm(vu[2][w], vu[3][w], h ? 0x7632 : 0x5410);
 #pragma unroll
           for (int h2 = 0; h2 < 2; ++h2) {
-            const uint32_t y0 = h2 ? z0 >> 8 : z0, y1 = h2 ? z1 >> 8 : z1;
+            uint32_t e0, o0, e1, o1;
+            if (h2) {
+              codes_upper(z0, e0, o0);
+              codes_upper(z1, e1, o1);
+            } else {
+              codes_lower(z0, e0, o0);
+              codes_lower(z1, e1, o1);
+            }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int pl = 0; pl < P; ++pl)
-                mma_f16(o[4 * w + 2 * h + h2][nt], y0 & 0x000f000fu, y0 & 0x00f000f0u, y1 & 0x000f000fu,
-                        y1 & 0x00f000f0u, b0[pl][nt], b1[pl][nt]);
+                mma_f16(o[4 * w + 2 * h + h2][nt], e0, o0, e1, o1, b0[pl][nt], b1[pl][nt]);
           }
         }
     }
@@ -617,7 +646,7 @@ kv4_join_kernel(const float* __restrict__ part, T* __restrict__ out, int64_t row
 // them, else several, so that sequences of other lengths even out; every part at least one tile for each
 // warp.  The lengths are on the device, so the table's width stands for the longest.
 int splits_for(int64_t units, int max_tokens) {
-  const int64_t slots = 3ll * device_sms();            // three blocks of 168 registers a thread per SM
+  const int64_t slots = (int64_t)kBlocksPerSm * device_sms();
   const int64_t want = 2 * units <= slots ? slots / units : ceil_div64(3 * slots, units);
   const int64_t most = ceil_div64(max_tokens, kTile * kWarps);
   const int64_t s = want < most ? want : most;
