@@ -705,7 +705,7 @@ int modiff_kv4_append(const modiff_kv4_cache* cache, const void* k, int64_t k_se
 int modiff_kv4_read(const modiff_kv4_cache* cache, const int32_t* table, const int32_t* lengths, int batch,
                     int count, int max_pages, void* k, void* v, int dtype, void* stream);
 int64_t modiff_kv4_attention_bytes(const modiff_kv4_cache* cache, int batch, int count, int heads,
-                                   int max_pages, int window, int sinks);
+                                   int max_pages, int window, int sinks, int dtype);
 int modiff_kv4_attention(const void* q, int64_t q_seq, int64_t q_token, int64_t q_head,
                          const modiff_kv4_cache* cache, const int32_t* table, const int32_t* lengths, void* out, int batch, int count,
                          int heads, int max_pages, float scale, int causal, int window, int sinks,

@@ -167,7 +167,7 @@ SIGNATURES = {
     "modiff_kv4_append": (C.c_int, [_KV4] + [_P, C.c_int64, C.c_int64, C.c_int64] * 2 + [_P, _P] +
                           [C.c_int] * 4 + [_P]),
     "modiff_kv4_read": (C.c_int, [_KV4, _P, _P, C.c_int, C.c_int, C.c_int, _P, _P, C.c_int, _P]),
-    "modiff_kv4_attention_bytes": (C.c_int64, [_KV4] + [C.c_int] * 6),
+    "modiff_kv4_attention_bytes": (C.c_int64, [_KV4] + [C.c_int] * 7),
     "modiff_kv4_attention": (C.c_int, [_P, C.c_int64, C.c_int64, C.c_int64, _KV4, _P, _P, _P, C.c_int,
                                        C.c_int, C.c_int, C.c_int,
                                        C.c_float, C.c_int, C.c_int, C.c_int, C.c_int, _P, _P]),

@@ -843,6 +843,7 @@ int read_device_status_attention_i8(int* status, int reset);   // attention_i8.c
 int read_device_status_conv_f32(int* status, int reset);       // conv_f32_tc.cu
 int read_device_status_fp8(int* status, int reset);            // fp8_linear.cu
 int read_device_status_fp8_pair(int* status, int reset);       // fp8_linear_pair.cu
+int read_device_status_kv4(int* status, int reset);            // kv4_attention_tc.cu
 bool pair_supported(const modiff_conv_geom* g, int with_sum_rows, int per_sample, const float* bias,
                     const int32_t* acc_out, const float* o_hat);
 int launch_igemm_pair(const int8_t* codes, const int8_t* wcodes, int with_sum_rows,
@@ -904,7 +905,10 @@ int read_device_status(int* status, int reset) {
   int f8p = 0;
   rc = read_device_status_fp8_pair(&f8p, reset);
   if (rc) return rc;
-  *status = a | b | c | d | e | f | h | i8 | f32 | f8 | f8p;
+  int k4 = 0;
+  rc = read_device_status_kv4(&k4, reset);
+  if (rc) return rc;
+  *status = a | b | c | d | e | f | h | i8 | f32 | f8 | f8p | k4;
   return MODIFF_OK;
 }
 

@@ -37,20 +37,6 @@ constexpr float kExponentBias = 47.0f;    // of the exponents of s_v in the runn
 constexpr int kMaxSplits = 256;
 constexpr int kBlocksPerSm = 4;           // of the single-token kernel: 128 registers a thread
 
-struct AttnParams {
-  const void* q;
-  int64_t qb, qt, qh;                     // element strides: sequence, token, head
-  void* out;                              // [batch][count][heads][dim]
-  float* part;                            // [splits][rows][dim], then sums and maxima [splits][rows] each
-  Kv4Pages c;
-  const int32_t* table;
-  const int32_t* lengths;
-  int batch, count, heads, group, max_pages, splits, row_tiles;
-  int causal, window, sinks;
-  float scale2;                           // scale * log2(e)
-  int64_t rows;                           // batch * count * heads
-};
-
 __device__ inline void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                uint32_t b1) {
   asm volatile(
@@ -65,17 +51,6 @@ __device__ inline uint32_t transpose8(uint32_t v) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-__device__ inline float exp2_fast(float x) {   // hardware exp2, relative error about 2^-22
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-__device__ inline uint32_t half_pair(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ inline float2 half_values(uint32_t h) { return __half22float2(*reinterpret_cast<const __half2*>(&h)); }
-
 // Two channels of four codes out of a word: `even` the low halves of two bytes 16 bits apart, as n 2^-24,
 // `odd` the high halves, as 16 n 2^-24.  The even ones of the upper bytes come from a subtraction (exact),
 // because logic instructions, of half the rate of additions, are what this kernel has most of.
@@ -90,79 +65,6 @@ __device__ inline void codes_upper(uint32_t w, uint32_t& even, uint32_t& odd) {
   even = *reinterpret_cast<const uint32_t*>(&d);
 }
 
-// pairs of fp32 values, one instruction for both
-__device__ inline uint64_t pack2(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ inline float2 unpack2(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ inline uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ inline uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ inline uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-
-template <int BYTES>
-__device__ inline void load_words(const uint8_t* src, uint32_t (&w)[BYTES / 4]) {
-  if constexpr (BYTES % 16 == 0) {
-#pragma unroll
-    for (int i = 0; i < BYTES / 16; ++i) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + i);
-      w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
-    }
-  } else if constexpr (BYTES % 8 == 0) {
-#pragma unroll
-    for (int i = 0; i < BYTES / 8; ++i) {
-      const uint2 v = __ldg(reinterpret_cast<const uint2*>(src) + i);
-      w[2 * i] = v.x; w[2 * i + 1] = v.y;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < BYTES / 4; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(src) + i);
-  }
-}
-
-// Tiles of kTile tokens that rows at positions [p_lo, p_hi] see any of: `first` tiles from 0 on (the
-// sinks), the others from tile `start` on.
-struct TileRange {
-  int first, start, count;
-  __device__ int tile(int i) const { return i < first ? i : start + (i - first); }
-};
-__device__ inline TileRange tiles_of(const AttnParams& p, int length, int p_lo, int p_hi) {
-  TileRange r;
-  const int end = p.causal ? min(length, p_hi + 1) : length;
-  int lo = 0, sink_end = 0;
-  if (p.window > 0) {
-    lo = max(0, p_lo - p.window + 1);
-    sink_end = min(min(p.sinks, lo), max(end, 0));
-  }
-  r.first = (sink_end + kTile - 1) / kTile;
-  r.start = max(lo / kTile, r.first);
-  const int last = end > 0 ? (end + kTile - 1) / kTile : 0;
-  r.count = r.first + max(0, last - r.start);
-  return r;
-}
-
-__device__ inline bool sees(const AttnParams& p, int t, int pos) {
-  if (p.causal && t > pos) return false;
-  return p.window <= 0 || t > pos - p.window || t < p.sinks;
-}
-
 template <typename T, int D, int NT>
 constexpr int smem_bytes() {
   constexpr int planes = sizeof(T) == 4 ? 2 : 1;
@@ -175,7 +77,7 @@ constexpr int smem_bytes() {
 // the tokens.
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kThreads, NT > 1 || D > 128 ? 2 : kBlocksPerSm)
-kv4_attention_kernel(const AttnParams p) {
+kv4_attention_kernel(const Kv4Attention p) {
   constexpr int P = sizeof(T) == 4 ? 2 : 1;       // fp16 planes of q and of the weights
   constexpr int R = 8 * NT;
   constexpr int KW = D / 32;                      // words of a key row that a thread holds
@@ -246,7 +148,7 @@ kv4_attention_kernel(const AttnParams p) {
 
   const int pos_lo = length - p.count + row0 / p.group;
   const int pos_hi = length - p.count + (row0 + rows_here - 1) / p.group;
-  const TileRange range = tiles_of(p, length, pos_lo, pos_hi);
+  const TileRange range = tiles_of<kTile>(p, length, pos_lo, pos_hi);
   const int t_begin = (int)((int64_t)range.count * split / p.splits);
   const int t_end = (int)((int64_t)range.count * (split + 1) / p.splits);
 
@@ -643,12 +545,12 @@ kv4_join_kernel(const float* __restrict__ part, T* __restrict__ out, int64_t row
 }
 
 // Parts of the tokens of one sequence and key head: one round of blocks over all SMs if there are few of
-// them, else several, so that sequences of other lengths even out; every part at least one tile for each
-// warp.  The lengths are on the device, so the table's width stands for the longest.
-int splits_for(int64_t units, int max_tokens) {
-  const int64_t slots = (int64_t)kBlocksPerSm * device_sms();
+// them, else several, so that sequences of other lengths even out; every part at least `least` tokens.  The
+// lengths are on the device, so the table's width stands for the longest.
+int splits_for(int64_t units, int max_tokens, int per_sm, int least) {
+  const int64_t slots = (int64_t)per_sm * device_sms();
   const int64_t want = 2 * units <= slots ? slots / units : ceil_div64(3 * slots, units);
-  const int64_t most = ceil_div64(max_tokens, kTile * kWarps);
+  const int64_t most = max_tokens / least;
   const int64_t s = want < most ? want : most;
   return (int)(s < 1 ? 1 : (s > kMaxSplits ? kMaxSplits : s));
 }
@@ -657,46 +559,58 @@ int row_block(int rows, int dim) { return rows <= 8 ? 1 : (rows <= 16 || dim > 1
 
 struct Plan {
   int nt, row_tiles, splits;
+  bool tc;                              // the tensor-core kernel for many rows
   int64_t blocks;
 };
-Plan plan_of(const modiff_kv4_cache* c, int batch, int count, int heads, int max_pages, int window, int sinks) {
+Plan plan_of(const modiff_kv4_cache* c, int batch, int count, int heads, int max_pages, int window, int sinks,
+             int dtype) {
   Plan pl;
   const int rows = count * (heads / c->heads);
+  pl.tc = kv4_tc_wanted(rows, c->dim, dtype);
   pl.nt = row_block(rows, c->dim);
-  pl.row_tiles = ceil_div(rows, 8 * pl.nt);
+  const int tile = pl.tc ? kv4_tc_rows() : 8 * pl.nt;
+  pl.row_tiles = ceil_div(rows, tile);
   const int64_t units = (int64_t)batch * c->heads * pl.row_tiles;
   int64_t tokens = (int64_t)max_pages * c->page_size;
-  if (window > 0 && (int64_t)window + sinks + 8 * pl.nt < tokens) tokens = (int64_t)window + sinks + 8 * pl.nt;
-  pl.splits = splits_for(units, (int)tokens);
+  if (window > 0 && (int64_t)window + sinks + tile < tokens) tokens = (int64_t)window + sinks + tile;
+  pl.splits = splits_for(units, (int)tokens, pl.tc ? 1 : kBlocksPerSm, pl.tc ? 1024 : 4 * kTile * kWarps);
   pl.blocks = units * pl.splits;
   return pl;
 }
 
+template <typename T, int D>
+int join(const Kv4Attention& p, cudaStream_t s) {
+  if (p.splits == 1) return MODIFF_OK;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)p.rows);
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  MODIFF_CUDA(cudaLaunchKernelEx(&cfg, kv4_join_kernel<T, D>, (const float*)p.part, static_cast<T*>(p.out), p.rows,
+                                 p.splits));
+  return MODIFF_OK;
+}
+
 template <typename T, int D, int NT>
-int launch_attention(const AttnParams& p, int64_t blocks, cudaStream_t s) {
+int launch_attention(const Kv4Attention& p, int64_t blocks, cudaStream_t s) {
   constexpr int smem = smem_bytes<T, D, NT>();
   static SmemLimit limit;
   MODIFF_CUDA(raise_smem_limit(kv4_attention_kernel<T, D, NT>, smem, limit));
   kv4_attention_kernel<T, D, NT><<<(unsigned)blocks, kThreads, smem, s>>>(p);
   MODIFF_LAUNCH_CHECK("kv4_attention_kernel");
-  if (p.splits > 1) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)p.rows);
-    cfg.blockDim = dim3(kJoinThreads);
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    MODIFF_CUDA(cudaLaunchKernelEx(&cfg, kv4_join_kernel<T, D>, (const float*)p.part, static_cast<T*>(p.out), p.rows,
-                                   p.splits));
-  }
-  return MODIFF_OK;
+  return join<T, D>(p, s);
 }
 
 template <typename T, int D>
-int by_rows(const AttnParams& p, const Plan& pl, cudaStream_t s) {
+int by_rows(const Kv4Attention& p, const Plan& pl, int dtype, cudaStream_t s) {
+  if (pl.tc) {
+    const int rc = kv4_launch_tc(p, dtype, s);
+    return rc ? rc : join<T, D>(p, s);
+  }
   if (pl.nt == 1) return launch_attention<T, D, 1>(p, pl.blocks, s);
   if (pl.nt == 2) return launch_attention<T, D, 2>(p, pl.blocks, s);
   if constexpr (D <= 128) return launch_attention<T, D, 4>(p, pl.blocks, s);
@@ -716,9 +630,9 @@ int check_shape(const modiff_kv4_cache* c, int batch, int count, int heads) {
 using namespace modiff;
 
 extern "C" int64_t modiff_kv4_attention_bytes(const modiff_kv4_cache* cache, int batch, int count, int heads,
-                                              int max_pages, int window, int sinks) {
-  if (!cache || cache->heads <= 0 || batch <= 0 || count <= 0 || check_shape(cache, batch, count, heads)) return 0;
-  const Plan pl = plan_of(cache, batch, count, heads, max_pages, window, sinks);
+                                              int max_pages, int window, int sinks, int dtype) {
+  if (!cache || !dtype_ok(dtype) || cache->heads <= 0 || batch <= 0 || count <= 0 || check_shape(cache, batch, count, heads)) return 0;
+  const Plan pl = plan_of(cache, batch, count, heads, max_pages, window, sinks, dtype);
   if (pl.splits == 1) return 0;
   return 4ll * pl.splits * batch * count * heads * (cache->dim + 2);
 }
@@ -738,10 +652,10 @@ extern "C" int modiff_kv4_attention(const void* q, int64_t q_seq, int64_t q_toke
   MODIFF_CHECK_ARG(q && out, "NULL pointer argument");
   const int size = dtype_bytes(dtype);
   MODIFF_CHECK_ARG((uintptr_t)q % size == 0 && (uintptr_t)out % 16 == 0, "misaligned tensor");
-  const Plan pl = plan_of(cache, batch, count, heads, max_pages, window, sinks);
+  const Plan pl = plan_of(cache, batch, count, heads, max_pages, window, sinks, dtype);
   MODIFF_CHECK_ARG(pl.blocks <= 0x7fffffff, "too many query rows");
   MODIFF_CHECK_ARG(pl.splits == 1 || (workspace && (uintptr_t)workspace % 16 == 0), "NULL or misaligned workspace");
-  AttnParams p;
+  Kv4Attention p;
   p.q = q;
   p.qb = q_seq; p.qt = q_token; p.qh = q_head;
   p.out = out;
@@ -762,10 +676,10 @@ extern "C" int modiff_kv4_attention(const void* q, int64_t q_seq, int64_t q_toke
   return with_dtype(dtype, [&](auto tag) {
     using T = decltype(tag);
     switch (cache->dim) {
-      case 64: return by_rows<T, 64>(p, pl, st);
-      case 128: return by_rows<T, 128>(p, pl, st);
-      case 192: return by_rows<T, 192>(p, pl, st);
-      default: return by_rows<T, 256>(p, pl, st);
+      case 64: return by_rows<T, 64>(p, pl, dtype, st);
+      case 128: return by_rows<T, 128>(p, pl, dtype, st);
+      case 192: return by_rows<T, 192>(p, pl, dtype, st);
+      default: return by_rows<T, 256>(p, pl, dtype, st);
     }
   });
 }

@@ -1,0 +1,491 @@
+// Attention over the 4-bit cache for many query rows per key head (prompts and pieces of them), on the
+// 5th-generation tensor cores.  Same result as kv4_attention.cu, fp16 and bf16 tensors.
+//
+// A block owns 256 query rows (query, head of the group) of one sequence and key head, as two groups of
+// 128, and walks the keys in tiles of 128 that both groups share:
+//   four loader warps read the codes through the page table and write keys and values as fp16 numbers
+//   s code + m, rounded once, as operands of an MMA (128-byte swizzle; a key's channels stay in its row,
+//   which is K-major for the scores and N-major for the output; eight channels of a word lie in the
+//   order 0 4 1 5 2 6 3 7, in which they come out of it, and so do the queries');
+//   one warp issues S = Q K^T into tensor memory (128 columns a group) and O += P V, with P read from
+//   tensor memory, where the softmax has put it in place of S;
+//   four softmax warps a group, a thread per row, no exchange between threads: maximum, then weights.
+//   O is rescaled only when a row's maximum has grown by more than 2^8; weights are fp16 in units of
+//   2^(reference - 6), at most 2^14.
+// While one group's softmax runs the tensor pipe works for the other.
+//
+// Queries are brought to fp16 by a power of two per row (exact for bf16).  A value that is not finite is
+// replaced by zero and makes the rows that see it NaN, so that rows that do not see it never meet it.
+//
+// Bound: tensor pipe (2048 cycles a tile of 128 keys and 256 rows of 128 channels); the loaders need about
+// 500 issue slots of a scheduler for it, the softmax about 1000.
+#include "kv4.cuh"
+#include "tc_common.cuh"
+
+namespace modiff {
+
+int read_device_status_kv4(int* status, int reset) { return read_status_this_unit(status, reset); }
+
+namespace {
+
+constexpr int kKeys = 128;                  // keys of a tile
+constexpr int kRows = 256;                  // query rows of a block
+constexpr int kLoaders = 4;                 // warps 0 .. 3; softmax warps 4 .. 11; MMA warp 12
+constexpr int kMmaWarp = 12;
+constexpr int kThreads = 32 * (kMmaWarp + 1);
+constexpr int kChunk = kKeys * 128;         // bytes of 128 rows of 64 channels
+constexpr float kGrowth = 8.0f;             // of a row's maximum, in powers of two, before O is rescaled
+constexpr float kRoom = 6.0f;               // weights are at most 2^(kGrowth + kRoom)
+constexpr int kBitSlots = 4;
+
+// fp16 x fp16 -> fp32, A from tensor memory
+__device__ inline void tc_mma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                     uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ inline void tc_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+// Instruction descriptor of kind::f16 with fp16 operands and fp32 accumulation; B K-major or N-major.
+__host__ __device__ inline uint32_t make_idesc_f16(int m, int n, bool b_n_major) {
+  return (1u << 4) | (b_n_major ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+// Operand whose rows of 128 bytes are steps of K (N-major): 64-element pieces of N `kChunk` apart, groups of
+// eight rows 1024 bytes apart.
+__device__ inline uint64_t make_n_major_desc(uint32_t saddr) {
+  uint64_t d = make_smem_desc(saddr);
+  d &= ~((uint64_t)0x3fff << 16);
+  d |= (uint64_t)(kChunk >> 4) << 16;
+  return d;
+}
+
+__device__ inline __half2 as_half2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
+__device__ inline uint32_t as_u32(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
+
+// One word of eight codes as fp16 values s code + m.  1024 + n is the fp16 number 0x6400 | n, and 1024 + 16 n
+// that of the other half of a byte; taking 1024 (and the factor) out again is exact.
+template <bool CLAMP>
+__device__ inline uint4 dequantise(uint32_t w, __half2 s, __half2 m) {
+  const __half2 k1024 = as_half2(0x64006400u), k16th = as_half2(0x2c002c00u), k64 = as_half2(0xd400d400u);   // 1024, 1/16, -64
+  __half2 v[4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t x = i ? w >> 8 : w;
+    v[2 * i] = __hfma2(__hsub2(as_half2((x & 0x000f000fu) | 0x64006400u), k1024), s, m);
+    v[2 * i + 1] = __hfma2(__hfma2(as_half2((x & 0x00f000f0u) | 0x64006400u), k16th, k64), s, m);
+  }
+  if (CLAMP) {
+    // s rounded up can carry the largest code past fp16's range
+    const __half2 top = as_half2(0x7bff7bffu), low = as_half2(0xfbfffbffu);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __hmin2(__hmax2(v[i], low), top);
+  }
+  return make_uint4(as_u32(v[0]), as_u32(v[1]), as_u32(v[2]), as_u32(v[3]));
+}
+
+// A row of codes into its place of an operand tile.
+template <int D>
+__device__ inline void store_row(uint8_t* tile, int row, const uint32_t (&w)[D / 8], uint32_t params, bool there) {
+  const __half2 sm = as_half2(params);
+  const __half2 s = __low2half2(sm), m = __high2half2(sm);
+  const float2 f = half_values(params);
+  const bool edge = fabsf(f.y) > 65000.0f || fabsf(fmaf(15.0f, f.x, f.y)) > 65000.0f;
+  uint8_t* base = tile + row * 128;
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i) {
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (there) v = edge ? dequantise<true>(w[i], s, m) : dequantise<false>(w[i], s, m);
+    *reinterpret_cast<uint4*>(base + (i >> 3) * kChunk + (((i & 7) ^ (row & 7)) << 4)) = v;
+  }
+}
+
+// low bits [0, n) of a word, n clamped to 0 .. 32
+__device__ inline uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u); }
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+kv4_attention_tc_kernel(const Kv4Attention p) {
+  constexpr int kQTile = 128 * D * 2, kKvTile = kKeys * D * 2;
+  extern __shared__ __align__(1024) uint8_t smem[];          // Q [2], K [2], V [2]
+  __shared__ __align__(8) uint64_t bar_k_full[2], bar_k_empty[2], bar_v_full[2], bar_v_empty[2];
+  __shared__ __align__(8) uint64_t bar_s_full[2], bar_p_ready[2], bar_bits[kBitSlots], bar_o_full;
+  __shared__ uint32_t there_sh[kBitSlots][4], bad_sh[kBitSlots][4];   // tokens that exist; values that are not finite
+  __shared__ float row_a[kRows];
+  __shared__ uint32_t tmem_base_sh;
+  __shared__ int abort_sh;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int* abort_flag = &abort_sh;
+  uint8_t* q_sh = smem;
+  uint8_t* k_sh = smem + 2 * kQTile;
+  uint8_t* v_sh = k_sh + 2 * kKvTile;
+
+  if (p.splits > 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  int id = blockIdx.x;
+  const int split = id % p.splits;
+  id /= p.splits;
+  // the last rows of a causal call have the most keys: they start first
+  const int rt = p.row_tiles - 1 - id % p.row_tiles;
+  id /= p.row_tiles;
+  const int head = id % p.c.heads, b = id / p.c.heads;
+  const int row0 = rt * kRows;
+  const int rows_here = min(kRows, p.count * p.group - row0);
+  const bool two = rows_here > 128;
+  const int32_t* table = p.table + (int64_t)b * p.max_pages;
+  const int length = min(max(__ldg(p.lengths + b), 0), p.max_pages * p.c.page_size);
+  const int pos_lo = length - p.count + row0 / p.group;
+  const int pos_hi = length - p.count + (row0 + rows_here - 1) / p.group;
+  const TileRange range = tiles_of<kKeys>(p, length, pos_lo, pos_hi);
+  const int t_begin = (int)((int64_t)range.count * split / p.splits);
+  const int tiles = (int)((int64_t)range.count * (split + 1) / p.splits) - t_begin;
+
+  if (threadIdx.x == 0) {
+    abort_sh = 0;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&bar_k_full[i]), kLoaders);
+      mbar_init(smem_u32(&bar_k_empty[i]), 1);
+      mbar_init(smem_u32(&bar_v_full[i]), kLoaders);
+      mbar_init(smem_u32(&bar_v_empty[i]), 1);
+      mbar_init(smem_u32(&bar_s_full[i]), 1);
+      mbar_init(smem_u32(&bar_p_ready[i]), 4);
+    }
+    for (int i = 0; i < kBitSlots; ++i) mbar_init(smem_u32(&bar_bits[i]), kLoaders);
+    mbar_init(smem_u32(&bar_o_full), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_sh)),
+                 "r"(512u)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  // ---- queries, one warp a row
+  const float sign = p.scale2 < 0.0f ? -1.0f : 1.0f;           // the scale's sign goes into the queries
+  for (int r = warp; r < (two ? kRows : 128); r += kMmaWarp + 1) {
+    const int rr = row0 + r;
+    const bool real = r < rows_here;
+    const T* src = static_cast<const T*>(p.q) + (int64_t)b * p.qb + (int64_t)(rr / p.group) * p.qt +
+                   (int64_t)(head * p.group + rr % p.group) * p.qh;
+    float x[D / 32];
+    float top = 0.0f;
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) {
+      x[e] = real ? to_f32<T>(src[lane + 32 * e]) : 0.0f;
+      top = fmaxf(top, fabsf(x[e]));
+    }
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    // power of two that brings the largest element to [2^14, 2^15); in two factors, for bf16's range
+    int e2 = 0;
+    if (top > 0.0f && top < INFINITY) { frexpf(top, &e2); e2 = 15 - e2; }
+    const float f1 = ldexpf(sign, e2 / 2), f2 = ldexpf(1.0f, e2 - e2 / 2);
+    if (lane == 0) row_a[r] = p.scale2 / f1 / f2;
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) {
+      const int ch = lane + 32 * e, w = (ch & 63) >> 3, n = ch & 7;
+      const int at = ((n & 3) << 1) | (n >> 2);                // 0 4 1 5 2 6 3 7
+      uint8_t* dst = q_sh + (r >> 7) * kQTile + (ch >> 6) * kChunk + (r & 127) * 128 + ((w ^ (r & 7)) << 4) + 2 * at;
+      *reinterpret_cast<__half*>(dst) = __float2half_rn(x[e] * f1 * f2);
+    }
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = tmem_base_sh;
+
+  if (warp < kLoaders) {
+    // ------------------------------------------------------------ keys and values
+    const int key = threadIdx.x;
+    uint32_t kw[D / 8], vw[D / 8], kp = 0, vp = 0;
+    int64_t place = -1, next = -1;
+    auto find = [&](int i) -> int64_t {
+      const int t = range.tile(t_begin + i) * kKeys + key;
+      return t < length ? kv4_place(p.c, table, p.max_pages, t, head) : -1;
+    };
+    auto load_keys = [&](int64_t at) {
+      const int64_t a = at < 0 ? 0 : at;                       // what is not there is read from the beginning
+      load_words<D / 2>(p.c.k_codes + a * (D / 2), kw);
+      kp = __ldg(reinterpret_cast<const uint32_t*>(p.c.k_params) + a);
+    };
+    auto load_values = [&](int64_t at) {
+      const int64_t a = at < 0 ? 0 : at;
+      load_words<D / 2>(p.c.v_codes + a * (D / 2), vw);
+      vp = __ldg(reinterpret_cast<const uint32_t*>(p.c.v_params) + a);
+    };
+    if (tiles > 0) {
+      place = find(0);
+      load_keys(place);
+      load_values(place);
+    }
+    for (int i = 0; i < tiles; ++i) {
+      const int st = i & 1;
+      const uint32_t phase = (uint32_t)(i >> 1) & 1u;
+      if (i + 1 < tiles) next = find(i + 1);
+      if (!mbar_wait(smem_u32(&bar_k_empty[st]), phase ^ 1u, abort_flag)) break;
+      store_row<D>(k_sh + st * kKvTile, key, kw, kp, place >= 0);
+      // exponent field of all ones: infinity or NaN
+      const bool bad = place >= 0 && ((vp & 0x7c00u) == 0x7c00u || (vp & 0x7c000000u) == 0x7c000000u);
+      const uint32_t there_bits = __ballot_sync(0xffffffffu, place >= 0), bad_bits = __ballot_sync(0xffffffffu, bad);
+      if (lane == 0) {
+        there_sh[i % kBitSlots][warp] = there_bits;
+        bad_sh[i % kBitSlots][warp] = bad_bits;
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(smem_u32(&bar_bits[i % kBitSlots]));
+        mbar_arrive(smem_u32(&bar_k_full[st]));
+      }
+      if (i + 1 < tiles) load_keys(next);
+      if (!mbar_wait(smem_u32(&bar_v_empty[st]), phase ^ 1u, abort_flag)) break;
+      store_row<D>(v_sh + st * kKvTile, key, vw, vp, place >= 0 && !bad);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&bar_v_full[st]));
+      if (i + 1 < tiles) load_values(next);
+      place = next;
+    }
+    __syncwarp();
+  } else if (warp == kMmaWarp) {
+    // ------------------------------------------------------------ MMAs
+    const uint32_t idesc_s = make_idesc_f16(128, kKeys, false), idesc_o = make_idesc_f16(128, D, true);
+    const uint32_t q_addr = smem_u32(q_sh), k_addr = smem_u32(k_sh), v_addr = smem_u32(v_sh);
+    const int groups = two ? 2 : 1;
+    auto scores = [&](int g, int st) {
+      if (elect_one()) {
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+          const uint64_t a = make_smem_desc(q_addr + g * kQTile + c * kChunk);
+          const uint64_t kd = make_smem_desc(k_addr + st * kKvTile + c * kChunk);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            tc_mma_bf16(tmem_base + (uint32_t)(128 * g), a + (uint64_t)(2 * k), kd + (uint64_t)(2 * k), idesc_s,
+                        c > 0 || k > 0 ? 1u : 0u);
+        }
+        tc_commit(smem_u32(&bar_s_full[g]));
+      }
+      __syncwarp();
+    };
+    bool ok = true;
+    if (tiles > 0) {
+      ok = mbar_wait(smem_u32(&bar_k_full[0]), 0, abort_flag);
+      if (ok) {
+        tc_fence_after();
+        for (int g = 0; g < groups; ++g) scores(g, 0);
+        if (elect_one()) tc_commit(smem_u32(&bar_k_empty[0]));
+        __syncwarp();
+      }
+    }
+    for (int i = 0; i < tiles && ok; ++i) {
+      const int st = i & 1;
+      ok = mbar_wait(smem_u32(&bar_v_full[st]), (uint32_t)(i >> 1) & 1u, abort_flag);
+      if (ok && i + 1 < tiles) ok = mbar_wait(smem_u32(&bar_k_full[st ^ 1]), (uint32_t)((i + 1) >> 1) & 1u, abort_flag);
+      for (int g = 0; g < groups && ok; ++g) {
+        ok = mbar_wait(smem_u32(&bar_p_ready[g]), (uint32_t)i & 1u, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t vd = make_n_major_desc(v_addr + st * kKvTile);
+#pragma unroll
+          for (int k = 0; k < kKeys / 16; ++k)
+            tc_mma_f16_ta(tmem_base + (uint32_t)(256 + 128 * g), tmem_base + (uint32_t)(128 * g + 8 * k),
+                          vd + (uint64_t)(k * (16 * 128 >> 4)), idesc_o, i > 0 || k > 0 ? 1u : 0u);
+        }
+        __syncwarp();
+        if (i + 1 < tiles) scores(g, st ^ 1);
+      }
+      if (!ok) break;
+      if (elect_one()) {
+        tc_commit(smem_u32(&bar_v_empty[st]));
+        if (i + 1 < tiles) tc_commit(smem_u32(&bar_k_empty[st ^ 1]));
+        if (i == tiles - 1) tc_commit(smem_u32(&bar_o_full));
+      }
+      __syncwarp();
+    }
+  } else {
+    // ------------------------------------------------------------ softmax, output
+    const int g = (warp - kLoaders) >> 2, quarter = warp & 3;
+    const int r = 128 * g + 32 * quarter + lane;
+    const uint32_t t_lane = tmem_base + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t t_s = t_lane + (uint32_t)(128 * g), t_o = t_lane + (uint32_t)(256 + 128 * g);
+    if (g == 0 || two) {
+      const float ra = row_a[r];
+      const uint64_t ra2 = pack2(ra, ra);
+      const int pos = length - p.count + (row0 + r) / p.group;
+      float m_ref = -INFINITY;                                 // the row's reference, in units of log2
+      uint64_t l2 = 0ull;                                      // sums of even and odd columns
+      bool ok = true, poisoned = false;
+      for (int i = 0; i < tiles; ++i) {
+        const int t0 = range.tile(t_begin + i) * kKeys, slot = i % kBitSlots;
+        ok = mbar_wait(smem_u32(&bar_bits[slot]), (uint32_t)(i / kBitSlots) & 1u, abort_flag) &&
+             mbar_wait(smem_u32(&bar_s_full[g]), (uint32_t)i & 1u, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t all = 0xffffffffu, bad_any = 0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          all &= there_sh[slot][c];
+          bad_any |= bad_sh[slot][c];
+        }
+        bool whole = all == 0xffffffffu && bad_any == 0;
+        if (p.causal) whole &= t0 + kKeys <= pos_lo + 1;
+        if (p.window > 0) whole &= t0 > pos_hi - p.window || t0 + kKeys <= p.sinks;
+        uint32_t vis[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+        if (!whole) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int tb = t0 + 32 * c;
+            vis[c] = there_sh[slot][c];
+            if (p.causal) vis[c] &= low_bits(pos - tb + 1);
+            if (p.window > 0) vis[c] &= ~low_bits(pos - p.window + 1 - tb) | low_bits(p.sinks - tb);
+            poisoned |= (vis[c] & bad_sh[slot][c]) != 0;
+          }
+        }
+        // ---- maximum
+        float top = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          int v[32];
+          tc_ld32(t_s + 32 * c, v);
+          tc_wait_ld();
+          if (whole) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) top = fmaxf(top, __int_as_float(v[j]));
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (vis[c] >> j & 1u) top = fmaxf(top, __int_as_float(v[j]));
+          }
+        }
+        const float m_new = top == -INFINITY ? -INFINITY : top * ra;
+        const bool grow = m_new > m_ref + kGrowth || (m_ref == -INFINITY && m_new > -INFINITY);
+        if (__any_sync(0xffffffffu, grow)) {
+          const float alpha = grow ? exp2_fast(m_ref - m_new) : 1.0f;       // 0 while nothing was seen
+          if (grow) m_ref = m_new;
+          l2 = mul2(l2, pack2(alpha, alpha));
+          if (i > 0) {
+            // the products before this tile's scores are complete: O may be rewritten
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+              int v[32];
+              tc_ld32(t_o + c, v);
+              tc_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = __float_as_int(__int_as_float(v[j]) * alpha);
+              tc_st32(t_o + c, v);
+            }
+          }
+        }
+        // ---- weights, in place of the scores: two fp16 a column
+        const float ref = m_ref == -INFINITY ? 0.0f : kRoom - m_ref;
+        const uint64_t ref2 = pack2(ref, ref);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          int v[32];
+          tc_ld32(t_s + 32 * c, v);
+          tc_wait_ld();
+          uint32_t w[16];
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            const float2 a = unpack2(fma2(pack2(__int_as_float(v[j]), __int_as_float(v[j + 1])), ra2, ref2));
+            float2 e = make_float2(exp2_fast(a.x), exp2_fast(a.y));
+            if (!whole) {
+              if (!(vis[c] >> j & 1u)) e.x = 0.0f;
+              if (!(vis[c] >> (j + 1) & 1u)) e.y = 0.0f;
+            }
+            l2 = add2(l2, pack2(e.x, e.y));
+            w[j / 2] = half_pair(e.x, e.y);
+          }
+          tc_st16(t_s + 16 * c, w);
+        }
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bar_p_ready[g]));
+      }
+      const float2 lp = unpack2(l2);
+      float l = lp.x + lp.y;
+      if (poisoned) l = __int_as_float(0x7fc00000);
+      if (ok && tiles > 0) ok = mbar_wait(smem_u32(&bar_o_full), 0, abort_flag);
+      if (ok) {
+        tc_fence_after();
+        const int rr = row0 + r;
+        const bool real = r < rows_here;
+        const int64_t out_row = ((int64_t)b * p.count + rr / p.group) * p.heads + head * p.group + rr % p.group;
+        const int64_t at = split * p.rows + out_row;
+        const float inv = p.splits > 1 ? 1.0f : (l != 0.0f ? 1.0f / l : 0.0f);   // a row that sees nothing is 0
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          int v[32];
+          if (tiles > 0) {
+            tc_ld32(t_o + c, v);
+            tc_wait_ld();
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = 0;
+          }
+          if (real) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              float o[8];
+#pragma unroll
+              for (int n = 0; n < 8; ++n) {
+                // a row that sees nothing has no weights, whatever its products are
+                const float x = __int_as_float(v[8 * w + (((n & 3) << 1) | (n >> 2))]) * inv;
+                o[n] = m_ref == -INFINITY && l == 0.0f ? 0.0f : x;
+              }
+              if (p.splits > 1) store_f32<float, 8>(p.part + at * D + c + 8 * w, o);
+              else store_f32<T, 8>(static_cast<T*>(p.out) + out_row * D + c + 8 * w, o);
+            }
+          }
+        }
+        if (p.splits > 1 && real) {
+          float* lm = p.part + (int64_t)p.splits * p.rows * D;
+          lm[at] = l;
+          lm[(int64_t)p.splits * p.rows + at] = m_ref == -INFINITY ? -INFINITY : m_ref - kRoom;
+        }
+      }
+    }
+    __syncwarp();
+  }
+
+  // ---------------------------------------------------------------- teardown
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+  }
+}
+
+template <typename T, int D>
+int launch(const Kv4Attention& p, cudaStream_t s) {
+  constexpr int smem = 2 * 128 * D * 2 + 4 * kKeys * D * 2;
+  static SmemLimit limit;
+  MODIFF_CUDA(raise_smem_limit(kv4_attention_tc_kernel<T, D>, smem, limit));
+  const int64_t blocks = (int64_t)p.batch * p.c.heads * p.row_tiles * p.splits;
+  kv4_attention_tc_kernel<T, D><<<(unsigned)blocks, kThreads, smem, s>>>(p);
+  MODIFF_LAUNCH_CHECK("kv4_attention_tc_kernel");
+  return MODIFF_OK;
+}
+
+}  // namespace
+
+bool kv4_tc_wanted(int rows, int dim, int dtype) { return dtype != MODIFF_FP32 && dim <= 128 && rows >= 64; }
+int kv4_tc_rows() { return kRows; }
+
+int kv4_launch_tc(const Kv4Attention& p, int dtype, cudaStream_t s) {
+  if (dtype == MODIFF_FP16) return p.c.dim == 64 ? launch<__half, 64>(p, s) : launch<__half, 128>(p, s);
+  return p.c.dim == 64 ? launch<__nv_bfloat16, 64>(p, s) : launch<__nv_bfloat16, 128>(p, s);
+}
+
+}  // namespace modiff

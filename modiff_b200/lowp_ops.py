@@ -18,21 +18,25 @@ FP8_BLOCK = 128
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
+_Tensor, _grad_enabled = torch.Tensor, torch.is_grad_enabled
 _stream = torch._C._cuda_getCurrentRawStream       # what torch.cuda.current_stream(device).cuda_stream wraps
 
 
 def _device(name, *tensors):
     """The device that all `tensors` (None allowed) are on; CUDA tensors, none of which needs gradients."""
-    device, grad = -1, torch.is_grad_enabled()
+    device, grad = -2, _grad_enabled()
     for t in tensors:
         if t is None:
             continue
-        if not isinstance(t, torch.Tensor) or t.get_device() < 0:
+        if not isinstance(t, _Tensor):
             raise ModiffError(f"{name}: every tensor must be a CUDA tensor (there is no CPU fallback)")
-        if device < 0:
-            device = t.get_device()
-        elif t.get_device() != device:
-            raise ModiffError(f"{name}: tensors on cuda:{device} and {t.device}")
+        d = t.get_device()
+        if d != device:
+            if d < 0:
+                raise ModiffError(f"{name}: every tensor must be a CUDA tensor (there is no CPU fallback)")
+            if device >= 0:
+                raise ModiffError(f"{name}: tensors on cuda:{device} and cuda:{d}")
+            device = d
         if grad and t.requires_grad:
             raise ModiffError(f"{name} has no backward pass: call it under torch.no_grad() or detach its inputs")
     return device
@@ -48,11 +52,11 @@ def _dtype(name, x):
 def _call(device, entry, *args, nbytes=0, nops=0, more=0):
     """One entry point on `device`'s current stream, whatever the current device is; `more` kernels
     beyond its first."""
-    if device == torch.cuda.current_device():
-        _lib.call(entry, *args, _stream(device), nbytes=nbytes, nops=nops)
-    else:
+    if device != torch.cuda.current_device():
         with torch.cuda.device(device):
             _lib.call(entry, *args, _stream(device), nbytes=nbytes, nops=nops)
+    else:
+        _lib.call(entry, *args, _stream(device), nbytes=nbytes, nops=nops)
     _lib.LAUNCHES[0] += more
 
 
@@ -122,7 +126,7 @@ def fp8_linear(x, w, w_scale, bias=None):
     ready = isinstance(x, Fp8Rows)
     src = x.codes if ready else x
     device = _device("fp8_linear", src, w, w_scale, bias)
-    if w.dtype != torch.float8_e4m3fn or w.dim() != 2 or w.numel() == 0:
+    if w.dtype is not torch.float8_e4m3fn or w.dim() != 2 or w.numel() == 0:
         raise ModiffError("fp8_linear: weight codes are a float8_e4m3fn matrix [n, k] (fp8_pack_weight)")
     n, k = w.shape
     w_pitch, step = w.stride()
@@ -200,18 +204,21 @@ def _tokens(name, x):
 
 
 def _norm_weight(name, w, d):
+    """Address of a weight, and the tensor that holds it."""
     if w is None:
-        return None
-    if w.dtype != torch.float32 or w.shape != (d,):
+        return None, None
+    if w.dtype is not torch.float32 or w.shape != (d,):
         raise ModiffError(f"{name}: fp32 weights of {d} values, got {tuple(w.shape)} {w.dtype}")
-    return w.contiguous()
+    w = w.contiguous()
+    return w.data_ptr(), w
 
 
-def _norm_out(name, x, out):
-    """Where the result of `x` goes: a new tensor, or `out`, as the caller sees it and as [tokens, heads, d]."""
+def _norm_side(name, x, out):
+    """One of q and k: (input, its copy if one had to be made, result, arguments of the entry point)."""
+    x3 = _tokens(name, x)
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    elif out.shape != x.shape or out.dtype != x.dtype:
+        out = torch.empty_like(x3) if x3 is x else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    elif out.shape != x.shape or out.dtype is not x.dtype:
         raise ModiffError(f"{name}: out {tuple(out.shape)} {out.dtype} for {tuple(x.shape)} {x.dtype}")
     flat = out
     if out.dim() != 3:
@@ -219,9 +226,11 @@ def _norm_out(name, x, out):
             flat = out.view(-1, *out.shape[-2:]) if out.numel() else out.flatten(0, -3)
         except RuntimeError:
             raise ModiffError(f"{name}: out needs leading dimensions that merge, got strides {out.stride()}") from None
-    if flat.stride(2) != 1:
+    x_token, x_head, _ = x3.stride()
+    y_token, y_head, step = flat.stride()
+    if step != 1:
         raise ModiffError(f"{name}: out needs contiguous channels, got strides {out.stride()}")
-    return out, flat
+    return x3, out, (x3.data_ptr(), x_token, x_head, flat.data_ptr(), y_token, y_head, x3.shape[1])
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6, interleaved=False, out=None):
@@ -238,45 +247,39 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6, i
     device = _device(name, q, k, q_weight, k_weight, cos, sin, positions, *(out or ()))
     dt = _dtype(name, q)
     d = q.shape[-1] if q.dim() else 0
-    if k is not None and (k.dtype != q.dtype or k.shape[-1] != d or k.shape[:-2] != q.shape[:-2]):
+    if k is not None and (k.dtype is not q.dtype or k.shape[-1] != d or k.shape[:-2] != q.shape[:-2]):
         raise ModiffError(f"{name}: q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} differ in more "
                           "than their heads")
     if d % 2 or not 2 <= d <= 256:
         raise ModiffError(f"{name}: heads of an even number of channels up to 256, got {d}")
-    q_weight, k_weight = _norm_weight(name, q_weight, d), _norm_weight(name, k_weight, d)
-    if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2 or cos.shape != sin.shape
-            or 2 * cos.shape[1] > d):
+    qw, q_weight = _norm_weight(name, q_weight, d)
+    kw, k_weight = _norm_weight(name, k_weight, d)
+    shape = cos.shape
+    if (cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or len(shape) != 2 or sin.shape != shape
+            or 2 * shape[1] > d):
         raise ModiffError(f"{name}: fp32 tables [rows, at most {d // 2}], got {tuple(cos.shape)} and "
                           f"{tuple(sin.shape)}")
     cos, sin = cos.contiguous(), sin.contiguous()
-    rows, half = cos.shape
-    q3 = _tokens(name, q)
+    rows, half = shape
+    q3, q_out, q_args = _norm_side(name, q, None if out is None else out[0])
     n = q3.shape[0]
+    k3, k_out, k_args = None, None, (None, 0, 0, None, 0, 0, 0)
+    if k is not None:
+        k3, k_out, k_args = _norm_side(name, k, None if out is None else out[1])
     wide, at = 0, None
     if positions is not None:
-        wide = int(positions.dtype == torch.int64)
-        if not (wide or positions.dtype == torch.int32) or positions.numel() != n:
+        wide = int(positions.dtype is torch.int64)
+        if not (wide or positions.dtype is torch.int32) or positions.numel() != n:
             raise ModiffError(f"{name}: {n} positions of int32 or int64, got {tuple(positions.shape)} "
                               f"{positions.dtype}")
         positions = positions.contiguous()
         at = positions.data_ptr()
     elif half and rows < n:
         raise ModiffError(f"{name}: tables of {rows} rows for {n} tokens")
-    q_out, qo = _norm_out(name, q, None if out is None else out[0])
-    heads = q3.shape[1]
-    args = [q3.data_ptr(), q3.stride(0), q3.stride(1), qo.data_ptr(), qo.stride(0), qo.stride(1), heads]
-    k_out = None
-    if k is None:
-        args += [None, 0, 0, None, 0, 0, 0]
-    else:
-        k3 = _tokens(name, k)
-        k_out, ko = _norm_out(name, k, None if out is None else out[1])
-        args += [k3.data_ptr(), k3.stride(0), k3.stride(1), ko.data_ptr(), ko.stride(0), ko.stride(1), k3.shape[1]]
-        heads += k3.shape[1]
     if n:
-        _call(device, 'modiff_qk_norm_rope', *args, _lib.ptr(q_weight), _lib.ptr(k_weight), cos.data_ptr(),
-              sin.data_ptr(), rows, at, wide, n, d, 2 * half, int(bool(interleaved)), float(eps), dt,
-              nbytes=2 * n * heads * d * q.element_size())
+        _call(device, 'modiff_qk_norm_rope', *q_args, *k_args, qw, kw, cos.data_ptr(), sin.data_ptr(), rows, at, wide, n,
+              d, 2 * half, int(bool(interleaved)), eps, dt,
+              nbytes=2 * n * (q_args[6] + k_args[6]) * d * q.element_size())
     return q_out, k_out
 
 
@@ -304,21 +307,22 @@ def kv4_cache(pages, kv_heads, page_size, head_dim, device):
 
 
 def _cache(name, cache, table, lengths):
+    """(the cache as the entry points take it, its heads and channels, table and lengths without gaps)"""
     kc, kp, vc, vp = cache
-    shape = kc.shape
-    if (len(shape) != 4 or kc.dtype != torch.uint8 or vc.dtype != torch.uint8 or vc.shape != shape
-            or kp.dtype != torch.float16 or vp.dtype != torch.float16 or kp.shape != shape[:3] + (2,)
-            or vp.shape != kp.shape
+    shape, par = kc.shape, kp.shape
+    if (len(shape) != 4 or kc.dtype is not torch.uint8 or vc.dtype is not torch.uint8 or vc.shape != shape
+            or kp.dtype is not torch.float16 or vp.dtype is not torch.float16 or par != (*shape[:3], 2) or vp.shape != par
             or not (kc.is_contiguous() and vc.is_contiguous() and kp.is_contiguous() and vp.is_contiguous())):
         raise ModiffError(f"{name}: a cache is contiguous uint8 codes [pages, heads, page_size, d / 2] and fp16 "
                           f"[pages, heads, page_size, 2], got {tuple(kc.shape)} {kc.dtype}, {tuple(kp.shape)} {kp.dtype}")
-    if (table.dim() != 2 or table.dtype != torch.int32 or lengths.dtype != torch.int32
-            or lengths.shape != table.shape[:1] or table.shape[1] == 0):
+    where = table.shape
+    if (len(where) != 2 or table.dtype is not torch.int32 or lengths.dtype is not torch.int32
+            or lengths.shape != where[:1] or where[1] == 0):
         raise ModiffError(f"{name}: int32 table [batch, pages] and lengths [batch], got {tuple(table.shape)} "
                           f"{table.dtype} and {tuple(lengths.shape)} {lengths.dtype}")
     pages, heads, size, half = shape
-    return (_lib.Kv4CacheStruct(kc.data_ptr(), vc.data_ptr(), kp.data_ptr(), vp.data_ptr(), pages, heads, size,
-                                2 * half), table.contiguous(), lengths.contiguous())
+    return (C.byref(_lib.Kv4CacheStruct(kc.data_ptr(), vc.data_ptr(), kp.data_ptr(), vp.data_ptr(), pages, heads, size,
+                                        2 * half)), heads, 2 * half, table.contiguous(), lengths.contiguous())
 
 
 def kv4_append(cache, k, v, table, lengths):
@@ -328,21 +332,25 @@ def kv4_append(cache, k, v, table, lengths):
     numbers outside the cache are skipped.  No two sequences may name the same place."""
     name = "kv4_append"
     device = _device(name, k, v, table, lengths, *cache)
-    c, table, lengths = _cache(name, cache, table, lengths)
+    c, heads, dim, table, lengths = _cache(name, cache, table, lengths)
     dt = _dtype(name, k)
-    b = table.shape[0]
-    if (k.dim() != 4 or k.shape != v.shape or v.dtype != k.dtype or k.shape[0] != b or k.shape[2] != c.heads
-            or k.shape[3] != c.dim):
-        raise ModiffError(f"{name}: k and v [{b}, n, {c.heads}, {c.dim}] of one type, got {tuple(k.shape)} {k.dtype} "
+    b, per = table.shape
+    shape = k.shape
+    if (len(shape) != 4 or v.shape != shape or v.dtype is not k.dtype or shape[0] != b or shape[2] != heads
+            or shape[3] != dim):
+        raise ModiffError(f"{name}: k and v [{b}, n, {heads}, {dim}] of one type, got {tuple(k.shape)} {k.dtype} "
                           f"and {tuple(v.shape)} {v.dtype}")
-    if k.stride(3) != 1:
+    ks, vs = k.stride(), v.stride()
+    if ks[3] != 1:
         k = k.contiguous()
-    if v.stride(3) != 1:
+        ks = k.stride()
+    if vs[3] != 1:
         v = v.contiguous()
-    if k.numel():
-        _call(device, 'modiff_kv4_append', C.byref(c), k.data_ptr(), *k.stride()[:3], v.data_ptr(),
-              *v.stride()[:3], table.data_ptr(), lengths.data_ptr(), b, k.shape[1], table.shape[1], dt,
-              nbytes=2 * k.numel() * k.element_size() + k.numel() // c.dim * 2 * (c.dim // 2 + 4))
+        vs = v.stride()
+    rows = b * shape[1] * heads
+    if rows:
+        _call(device, 'modiff_kv4_append', c, k.data_ptr(), *ks[:3], v.data_ptr(), *vs[:3], table.data_ptr(),
+              lengths.data_ptr(), b, shape[1], per, dt, nbytes=2 * rows * (dim * k.element_size() + dim // 2 + 4))
 
 
 def kv4_read(cache, table, lengths, n, dtype=torch.float32):
@@ -350,16 +358,16 @@ def kv4_read(cache, table, lengths, n, dtype=torch.float32):
     positions below 0 and pages outside the cache."""
     name = "kv4_read"
     device = _device(name, table, lengths, *cache)
-    c, table, lengths = _cache(name, cache, table, lengths)
+    c, heads, dim, table, lengths = _cache(name, cache, table, lengths)
     if dtype not in _DTYPES or n < 0:
         raise ModiffError(f"{name}: n >= 0 tokens as fp32, fp16 or bf16, got {n} and {dtype}")
-    b = table.shape[0]
-    k = torch.empty((b, n, c.heads, c.dim), dtype=dtype, device=table.device)
+    b, per = table.shape
+    k = torch.empty((b, n, heads, dim), dtype=dtype, device=table.device)
     v = torch.empty_like(k)
-    if k.numel():
-        _call(device, 'modiff_kv4_read', C.byref(c), table.data_ptr(), lengths.data_ptr(), b, n, table.shape[1],
-              k.data_ptr(), v.data_ptr(), _DTYPES[dtype],
-              nbytes=2 * k.numel() * k.element_size() + k.numel() // c.dim * 2 * (c.dim // 2 + 4))
+    rows = b * n * heads
+    if rows:
+        _call(device, 'modiff_kv4_read', c, table.data_ptr(), lengths.data_ptr(), b, n, per, k.data_ptr(), v.data_ptr(),
+              _DTYPES[dtype], nbytes=2 * rows * (dim * k.element_size() + dim // 2 + 4))
     return k, v
 
 
@@ -372,25 +380,28 @@ def kv4_attention(q, cache, table, lengths, scale=None, causal=True, window=0, s
     sees all lengths[b] tokens.  A row that sees nothing is 0.  scale defaults to d ** -0.5."""
     name = "kv4_attention"
     device = _device(name, q, table, lengths, *cache)
-    c, table, lengths = _cache(name, cache, table, lengths)
+    c, kv_heads, dim, table, lengths = _cache(name, cache, table, lengths)
     dt = _dtype(name, q)
-    b = table.shape[0]
-    if q.dim() != 4 or q.shape[0] != b or q.shape[3] != c.dim or q.shape[2] == 0 or q.shape[2] % c.heads:
-        raise ModiffError(f"{name}: q [{b}, n, a multiple of {c.heads}, {c.dim}], got {tuple(q.shape)}")
+    b, per = table.shape
+    shape = q.shape
+    if len(shape) != 4 or shape[0] != b or shape[3] != dim or shape[2] == 0 or shape[2] % kv_heads:
+        raise ModiffError(f"{name}: q [{b}, n, a multiple of {kv_heads}, {dim}], got {tuple(shape)}")
     window, sinks = int(window), int(sinks)
     if window < 0 or sinks < 0 or (window and not causal) or (sinks and not window):
         raise ModiffError(f"{name}: window {window} and sinks {sinks}: a window needs causal positions, sinks need "
                           "a window")
-    if q.stride(3) != 1:
-        q = q.contiguous()
-    n, heads = q.shape[1], q.shape[2]
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if out.numel():
+    if q.is_contiguous():
+        out = torch.empty_like(q)
+    else:
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        if q.stride(3) != 1:
+            q = q.contiguous()
+    n, heads = shape[1], shape[2]
+    if b * n:
         window, sinks = min(window, 1 << 30), min(sinks, 1 << 30)
-        size = _lib.lib().modiff_kv4_attention_bytes(C.byref(c), b, n, heads, table.shape[1], window, sinks)
+        size = _lib.lib().modiff_kv4_attention_bytes(c, b, n, heads, per, window, sinks, dt)
         work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-        scale = float(scale) if scale is not None else c.dim ** -0.5
-        _call(device, 'modiff_kv4_attention', q.data_ptr(), *q.stride()[:3], C.byref(c), table.data_ptr(),
-              lengths.data_ptr(), out.data_ptr(), b, n, heads, table.shape[1], scale, int(bool(causal)), window, sinks,
-              dt, _lib.ptr(work), more=int(size > 0))
+        _call(device, 'modiff_kv4_attention', q.data_ptr(), *q.stride()[:3], c, table.data_ptr(), lengths.data_ptr(),
+              out.data_ptr(), b, n, heads, per, dim ** -0.5 if scale is None else scale, 1 if causal else 0, window,
+              sinks, dt, None if work is None else work.data_ptr(), more=int(size > 0))
     return out

@@ -363,7 +363,7 @@ def _attend(cuda, lengths, n, heads, kv_heads, page, d, dtype, seed=0, gain=2.0,
     lens = torch.tensor(lengths, dtype=torch.int32, device=cuda)
     q = (gain * torch.randn(batch, n, heads, d, generator=_gen(seed))).to(dtype)
     got = ops.kv4_attention(q.to(cuda), cache, table, lens, **kw)
-    want, tol = ref.attention(q, cache, table, lens, d ** -0.5, **kw)
+    want, tol = ref.attention(q, cache, table, lens, **{"scale": d ** -0.5, **kw})
     assert got.dtype == dtype
     _close(got, want, tol)
     return q, cache, table, lens, got
@@ -403,13 +403,37 @@ def test_kv4_attention_split_over_tokens(cuda, lengths, n, heads, kv_heads, d, k
 
 
 @gpu
-@pytest.mark.parametrize("n", [1, 20])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lengths,n,heads,kv_heads,page,d,kw", [
+    ([64], 64, 1, 1, 16, 64, {}), ([128], 128, 1, 1, 64, 128, {}), ([129, 700], 129, 2, 2, 48, 128, {}),
+    ([257], 257, 1, 1, 16, 64, dict(causal=False)), ([500, 130, 0, 3], 130, 6, 2, 32, 128, {}),
+    ([400], 65, 8, 1, 128, 128, dict(window=30, sinks=2)), ([900], 300, 2, 1, 64, 64, dict(window=200, sinks=140)),
+    ([6000], 33, 4, 1, 64, 128, {}), ([4100], 16, 8, 1, 64, 64, dict(window=3000, sinks=5))])
+def test_kv4_attention_of_many_rows(cuda, lengths, n, heads, kv_heads, page, d, kw, dtype):
+    q, cache, table, lens, got = _attend(cuda, lengths, n, heads, kv_heads, page, d, dtype, seed=n, **kw)
+    for _ in range(2):
+        assert torch.equal(ops.kv4_attention(q.to(cuda), cache, table, lens, **kw), got)
+    assert _lib.device_status() == 0
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("scale", [0.0, -0.1, 3.0])
+def test_kv4_attention_scale(cuda, scale, dtype):
+    for n in (1, 70):
+        _attend(cuda, [150, 71], n, 2, 2, 16, 64, dtype, seed=5, gain=0.7, scale=scale)
+
+
+@gpu
+@pytest.mark.parametrize("n", [1, 20, 40])
 def test_kv4_attention_never_meets_hidden_tokens(cuda, n):
     """Infinities and NaN behind the last token, outside the window and in pages that are not there."""
     lengths, page, d = [100, 37], 16, 64
     cache, table = _filled(cuda, 2, 8, 2, page, d, 3)
     lens = torch.tensor(lengths, dtype=torch.int32, device=cuda)
     q = torch.randn(2, n, 4, d, generator=_gen(7)).to(cuda)
+    if n == 40:
+        q = q.half()                                       # rows enough for the kernel of many rows
     kw = dict(window=n + 30, sinks=2)
     clean = ops.kv4_attention(q, cache, table, lens, **kw)
     for b, length in enumerate(lengths):
@@ -420,6 +444,11 @@ def test_kv4_attention_never_meets_hidden_tokens(cuda, n):
     table[0, 100 // page + 1:] = -1                        # never read
     table[1, 37 // page + 1:] = 2 ** 31 - 1
     assert torch.equal(ops.kv4_attention(q, cache, table, lens, **kw), clean)
+    if n == 40:                                            # a value that only the later queries may meet
+        cache.v_params[int(table[0, 80 // page]), :, 80 % page, 1] = math.nan
+        got = ops.kv4_attention(q, cache, table, lens, **kw)
+        assert bool(torch.isnan(got[0, 20:]).all()) and torch.equal(got[0, :20], clean[0, :20])
+        assert torch.equal(got[1], clean[1])
     # a page that is missing in the middle: its tokens are not seen
     table[0, 5] = 18
     got = ops.kv4_attention(q, cache, table, lens)
