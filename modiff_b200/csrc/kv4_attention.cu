@@ -3,9 +3,9 @@
 //   p_t = exp(scale * q . (s_k[t] code_k[t] + m_k[t])) over the tokens that the query sees.
 //
 // The codes go into the tensor cores as they are.  A nibble n in the low bits of an fp16 word is the
-// subnormal number n 2^-24, in bits 4 - 7 it is 16 n 2^-24, both exact, so one AND (and a shift for the
-// upper byte) makes a pair of MMA operands out of eight packed codes' word; the factors 2^24 and 16 are
-// taken out of q and of the results.  Scale and minimum of a token leave the products:
+// subnormal number n 2^-24, in bits 4 - 7 it is 16 n 2^-24, both exact, so that masks alone make MMA
+// operands out of eight packed codes' word (fp32 tensors: see codes_lower); the factors are taken out of
+// q and of the results.  Scale and minimum of a token leave the products:
 //   q . k_t = s_k (q . code) + m_k sum(q)            sum_t p_t v_t = sum_t (p_t s_v) code + sum_t p_t m_v
 // Queries are brought to fp16 by a power of two per row (exact for 16-bit types; fp32 queries and
 // weights travel as two fp16 planes, hi + lo, 22 bits).  p_t s_v is held in fp16 relative to the running
@@ -51,18 +51,36 @@ __device__ inline uint32_t transpose8(uint32_t v) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-// Two channels of four codes out of a word: `even` the low halves of two bytes 16 bits apart, as n 2^-24,
-// `odd` the high halves, as 16 n 2^-24.  The even ones of the upper bytes come from a subtraction (exact),
-// because logic instructions, of half the rate of additions, are what this kernel has most of.
+// Two channels of four codes out of a word: `even` the low halves of two bytes 16 bits apart, as n unit,
+// `odd` the high halves, as 16 n unit.  For 16-bit types unit is 2^-24 and the masked bits are the subnormal
+// numbers; the even ones of the upper bytes come from a subtraction (exact), because logic instructions,
+// of half the rate of additions, are what this kernel has most of.  The tensor cores align the products
+// of subnormal numbers as if they had a leading bit, which leaves sums of them some 17 bits: fp32 takes
+// unit 1 (0x6400 | x is the number 1024 + x), and n - 8 for n, so that sums over tokens or channels do not
+// meet a large common part that the minima take out again (the accumulation truncates).
+__device__ inline uint32_t half_minus(uint32_t v, float c) {
+  const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&v), __float2half2_rn(c));
+  return *reinterpret_cast<const uint32_t*>(&d);
+}
+template <bool SUBNORMAL>
 __device__ inline void codes_lower(uint32_t w, uint32_t& even, uint32_t& odd) {
   even = w & 0x000f000fu;
   odd = w & 0x00f000f0u;
+  if (!SUBNORMAL) {
+    even = half_minus(even | 0x64006400u, 1024.0f + 8.0f);
+    odd = half_minus(odd | 0x64006400u, 1024.0f + 16.0f * 8.0f);
+  }
 }
+template <bool SUBNORMAL>
 __device__ inline void codes_upper(uint32_t w, uint32_t& even, uint32_t& odd) {
   const uint32_t t = __byte_perm(w, 0, 0x4341);
-  odd = t & 0x00f000f0u;
-  const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&t), *reinterpret_cast<const __half2*>(&odd));
-  even = *reinterpret_cast<const uint32_t*>(&d);
+  if (SUBNORMAL) {
+    odd = t & 0x00f000f0u;
+    const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&t), *reinterpret_cast<const __half2*>(&odd));
+    even = *reinterpret_cast<const uint32_t*>(&d);
+  } else {
+    codes_lower<false>(t, even, odd);
+  }
 }
 
 template <typename T, int D, int NT>
@@ -79,6 +97,7 @@ template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kThreads, NT > 1 || D > 128 ? 2 : kBlocksPerSm)
 kv4_attention_kernel(const Kv4Attention p) {
   constexpr int P = sizeof(T) == 4 ? 2 : 1;       // fp16 planes of q and of the weights
+  constexpr float kUnit = P == 1 ? 0x1p-24f : 1.0f;  // what a code of 1 is to the tensor cores
   constexpr int R = 8 * NT;
   constexpr int KW = D / 32;                      // words of a key row that a thread holds
   constexpr int VW = D / 64;                      // words of a value row that a thread holds
@@ -125,9 +144,9 @@ kv4_attention_kernel(const Kv4Attention p) {
     if (top > 0.0f && top < INFINITY) { frexpf(top, &e2); e2 = 15 - e2; }
     const float f1 = ldexpf(1.0f, e2 / 2), f2 = ldexpf(1.0f, e2 - e2 / 2);
     if (lane == 0) {
-      // score = a (s_k (q' . code') + m_k b) with q' the scaled query and code' = code 2^-24
-      row_a[r] = ((p.scale2 * 16777216.0f) / f1) / f2;
-      row_b[r] = sum * f1 * f2 * 0x1p-24f;
+      // score = a (s_k (q' . code') + m_k b) with q' the scaled query and code' = code * unit
+      row_a[r] = ((p.scale2 / kUnit) / f1) / f2;
+      row_b[r] = sum * f1 * f2 * kUnit;
     }
 #pragma unroll
     for (int e = 0; e < D / 32; ++e) {
@@ -261,11 +280,11 @@ kv4_attention_kernel(const Kv4Attention p) {
         for (int u = 0; u < kSub; ++u) {
           uint32_t e0, o0, e1, o1;
           if (h) {
-            codes_upper(kw[u][0][w], e0, o0);
-            codes_upper(kw[u][1][w], e1, o1);
+            codes_upper<P == 1>(kw[u][0][w], e0, o0);
+            codes_upper<P == 1>(kw[u][1][w], e1, o1);
           } else {
-            codes_lower(kw[u][0][w], e0, o0);
-            codes_lower(kw[u][1][w], e1, o1);
+            codes_lower<P == 1>(kw[u][0][w], e0, o0);
+            codes_lower<P == 1>(kw[u][1][w], e1, o1);
           }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
@@ -281,6 +300,10 @@ kv4_attention_kernel(const Kv4Attention p) {
       for (int e = 0; e < 2; ++e) {
         kf[u][e] = half_values(kp[u][e]);
         vf[u][e] = half_values(vp[u][e]);
+        if (P == 2) {                             // the minimum that belongs to n - 8
+          kf[u][e].y = fmaf(8.0f, kf[u][e].x, kf[u][e].y);
+          vf[u][e].y = fmaf(8.0f, vf[u][e].x, vf[u][e].y);
+        }
         if (!whole && (base[u] < 0 || t0 + 16 * u + g + 8 * e >= length))   // not there: whatever was read
           kf[u][e] = vf[u][e] = make_float2(0.0f, 0.0f);
       }
@@ -401,11 +424,11 @@ kv4_attention_kernel(const Kv4Attention p) {
           for (int h2 = 0; h2 < 2; ++h2) {
             uint32_t e0, o0, e1, o1;
             if (h2) {
-              codes_upper(z0, e0, o0);
-              codes_upper(z1, e1, o1);
+              codes_upper<P == 1>(z0, e0, o0);
+              codes_upper<P == 1>(z1, e1, o1);
             } else {
-              codes_lower(z0, e0, o0);
-              codes_lower(z1, e1, o1);
+              codes_lower<P == 1>(z0, e0, o0);
+              codes_lower<P == 1>(z1, e1, o1);
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -445,8 +468,8 @@ kv4_attention_kernel(const Kv4Attention p) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         float* dst = o_sh + (size_t)(warp * R + 8 * nt + 2 * j + c) * (D + 4) + g * (D / 8) + 2 * i;
-        dst[0] = o[i][nt][c] * 1024.0f;                       // 2^24 / 2^14
-        dst[1] = o[i][nt][2 + c] * 64.0f;                     // codes of odd channels stood for 16 n
+        dst[0] = o[i][nt][c] * (0x1p-14f / kUnit);
+        dst[1] = o[i][nt][2 + c] * (0x1p-18f / kUnit);        // codes of odd channels stood for 16 n
       }
   __syncthreads();
   for (int idx = threadIdx.x; idx < rows_here * (D / 4); idx += kThreads) {
