@@ -3,7 +3,7 @@
 //
 // A block owns 256 query rows (query, head of the group) of one sequence and key head, as two groups of
 // 128, and walks the keys in tiles of 128 that both groups share:
-//   four loader warps read the codes through the page table and write keys and values as fp16 numbers
+//   four warps each read the codes of keys and of values through the page table and write fp16 numbers
 //   s code + m, rounded once, as operands of an MMA (128-byte swizzle; a key's channels stay in its row,
 //   which is K-major for the scores and N-major for the output; eight channels of a word lie in the
 //   order 0 4 1 5 2 6 3 7, in which they come out of it, and so do the queries');
@@ -30,9 +30,12 @@ namespace {
 
 constexpr int kKeys = 128;                  // keys of a tile
 constexpr int kRows = 256;                  // query rows of a block
-constexpr int kLoaders = 4;                 // warps 0 .. 3; softmax warps 4 .. 11; MMA warp 12
-constexpr int kMmaWarp = 12;
-constexpr int kThreads = 32 * (kMmaWarp + 1);
+constexpr int kLoaders = 4;                 // warps 0 .. 3 keys, 4 .. 7 values; softmax 8 .. 15; MMAs 16
+constexpr int kSoftmaxWarp = 8, kMmaWarp = 16;
+constexpr int kThreads = 32 * 20;           // the last three warps only complete the MMA warp's group
+// Registers: 96 a thread at launch, dealt out anew by group of four warps.
+constexpr int kRegsAtLaunch = 96, kRegsLoad = 72, kRegsSoftmax = 136, kRegsMma = 56;
+static_assert(5 * kRegsAtLaunch >= 2 * kRegsLoad + 2 * kRegsSoftmax + kRegsMma, "register split");
 constexpr int kChunk = kKeys * 128;         // bytes of 128 rows of 64 channels
 constexpr float kGrowth = 8.0f;             // of a row's maximum, in powers of two, before O is rescaled
 constexpr float kRoom = 6.0f;               // weights are at most 2^(kGrowth + kRoom)
@@ -101,11 +104,16 @@ __device__ inline void store_row(uint8_t* tile, int row, const uint32_t (&w)[D /
   const float2 f = half_values(params);
   const bool edge = fabsf(f.y) > 65000.0f || fabsf(fmaf(15.0f, f.x, f.y)) > 65000.0f;
   uint8_t* base = tile + row * 128;
+  auto place = [&](int i) { return reinterpret_cast<uint4*>(base + (i >> 3) * kChunk + (((i & 7) ^ (row & 7)) << 4)); };
+  if (!there) {
 #pragma unroll
-  for (int i = 0; i < D / 8; ++i) {
-    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (there) v = edge ? dequantise<true>(w[i], s, m) : dequantise<false>(w[i], s, m);
-    *reinterpret_cast<uint4*>(base + (i >> 3) * kChunk + (((i & 7) ^ (row & 7)) << 4)) = v;
+    for (int i = 0; i < D / 8; ++i) *place(i) = make_uint4(0u, 0u, 0u, 0u);
+  } else if (edge) {
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) *place(i) = dequantise<true>(w[i], s, m);
+  } else {
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) *place(i) = dequantise<false>(w[i], s, m);
   }
 }
 
@@ -170,7 +178,7 @@ kv4_attention_tc_kernel(const Kv4Attention p) {
   }
   // ---- queries, one warp a row
   const float sign = p.scale2 < 0.0f ? -1.0f : 1.0f;           // the scale's sign goes into the queries
-  for (int r = warp; r < (two ? kRows : 128); r += kMmaWarp + 1) {
+  for (int r = warp; r < (two ? kRows : 128); r += kThreads / 32) {
     const int rr = row0 + r;
     const bool real = r < rows_here;
     const T* src = static_cast<const T*>(p.q) + (int64_t)b * p.qb + (int64_t)(rr / p.group) * p.qt +
@@ -202,118 +210,112 @@ kv4_attention_tc_kernel(const Kv4Attention p) {
   tc_fence_after();
   const uint32_t tmem_base = tmem_base_sh;
 
-  if (warp < kLoaders) {
-    // ------------------------------------------------------------ keys and values
-    const int key = threadIdx.x;
-    uint32_t kw[D / 8], vw[D / 8], kp = 0, vp = 0;
-    int64_t place = -1, next = -1;
-    auto find = [&](int i) -> int64_t {
+  if (warp < kSoftmaxWarp) {
+    // ------------------------------------------------------------ keys (warps 0 .. 3), values (4 .. 7)
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    const bool value = warp >= kLoaders;
+    const int key = threadIdx.x & 127;
+    const uint8_t* codes = value ? p.c.v_codes : p.c.k_codes;
+    const uint32_t* params = reinterpret_cast<const uint32_t*>(value ? p.c.v_params : p.c.k_params);
+    uint8_t* stages = value ? v_sh : k_sh;
+    const uint32_t empty0 = smem_u32(value ? &bar_v_empty[0] : &bar_k_empty[0]);
+    const uint32_t full0 = smem_u32(value ? &bar_v_full[0] : &bar_k_full[0]);
+    uint32_t w[D / 8], sm = 0;
+    int64_t place = -1;
+    auto load = [&](int i) {
       const int t = range.tile(t_begin + i) * kKeys + key;
-      return t < length ? kv4_place(p.c, table, p.max_pages, t, head) : -1;
+      place = t < length ? kv4_place(p.c, table, p.max_pages, t, head) : -1;
+      const int64_t a = place < 0 ? 0 : place;                 // what is not there is read from the beginning
+      load_words<D / 2>(codes + a * (D / 2), w);
+      sm = __ldg(params + a);
     };
-    auto load_keys = [&](int64_t at) {
-      const int64_t a = at < 0 ? 0 : at;                       // what is not there is read from the beginning
-      load_words<D / 2>(p.c.k_codes + a * (D / 2), kw);
-      kp = __ldg(reinterpret_cast<const uint32_t*>(p.c.k_params) + a);
-    };
-    auto load_values = [&](int64_t at) {
-      const int64_t a = at < 0 ? 0 : at;
-      load_words<D / 2>(p.c.v_codes + a * (D / 2), vw);
-      vp = __ldg(reinterpret_cast<const uint32_t*>(p.c.v_params) + a);
-    };
-    if (tiles > 0) {
-      place = find(0);
-      load_keys(place);
-      load_values(place);
-    }
+    if (tiles > 0) load(0);
     for (int i = 0; i < tiles; ++i) {
-      const int st = i & 1;
-      const uint32_t phase = (uint32_t)(i >> 1) & 1u;
-      if (i + 1 < tiles) next = find(i + 1);
-      if (!mbar_wait(smem_u32(&bar_k_empty[st]), phase ^ 1u, abort_flag)) break;
-      store_row<D>(k_sh + st * kKvTile, key, kw, kp, place >= 0);
-      // exponent field of all ones: infinity or NaN
-      const bool bad = place >= 0 && ((vp & 0x7c00u) == 0x7c00u || (vp & 0x7c000000u) == 0x7c000000u);
-      const uint32_t there_bits = __ballot_sync(0xffffffffu, place >= 0), bad_bits = __ballot_sync(0xffffffffu, bad);
-      if (lane == 0) {
-        there_sh[i % kBitSlots][warp] = there_bits;
-        bad_sh[i % kBitSlots][warp] = bad_bits;
+      const int st = i & 1, slot = i % kBitSlots;
+      if (!mbar_wait(empty0 + 8 * st, ((uint32_t)(i >> 1) & 1u) ^ 1u, abort_flag)) break;
+      bool there = place >= 0;
+      if (value) {
+        // exponent field of all ones: infinity or NaN
+        const bool bad = there && ((sm & 0x7c00u) == 0x7c00u || (sm & 0x7c000000u) == 0x7c000000u);
+        const uint32_t there_bits = __ballot_sync(0xffffffffu, there), bad_bits = __ballot_sync(0xffffffffu, bad);
+        if (lane == 0) {
+          there_sh[slot][warp - kLoaders] = there_bits;
+          bad_sh[slot][warp - kLoaders] = bad_bits;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bar_bits[slot]));
+        there = there && !bad;
       }
+      store_row<D>(stages + st * kKvTile, key, w, sm, there);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(smem_u32(&bar_bits[i % kBitSlots]));
-        mbar_arrive(smem_u32(&bar_k_full[st]));
-      }
-      if (i + 1 < tiles) load_keys(next);
-      if (!mbar_wait(smem_u32(&bar_v_empty[st]), phase ^ 1u, abort_flag)) break;
-      store_row<D>(v_sh + st * kKvTile, key, vw, vp, place >= 0 && !bad);
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&bar_v_full[st]));
-      if (i + 1 < tiles) load_values(next);
-      place = next;
+      if (lane == 0) mbar_arrive(full0 + 8 * st);
+      if (i + 1 < tiles) load(i + 1);
     }
     __syncwarp();
-  } else if (warp == kMmaWarp) {
+  } else if (warp >= kMmaWarp) {
     // ------------------------------------------------------------ MMAs
-    const uint32_t idesc_s = make_idesc_f16(128, kKeys, false), idesc_o = make_idesc_f16(128, D, true);
-    const uint32_t q_addr = smem_u32(q_sh), k_addr = smem_u32(k_sh), v_addr = smem_u32(v_sh);
-    const int groups = two ? 2 : 1;
-    auto scores = [&](int g, int st) {
-      if (elect_one()) {
-#pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-          const uint64_t a = make_smem_desc(q_addr + g * kQTile + c * kChunk);
-          const uint64_t kd = make_smem_desc(k_addr + st * kKvTile + c * kChunk);
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            tc_mma_bf16(tmem_base + (uint32_t)(128 * g), a + (uint64_t)(2 * k), kd + (uint64_t)(2 * k), idesc_s,
-                        c > 0 || k > 0 ? 1u : 0u);
-        }
-        tc_commit(smem_u32(&bar_s_full[g]));
-      }
-      __syncwarp();
-    };
-    bool ok = true;
-    if (tiles > 0) {
-      ok = mbar_wait(smem_u32(&bar_k_full[0]), 0, abort_flag);
-      if (ok) {
-        tc_fence_after();
-        for (int g = 0; g < groups; ++g) scores(g, 0);
-        if (elect_one()) tc_commit(smem_u32(&bar_k_empty[0]));
-        __syncwarp();
-      }
-    }
-    for (int i = 0; i < tiles && ok; ++i) {
-      const int st = i & 1;
-      ok = mbar_wait(smem_u32(&bar_v_full[st]), (uint32_t)(i >> 1) & 1u, abort_flag);
-      if (ok && i + 1 < tiles) ok = mbar_wait(smem_u32(&bar_k_full[st ^ 1]), (uint32_t)((i + 1) >> 1) & 1u, abort_flag);
-      for (int g = 0; g < groups && ok; ++g) {
-        ok = mbar_wait(smem_u32(&bar_p_ready[g]), (uint32_t)i & 1u, abort_flag);
-        if (!ok) break;
-        tc_fence_after();
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == kMmaWarp) {
+      const uint32_t idesc_s = make_idesc_f16(128, kKeys, false), idesc_o = make_idesc_f16(128, D, true);
+      const uint32_t q_addr = smem_u32(q_sh), k_addr = smem_u32(k_sh), v_addr = smem_u32(v_sh);
+      const int groups = two ? 2 : 1;
+      auto scores = [&](int g, int st) {
         if (elect_one()) {
-          const uint64_t vd = make_n_major_desc(v_addr + st * kKvTile);
 #pragma unroll
-          for (int k = 0; k < kKeys / 16; ++k)
-            tc_mma_f16_ta(tmem_base + (uint32_t)(256 + 128 * g), tmem_base + (uint32_t)(128 * g + 8 * k),
-                          vd + (uint64_t)(k * (16 * 128 >> 4)), idesc_o, i > 0 || k > 0 ? 1u : 0u);
+          for (int c = 0; c < D / 64; ++c) {
+            const uint64_t a = make_smem_desc(q_addr + g * kQTile + c * kChunk);
+            const uint64_t kd = make_smem_desc(k_addr + st * kKvTile + c * kChunk);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              tc_mma_bf16(tmem_base + (uint32_t)(128 * g), a + (uint64_t)(2 * k), kd + (uint64_t)(2 * k), idesc_s,
+                          c > 0 || k > 0 ? 1u : 0u);
+          }
+          tc_commit(smem_u32(&bar_s_full[g]));
         }
         __syncwarp();
-        if (i + 1 < tiles) scores(g, st ^ 1);
+      };
+      bool ok = true;
+      if (tiles > 0) {
+        ok = mbar_wait(smem_u32(&bar_k_full[0]), 0, abort_flag);
+        if (ok) {
+          tc_fence_after();
+          for (int g = 0; g < groups; ++g) scores(g, 0);
+          if (elect_one()) tc_commit(smem_u32(&bar_k_empty[0]));
+          __syncwarp();
+        }
       }
-      if (!ok) break;
-      if (elect_one()) {
-        tc_commit(smem_u32(&bar_v_empty[st]));
-        if (i + 1 < tiles) tc_commit(smem_u32(&bar_k_empty[st ^ 1]));
-        if (i == tiles - 1) tc_commit(smem_u32(&bar_o_full));
+      for (int i = 0; i < tiles && ok; ++i) {
+        const int st = i & 1;
+        ok = mbar_wait(smem_u32(&bar_v_full[st]), (uint32_t)(i >> 1) & 1u, abort_flag);
+        if (ok && i + 1 < tiles) ok = mbar_wait(smem_u32(&bar_k_full[st ^ 1]), (uint32_t)((i + 1) >> 1) & 1u, abort_flag);
+        for (int g = 0; g < groups && ok; ++g) {
+          ok = mbar_wait(smem_u32(&bar_p_ready[g]), (uint32_t)i & 1u, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint64_t vd = make_n_major_desc(v_addr + st * kKvTile);
+#pragma unroll
+            for (int k = 0; k < kKeys / 16; ++k)
+              tc_mma_f16_ta(tmem_base + (uint32_t)(256 + 128 * g), tmem_base + (uint32_t)(128 * g + 8 * k),
+                            vd + (uint64_t)(k * (16 * 128 >> 4)), idesc_o, i > 0 || k > 0 ? 1u : 0u);
+          }
+          __syncwarp();
+          if (i + 1 < tiles) scores(g, st ^ 1);
+        }
+        if (!ok) break;
+        if (elect_one()) {
+          tc_commit(smem_u32(&bar_v_empty[st]));
+          if (i + 1 < tiles) tc_commit(smem_u32(&bar_k_empty[st ^ 1]));
+          if (i == tiles - 1) tc_commit(smem_u32(&bar_o_full));
+        }
+        __syncwarp();
       }
-      __syncwarp();
     }
   } else {
     // ------------------------------------------------------------ softmax, output
-    const int g = (warp - kLoaders) >> 2, quarter = warp & 3;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
+    const int g = (warp - kSoftmaxWarp) >> 2, quarter = warp & 3;
     const int r = 128 * g + 32 * quarter + lane;
     const uint32_t t_lane = tmem_base + ((uint32_t)(quarter * 32) << 16);
     const uint32_t t_s = t_lane + (uint32_t)(128 * g), t_o = t_lane + (uint32_t)(256 + 128 * g);
@@ -472,6 +474,12 @@ int launch(const Kv4Attention& p, cudaStream_t s) {
   constexpr int smem = 2 * 128 * D * 2 + 4 * kKeys * D * 2;
   static SmemLimit limit;
   MODIFF_CUDA(raise_smem_limit(kv4_attention_tc_kernel<T, D>, smem, limit));
+  // the split waits for registers: they have to be there from the launch on
+  static const int regs = [] {
+    cudaFuncAttributes a;
+    return cudaFuncGetAttributes(&a, kv4_attention_tc_kernel<T, D>) == cudaSuccess ? a.numRegs : 0;
+  }();
+  if (regs != kRegsAtLaunch) return set_error(MODIFF_ERR_UNSUPPORTED, "kernel built with %d registers", regs);
   const int64_t blocks = (int64_t)p.batch * p.c.heads * p.row_tiles * p.splits;
   kv4_attention_tc_kernel<T, D><<<(unsigned)blocks, kThreads, smem, s>>>(p);
   MODIFF_LAUNCH_CHECK("kv4_attention_tc_kernel");
