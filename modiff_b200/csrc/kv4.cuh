@@ -23,6 +23,7 @@ struct Kv4Attention {
   const int32_t* lengths;
   int batch, count, heads, group, max_pages, splits, row_tiles;
   int causal, window, sinks;
+  int q_vec;                              // rows of q start on 16 bytes
   float scale2;                           // scale * log2(e)
   int64_t rows;                           // batch * count * heads
 };

@@ -681,6 +681,7 @@ extern "C" int modiff_kv4_attention(const void* q, int64_t q_seq, int64_t q_toke
   Kv4Attention p;
   p.q = q;
   p.qb = q_seq; p.qt = q_token; p.qh = q_head;
+  p.q_vec = (((uintptr_t)q | (uintptr_t)((q_seq | q_token | q_head) * size)) & 15) == 0;
   p.out = out;
   p.part = static_cast<float*>(workspace);
   p.c = kv4_pages(cache);

@@ -29,6 +29,7 @@ int read_device_status_kv4(int* status, int reset) { return read_status_this_uni
 namespace {
 
 constexpr int kKeys = 128;                  // keys of a tile
+constexpr int kHalf = 64;                   // keys of one softmax step
 constexpr int kRows = 256;                  // query rows of a block
 constexpr int kLoaders = 4;                 // warps 0 .. 3 keys, 4 .. 7 values; softmax 8 .. 15; MMAs 16
 constexpr int kSoftmaxWarp = 8, kMmaWarp = 16;
@@ -117,6 +118,22 @@ __device__ inline void store_row(uint8_t* tile, int row, const uint32_t (&w)[D /
   }
 }
 
+// the largest of three; a NaN is passed over
+__device__ inline float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ inline void tc_ld16(uint32_t taddr, int (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr)
+      : "memory");
+}
+
 // low bits [0, n) of a word, n clamped to 0 .. 32
 __device__ inline uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u); }
 
@@ -126,8 +143,8 @@ kv4_attention_tc_kernel(const Kv4Attention p) {
   constexpr int kQTile = 128 * D * 2, kKvTile = kKeys * D * 2;
   extern __shared__ __align__(1024) uint8_t smem[];          // Q [2], K [2], V [2]
   __shared__ __align__(8) uint64_t bar_k_full[2], bar_k_empty[2], bar_v_full[2], bar_v_empty[2];
-  __shared__ __align__(8) uint64_t bar_s_full[2], bar_p_ready[2], bar_bits[kBitSlots], bar_o_full;
-  __shared__ uint32_t there_sh[kBitSlots][4], bad_sh[kBitSlots][4];   // tokens that exist; values that are not finite
+  __shared__ __align__(8) uint64_t bar_s_full[2][2], bar_p_ready[2][2], bar_pv[2][2], bar_bits[kBitSlots];   // [group][half]
+  __shared__ __align__(16) uint32_t there_sh[kBitSlots][4], bad_sh[kBitSlots][4];   // tokens that exist; values that are not finite
   __shared__ float row_a[kRows];
   __shared__ uint32_t tmem_base_sh;
   __shared__ int abort_sh;
@@ -163,11 +180,13 @@ kv4_attention_tc_kernel(const Kv4Attention p) {
       mbar_init(smem_u32(&bar_k_empty[i]), 1);
       mbar_init(smem_u32(&bar_v_full[i]), kLoaders);
       mbar_init(smem_u32(&bar_v_empty[i]), 1);
-      mbar_init(smem_u32(&bar_s_full[i]), 1);
-      mbar_init(smem_u32(&bar_p_ready[i]), 4);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(smem_u32(&bar_s_full[i][h]), 1);
+        mbar_init(smem_u32(&bar_p_ready[i][h]), 4);
+        mbar_init(smem_u32(&bar_pv[i][h]), 1);
+      }
     }
     for (int i = 0; i < kBitSlots; ++i) mbar_init(smem_u32(&bar_bits[i]), kLoaders);
-    mbar_init(smem_u32(&bar_o_full), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kMmaWarp) {
@@ -178,30 +197,47 @@ kv4_attention_tc_kernel(const Kv4Attention p) {
   }
   // ---- queries, one warp a row
   const float sign = p.scale2 < 0.0f ? -1.0f : 1.0f;           // the scale's sign goes into the queries
-  for (int r = warp; r < (two ? kRows : 128); r += kThreads / 32) {
-    const int rr = row0 + r;
-    const bool real = r < rows_here;
-    const T* src = static_cast<const T*>(p.q) + (int64_t)b * p.qb + (int64_t)(rr / p.group) * p.qt +
-                   (int64_t)(head * p.group + rr % p.group) * p.qh;
-    float x[D / 32];
-    float top = 0.0f;
+  constexpr int kBatch = 4, kWarps = kThreads / 32, kPer = D / 32;   // rows whose loads a warp has in flight
+  for (int r0 = warp; r0 < (two ? kRows : 128); r0 += kBatch * kWarps) {
+    float x[kBatch][kPer];
 #pragma unroll
-    for (int e = 0; e < D / 32; ++e) {
-      x[e] = real ? to_f32<T>(src[lane + 32 * e]) : 0.0f;
-      top = fmaxf(top, fabsf(x[e]));
+    for (int u = 0; u < kBatch; ++u) {
+      const int r = r0 + u * kWarps, rr = row0 + r;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) x[u][e] = 0.0f;
+      if (r < rows_here) {
+        const T* src = static_cast<const T*>(p.q) + (int64_t)b * p.qb + (int64_t)(rr / p.group) * p.qt +
+                       (int64_t)(head * p.group + rr % p.group) * p.qh + kPer * lane;
+        if (p.q_vec) {
+          load_f32<T, kPer>(src, x[u]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) x[u][e] = to_f32<T>(src[e]);
+        }
+      }
     }
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    // power of two that brings the largest element to [2^14, 2^15); in two factors, for bf16's range
-    int e2 = 0;
-    if (top > 0.0f && top < INFINITY) { frexpf(top, &e2); e2 = 15 - e2; }
-    const float f1 = ldexpf(sign, e2 / 2), f2 = ldexpf(1.0f, e2 - e2 / 2);
-    if (lane == 0) row_a[r] = p.scale2 / f1 / f2;
 #pragma unroll
-    for (int e = 0; e < D / 32; ++e) {
-      const int ch = lane + 32 * e, w = (ch & 63) >> 3, n = ch & 7;
-      const int at = ((n & 3) << 1) | (n >> 2);                // 0 4 1 5 2 6 3 7
-      uint8_t* dst = q_sh + (r >> 7) * kQTile + (ch >> 6) * kChunk + (r & 127) * 128 + ((w ^ (r & 7)) << 4) + 2 * at;
-      *reinterpret_cast<__half*>(dst) = __float2half_rn(x[e] * f1 * f2);
+    for (int u = 0; u < kBatch; ++u) {
+      const int r = r0 + u * kWarps;
+      if (r >= (two ? kRows : 128)) break;
+      float top = 0.0f;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) top = fmaxf(top, fabsf(x[u][e]));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      // power of two that brings the largest element to [2^14, 2^15) (a subnormal one less far); in two
+      // factors, for bf16's range
+      int e2 = 0;
+      if (top > 0.0f && top < INFINITY) e2 = 141 - (int)(__float_as_uint(top) >> 23);
+      const float f1 = sign * __int_as_float((127 + e2 / 2) << 23), f2 = __int_as_float((127 + e2 - e2 / 2) << 23);
+      if (lane == 0) row_a[r] = p.scale2 / f1 / f2;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        const int ch = kPer * lane + e, w = (ch & 63) >> 3, n = ch & 7;
+        const int at = ((n & 3) << 1) | (n >> 2);              // 0 4 1 5 2 6 3 7
+        uint8_t* dst = q_sh + (r >> 7) * kQTile + (ch >> 6) * kChunk + (r & 127) * 128 + ((w ^ (r & 7)) << 4) + 2 * at;
+        *reinterpret_cast<__half*>(dst) = __float2half_rn(x[u][e] * f1 * f2);
+      }
     }
   }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -257,21 +293,22 @@ kv4_attention_tc_kernel(const Kv4Attention p) {
     // ------------------------------------------------------------ MMAs
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == kMmaWarp) {
-      const uint32_t idesc_s = make_idesc_f16(128, kKeys, false), idesc_o = make_idesc_f16(128, D, true);
+      const uint32_t idesc_s = make_idesc_f16(128, kHalf, false), idesc_o = make_idesc_f16(128, D, true);
       const uint32_t q_addr = smem_u32(q_sh), k_addr = smem_u32(k_sh), v_addr = smem_u32(v_sh);
       const int groups = two ? 2 : 1;
-      auto scores = [&](int g, int st) {
+      // scores of half h of the keys in stage st, into the group's buffer of that half
+      auto scores = [&](int g, int h, int st) {
         if (elect_one()) {
 #pragma unroll
           for (int c = 0; c < D / 64; ++c) {
             const uint64_t a = make_smem_desc(q_addr + g * kQTile + c * kChunk);
-            const uint64_t kd = make_smem_desc(k_addr + st * kKvTile + c * kChunk);
+            const uint64_t kd = make_smem_desc(k_addr + st * kKvTile + c * kChunk + h * kHalf * 128);
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              tc_mma_bf16(tmem_base + (uint32_t)(128 * g), a + (uint64_t)(2 * k), kd + (uint64_t)(2 * k), idesc_s,
+              tc_mma_bf16(tmem_base + (uint32_t)(128 * g + kHalf * h), a + (uint64_t)(2 * k), kd + (uint64_t)(2 * k), idesc_s,
                           c > 0 || k > 0 ? 1u : 0u);
           }
-          tc_commit(smem_u32(&bar_s_full[g]));
+          tc_commit(smem_u32(&bar_s_full[g][h]));
         }
         __syncwarp();
       };
@@ -280,7 +317,8 @@ kv4_attention_tc_kernel(const Kv4Attention p) {
         ok = mbar_wait(smem_u32(&bar_k_full[0]), 0, abort_flag);
         if (ok) {
           tc_fence_after();
-          for (int g = 0; g < groups; ++g) scores(g, 0);
+          for (int h = 0; h < 2; ++h)
+            for (int g = 0; g < groups; ++g) scores(g, h, 0);
           if (elect_one()) tc_commit(smem_u32(&bar_k_empty[0]));
           __syncwarp();
         }
@@ -289,25 +327,27 @@ kv4_attention_tc_kernel(const Kv4Attention p) {
         const int st = i & 1;
         ok = mbar_wait(smem_u32(&bar_v_full[st]), (uint32_t)(i >> 1) & 1u, abort_flag);
         if (ok && i + 1 < tiles) ok = mbar_wait(smem_u32(&bar_k_full[st ^ 1]), (uint32_t)((i + 1) >> 1) & 1u, abort_flag);
-        for (int g = 0; g < groups && ok; ++g) {
-          ok = mbar_wait(smem_u32(&bar_p_ready[g]), (uint32_t)i & 1u, abort_flag);
+#pragma unroll 1
+        for (int hg = 0; hg < 2 * groups && ok; ++hg) {
+          const int h = two ? hg >> 1 : hg, g = two ? hg & 1 : 0;
+          ok = mbar_wait(smem_u32(&bar_p_ready[g][h]), (uint32_t)i & 1u, abort_flag);
           if (!ok) break;
           tc_fence_after();
           if (elect_one()) {
-            const uint64_t vd = make_n_major_desc(v_addr + st * kKvTile);
+            const uint64_t vd = make_n_major_desc(v_addr + st * kKvTile + h * kHalf * 128);
 #pragma unroll
-            for (int k = 0; k < kKeys / 16; ++k)
-              tc_mma_f16_ta(tmem_base + (uint32_t)(256 + 128 * g), tmem_base + (uint32_t)(128 * g + 8 * k),
-                            vd + (uint64_t)(k * (16 * 128 >> 4)), idesc_o, i > 0 || k > 0 ? 1u : 0u);
+            for (int k = 0; k < kHalf / 16; ++k)
+              tc_mma_f16_ta(tmem_base + (uint32_t)(256 + 128 * g), tmem_base + (uint32_t)(128 * g + kHalf * h + 8 * k),
+                            vd + (uint64_t)(k * (16 * 128 >> 4)), idesc_o, i > 0 || h > 0 || k > 0 ? 1u : 0u);
+            tc_commit(smem_u32(&bar_pv[g][h]));
           }
           __syncwarp();
-          if (i + 1 < tiles) scores(g, st ^ 1);
+          if (i + 1 < tiles) scores(g, h, st ^ 1);
         }
         if (!ok) break;
         if (elect_one()) {
           tc_commit(smem_u32(&bar_v_empty[st]));
           if (i + 1 < tiles) tc_commit(smem_u32(&bar_k_empty[st ^ 1]));
-          if (i == tiles - 1) tc_commit(smem_u32(&bar_o_full));
         }
         __syncwarp();
       }
@@ -326,98 +366,94 @@ kv4_attention_tc_kernel(const Kv4Attention p) {
       float m_ref = -INFINITY;                                 // the row's reference, in units of log2
       uint64_t l2 = 0ull;                                      // sums of even and odd columns
       bool ok = true, poisoned = false;
-      for (int i = 0; i < tiles; ++i) {
-        const int t0 = range.tile(t_begin + i) * kKeys, slot = i % kBitSlots;
-        ok = mbar_wait(smem_u32(&bar_bits[slot]), (uint32_t)(i / kBitSlots) & 1u, abort_flag) &&
-             mbar_wait(smem_u32(&bar_s_full[g]), (uint32_t)i & 1u, abort_flag);
+      for (int step = 0; step < 2 * tiles; ++step) {
+        const int i = step >> 1, h = step & 1, slot = i % kBitSlots;
+        const int t0 = range.tile(t_begin + i) * kKeys + kHalf * h;
+        ok = mbar_wait(smem_u32(&bar_s_full[g][h]), (uint32_t)i & 1u, abort_flag) &&
+             (h == 1 || mbar_wait(smem_u32(&bar_bits[slot]), (uint32_t)(i / kBitSlots) & 1u, abort_flag));
         if (!ok) break;
         tc_fence_after();
-        uint32_t all = 0xffffffffu, bad_any = 0;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          all &= there_sh[slot][c];
-          bad_any |= bad_sh[slot][c];
-        }
-        bool whole = all == 0xffffffffu && bad_any == 0;
-        if (p.causal) whole &= t0 + kKeys <= pos_lo + 1;
-        if (p.window > 0) whole &= t0 > pos_hi - p.window || t0 + kKeys <= p.sinks;
-        uint32_t vis[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+        const uint32_t t_sh = t_s + (uint32_t)(kHalf * h);
+        int v[kHalf];
+        tc_ld32(t_sh, reinterpret_cast<int(&)[32]>(v[0]));
+        tc_ld32(t_sh + 32, reinterpret_cast<int(&)[32]>(v[32]));
+        const uint2 there = *reinterpret_cast<const uint2*>(&there_sh[slot][2 * h]);
+        const uint2 bad = *reinterpret_cast<const uint2*>(&bad_sh[slot][2 * h]);
+        bool whole = (there.x & there.y) == 0xffffffffu && (bad.x | bad.y) == 0;
+        if (p.causal) whole &= t0 + kHalf <= pos_lo + 1;
+        if (p.window > 0) whole &= t0 > pos_hi - p.window || t0 + kHalf <= p.sinks;
+        tc_wait_ld();
         if (!whole) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
+          for (int c = 0; c < 2; ++c) {
             const int tb = t0 + 32 * c;
-            vis[c] = there_sh[slot][c];
-            if (p.causal) vis[c] &= low_bits(pos - tb + 1);
-            if (p.window > 0) vis[c] &= ~low_bits(pos - p.window + 1 - tb) | low_bits(p.sinks - tb);
-            poisoned |= (vis[c] & bad_sh[slot][c]) != 0;
-          }
-        }
-        // ---- maximum
-        float top = -INFINITY;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          int v[32];
-          tc_ld32(t_s + 32 * c, v);
-          tc_wait_ld();
-          if (whole) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) top = fmaxf(top, __int_as_float(v[j]));
-          } else {
+            uint32_t vis = c ? there.y : there.x;
+            if (p.causal) vis &= low_bits(pos - tb + 1);
+            if (p.window > 0) vis &= ~low_bits(pos - p.window + 1 - tb) | low_bits(p.sinks - tb);
+            poisoned |= (vis & (c ? bad.y : bad.x)) != 0;
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-              if (vis[c] >> j & 1u) top = fmaxf(top, __int_as_float(v[j]));
+              if (!(vis >> j & 1u)) v[32 * c + j] = __float_as_int(-INFINITY);
           }
         }
+        float top = max3(__int_as_float(v[0]), __int_as_float(v[1]), -INFINITY);
+        float top2 = max3(__int_as_float(v[2]), __int_as_float(v[3]), -INFINITY);
+#pragma unroll
+        for (int j = 4; j < kHalf; j += 4) {
+          top = max3(__int_as_float(v[j]), __int_as_float(v[j + 1]), top);
+          top2 = max3(__int_as_float(v[j + 2]), __int_as_float(v[j + 3]), top2);
+        }
+        top = fmaxf(top, top2);
         const float m_new = top == -INFINITY ? -INFINITY : top * ra;
         const bool grow = m_new > m_ref + kGrowth || (m_ref == -INFINITY && m_new > -INFINITY);
         if (__any_sync(0xffffffffu, grow)) {
           const float alpha = grow ? exp2_fast(m_ref - m_new) : 1.0f;       // 0 while nothing was seen
           if (grow) m_ref = m_new;
           l2 = mul2(l2, pack2(alpha, alpha));
-          if (i > 0) {
-            // the products before this tile's scores are complete: O may be rewritten
-#pragma unroll
-            for (int c = 0; c < D; c += 32) {
-              int v[32];
-              tc_ld32(t_o + c, v);
+          if (step > 0) {
+            // O may be rewritten once the products of the step before are in it; those of two steps before
+            // are, this step's scores were multiplied behind them
+            ok = mbar_wait(smem_u32(&bar_pv[g][h ^ 1]), (uint32_t)((step - 1) >> 1) & 1u, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
+              int o[16];
+              tc_ld16(t_o + c, o);
               tc_wait_ld();
+              uint32_t w[16];
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = __float_as_int(__int_as_float(v[j]) * alpha);
-              tc_st32(t_o + c, v);
+              for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(__int_as_float(o[j]) * alpha);
+              tc_st16(t_o + c, w);
             }
           }
         }
-        // ---- weights, in place of the scores: two fp16 a column
+        // ---- weights, in place of the scores: two fp16 a column; a hidden key's score of -inf gives 0
         const float ref = m_ref == -INFINITY ? 0.0f : kRoom - m_ref;
         const uint64_t ref2 = pack2(ref, ref);
+        uint32_t w[kHalf / 2];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          int v[32];
-          tc_ld32(t_s + 32 * c, v);
-          tc_wait_ld();
-          uint32_t w[16];
-#pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            const float2 a = unpack2(fma2(pack2(__int_as_float(v[j]), __int_as_float(v[j + 1])), ra2, ref2));
-            float2 e = make_float2(exp2_fast(a.x), exp2_fast(a.y));
-            if (!whole) {
-              if (!(vis[c] >> j & 1u)) e.x = 0.0f;
-              if (!(vis[c] >> (j + 1) & 1u)) e.y = 0.0f;
-            }
-            l2 = add2(l2, pack2(e.x, e.y));
-            w[j / 2] = half_pair(e.x, e.y);
+        for (int j = 0; j < kHalf; j += 2) {
+          float2 a = unpack2(fma2(pack2(__int_as_float(v[j]), __int_as_float(v[j + 1])), ra2, ref2));
+          if (!whole) {                                        // 0 * inf where the scale is 0
+            if (v[j] == __float_as_int(-INFINITY)) a.x = -INFINITY;
+            if (v[j + 1] == __float_as_int(-INFINITY)) a.y = -INFINITY;
           }
-          tc_st16(t_s + 16 * c, w);
+          const float2 e = make_float2(exp2_fast(a.x), exp2_fast(a.y));
+          l2 = add2(l2, pack2(e.x, e.y));
+          w[j / 2] = half_pair(e.x, e.y);
         }
+        tc_st16(t_sh, reinterpret_cast<uint32_t(&)[16]>(w[0]));
+        tc_st16(t_sh + 16, reinterpret_cast<uint32_t(&)[16]>(w[16]));
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&bar_p_ready[g]));
+        if (lane == 0) mbar_arrive(smem_u32(&bar_p_ready[g][h]));
       }
       const float2 lp = unpack2(l2);
       float l = lp.x + lp.y;
       if (poisoned) l = __int_as_float(0x7fc00000);
-      if (ok && tiles > 0) ok = mbar_wait(smem_u32(&bar_o_full), 0, abort_flag);
+      if (ok && tiles > 0) ok = mbar_wait(smem_u32(&bar_pv[g][1]), (uint32_t)(tiles - 1) & 1u, abort_flag);
       if (ok) {
         tc_fence_after();
         const int rr = row0 + r;
