@@ -24,6 +24,7 @@ struct Kv4Attention {
   int batch, count, heads, group, max_pages, splits, row_tiles;
   int causal, window, sinks;
   int q_vec;                              // rows of q start on 16 bytes
+  FastDiv by_group;
   float scale2;                           // scale * log2(e)
   int64_t rows;                           // batch * count * heads
 };

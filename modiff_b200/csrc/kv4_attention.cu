@@ -687,6 +687,7 @@ extern "C" int modiff_kv4_attention(const void* q, int64_t q_seq, int64_t q_toke
   p.c = kv4_pages(cache);
   p.table = table; p.lengths = lengths;
   p.batch = batch; p.count = count; p.heads = heads; p.group = heads / cache->heads;
+  p.by_group = FastDiv(p.group);
   p.max_pages = max_pages;
   p.splits = pl.splits; p.row_tiles = pl.row_tiles;
   // positions and windows are subtracted in 32 bits; none of the cache's tokens is 2^30 back

@@ -195,49 +195,56 @@ kv4_attention_tc_kernel(const Kv4Attention p) {
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  // ---- queries, one warp a row
+  // ---- queries: D / 8 lanes a row, eight channels (a chunk of the operand) each; a warp's loads are all on
+  // their way before the first is looked at
   const float sign = p.scale2 < 0.0f ? -1.0f : 1.0f;           // the scale's sign goes into the queries
-  constexpr int kBatch = 4, kWarps = kThreads / 32, kPer = D / 32;   // rows whose loads a warp has in flight
-  for (int r0 = warp; r0 < (two ? kRows : 128); r0 += kBatch * kWarps) {
-    float x[kBatch][kPer];
+  constexpr int kLanes = D / 8, kPass = kThreads / kLanes, kBatch = (kRows + kPass - 1) / kPass;
+  const int q_row = threadIdx.x / kLanes, chunk = threadIdx.x % kLanes;
+  Pack<T, 8> raw[kBatch];
+  const T* q_lane = static_cast<const T*>(p.q) + (int64_t)b * p.qb + (int64_t)(head * p.group) * p.qh + 8 * chunk;
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const int r = r0 + u * kWarps, rr = row0 + r;
+  for (int u = 0; u < kBatch; ++u) {
+    const int r = q_row + u * kPass;
+    if (r < rows_here) {
+      int member;
+      const int token = p.by_group.divmod(row0 + r, member);
+      const T* src = q_lane + token * p.qt + member * p.qh;
+      if (p.q_vec) {
+        raw[u] = *reinterpret_cast<const Pack<T, 8>*>(src);
+      } else {
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) x[u][e] = 0.0f;
-      if (r < rows_here) {
-        const T* src = static_cast<const T*>(p.q) + (int64_t)b * p.qb + (int64_t)(rr / p.group) * p.qt +
-                       (int64_t)(head * p.group + rr % p.group) * p.qh + kPer * lane;
-        if (p.q_vec) {
-          load_f32<T, kPer>(src, x[u]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < kPer; ++e) x[u][e] = to_f32<T>(src[e]);
-        }
+        for (int e = 0; e < 8; ++e) raw[u].v[e] = src[e];
       }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) raw[u].v[e] = from_f32<T>(0.0f);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kBatch; ++u) {
+    const int r = q_row + u * kPass;
+    float x[8], top = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[e] = to_f32<T>(raw[u].v[e]);
+      top = fmaxf(top, fabsf(x[e]));
     }
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const int r = r0 + u * kWarps;
-      if (r >= (two ? kRows : 128)) break;
-      float top = 0.0f;
+    for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    // power of two that brings the largest element to [2^14, 2^15) (a subnormal one less far); in two
+    // factors, for bf16's range
+    int e2 = 0;
+    if (top > 0.0f && top < INFINITY) e2 = 141 - (int)(__float_as_uint(top) >> 23);
+    const float f1 = sign * __int_as_float((127 + e2 / 2) << 23), f2 = __int_as_float((127 + e2 - e2 / 2) << 23);
+    if (r < kRows) {
+      // divided by both (powers of two, exactly)
+      if (chunk == 0)
+        row_a[r] = fabsf(p.scale2) * __int_as_float((127 - e2 / 2) << 23) * __int_as_float((127 - (e2 - e2 / 2)) << 23);
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) top = fmaxf(top, fabsf(x[u][e]));
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      // power of two that brings the largest element to [2^14, 2^15) (a subnormal one less far); in two
-      // factors, for bf16's range
-      int e2 = 0;
-      if (top > 0.0f && top < INFINITY) e2 = 141 - (int)(__float_as_uint(top) >> 23);
-      const float f1 = sign * __int_as_float((127 + e2 / 2) << 23), f2 = __int_as_float((127 + e2 - e2 / 2) << 23);
-      if (lane == 0) row_a[r] = p.scale2 / f1 / f2;
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) {
-        const int ch = kPer * lane + e, w = (ch & 63) >> 3, n = ch & 7;
-        const int at = ((n & 3) << 1) | (n >> 2);              // 0 4 1 5 2 6 3 7
-        uint8_t* dst = q_sh + (r >> 7) * kQTile + (ch >> 6) * kChunk + (r & 127) * 128 + ((w ^ (r & 7)) << 4) + 2 * at;
-        *reinterpret_cast<__half*>(dst) = __float2half_rn(x[u][e] * f1 * f2);
-      }
+      for (int e = 0; e < 8; ++e) x[e] = x[e] * f1 * f2;
+      *reinterpret_cast<uint4*>(q_sh + (r >> 7) * kQTile + (chunk >> 3) * kChunk + (r & 127) * 128 +
+                                (((chunk & 7) ^ (r & 7)) << 4)) =
+          make_uint4(half_pair(x[0], x[4]), half_pair(x[1], x[5]), half_pair(x[2], x[6]), half_pair(x[3], x[7]));
     }
   }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
