@@ -42,14 +42,26 @@ constexpr float kGrowth = 8.0f;             // of a row's maximum, in powers of 
 constexpr float kRoom = 6.0f;               // weights are at most 2^(kGrowth + kRoom)
 constexpr int kBitSlots = 4;
 
-// fp16 x fp16 -> fp32, A from tensor memory
-__device__ inline void tc_mma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+// fp16 x fp16 -> fp32; descriptors as low words and the high word they share.  A from shared or tensor memory.
+__device__ inline void tc_mma_f16_lo(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc,
                                      uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %3};\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ inline void tc_mma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t hi, uint32_t idesc,
+                                     uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 __device__ inline void tc_st16(uint32_t taddr, const uint32_t (&v)[16]) {
@@ -300,63 +312,72 @@ kv4_attention_tc_kernel(const Kv4Attention p) {
     // ------------------------------------------------------------ MMAs
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == kMmaWarp) {
+      // This warp's instructions are the critical path (about five cycles each beside the other warps): the
+      // descriptors' low words are added to 32-bit constants, waits that come together are one.
       const uint32_t idesc_s = make_idesc_f16(128, kHalf, false), idesc_o = make_idesc_f16(128, D, true);
-      const uint32_t q_addr = smem_u32(q_sh), k_addr = smem_u32(k_sh), v_addr = smem_u32(v_sh);
-      const int groups = two ? 2 : 1;
+      const uint32_t q_lo = (uint32_t)make_smem_desc(smem_u32(q_sh)), desc_hi = (uint32_t)(make_smem_desc(0) >> 32);
+      const uint32_t k_lo = (uint32_t)make_smem_desc(smem_u32(k_sh)), v_lo = (uint32_t)make_n_major_desc(smem_u32(v_sh));
+      // every lane its own barrier and parity, until all have seen theirs
+      auto wait_all = [&](uint32_t bar, uint32_t parity) {
+        return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)) != 0;
+      };
       // scores of half h of the keys in stage st, into the group's buffer of that half
       auto scores = [&](int g, int h, int st) {
+        const uint32_t a = q_lo + (uint32_t)(g * (kQTile >> 4)), kd = k_lo + (uint32_t)(st * (kKvTile >> 4) + h * (kHalf * 128 >> 4));
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            tc_mma_f16_lo(tmem_base + (uint32_t)(128 * g + kHalf * h), a + (uint32_t)(c * (kChunk >> 4) + 2 * k),
+                          kd + (uint32_t)(c * (kChunk >> 4) + 2 * k), desc_hi, idesc_s, c > 0 || k > 0 ? 1u : 0u);
+        tc_commit(smem_u32(&bar_s_full[g][h]));
+      };
+      auto products = [&](int g, int h, int st, uint32_t accumulate) {
+        const uint32_t vd = v_lo + (uint32_t)(st * (kKvTile >> 4) + h * (kHalf * 128 >> 4));
+#pragma unroll
+        for (int k = 0; k < kHalf / 16; ++k)
+          tc_mma_f16_ta(tmem_base + (uint32_t)(256 + 128 * g), tmem_base + (uint32_t)(128 * g + kHalf * h + 8 * k),
+                        vd + (uint32_t)(k * (16 * 128 >> 4)), desc_hi, idesc_o, k > 0 ? 1u : accumulate);
+        tc_commit(smem_u32(&bar_pv[g][h]));
+      };
+      const uint32_t k_full0 = smem_u32(&bar_k_full[0]), v_full0 = smem_u32(&bar_v_full[0]);
+      bool ok = tiles > 0 && wait_all(k_full0, 0);
+      if (ok) {
+        tc_fence_after();
         if (elect_one()) {
-#pragma unroll
-          for (int c = 0; c < D / 64; ++c) {
-            const uint64_t a = make_smem_desc(q_addr + g * kQTile + c * kChunk);
-            const uint64_t kd = make_smem_desc(k_addr + st * kKvTile + c * kChunk + h * kHalf * 128);
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              tc_mma_bf16(tmem_base + (uint32_t)(128 * g + kHalf * h), a + (uint64_t)(2 * k), kd + (uint64_t)(2 * k), idesc_s,
-                          c > 0 || k > 0 ? 1u : 0u);
-          }
-          tc_commit(smem_u32(&bar_s_full[g][h]));
+          scores(0, 0, 0);
+          if (two) scores(1, 0, 0);
+          scores(0, 1, 0);
+          if (two) scores(1, 1, 0);
+          tc_commit(smem_u32(&bar_k_empty[0]));
         }
         __syncwarp();
-      };
-      bool ok = true;
-      if (tiles > 0) {
-        ok = mbar_wait(smem_u32(&bar_k_full[0]), 0, abort_flag);
-        if (ok) {
-          tc_fence_after();
-          for (int h = 0; h < 2; ++h)
-            for (int g = 0; g < groups; ++g) scores(g, h, 0);
-          if (elect_one()) tc_commit(smem_u32(&bar_k_empty[0]));
-          __syncwarp();
-        }
       }
       for (int i = 0; i < tiles && ok; ++i) {
         const int st = i & 1;
-        ok = mbar_wait(smem_u32(&bar_v_full[st]), (uint32_t)(i >> 1) & 1u, abort_flag);
-        if (ok && i + 1 < tiles) ok = mbar_wait(smem_u32(&bar_k_full[st ^ 1]), (uint32_t)((i + 1) >> 1) & 1u, abort_flag);
-#pragma unroll 1
-        for (int hg = 0; hg < 2 * groups && ok; ++hg) {
-          const int h = two ? hg >> 1 : hg, g = two ? hg & 1 : 0;
-          ok = mbar_wait(smem_u32(&bar_p_ready[g][h]), (uint32_t)i & 1u, abort_flag);
-          if (!ok) break;
+        const bool more = i + 1 < tiles;
+#pragma unroll
+        for (int hg = 0; hg < 4; ++hg) {
+          const int h = hg >> 1, g = hg & 1;
+          if (!ok || (g == 1 && !two)) continue;
+          uint32_t bar = smem_u32(&bar_p_ready[g][h]), parity = (uint32_t)i & 1u;
+          if (hg == 0) {
+            if (lane & 1) { bar = v_full0 + 8 * st; parity = (uint32_t)(i >> 1) & 1u; }
+            if (more && (lane & 2)) { bar = k_full0 + 8 * (st ^ 1); parity = (uint32_t)((i + 1) >> 1) & 1u; }
+          }
+          ok = wait_all(bar, parity);
+          if (!ok) continue;
           tc_fence_after();
           if (elect_one()) {
-            const uint64_t vd = make_n_major_desc(v_addr + st * kKvTile + h * kHalf * 128);
-#pragma unroll
-            for (int k = 0; k < kHalf / 16; ++k)
-              tc_mma_f16_ta(tmem_base + (uint32_t)(256 + 128 * g), tmem_base + (uint32_t)(128 * g + kHalf * h + 8 * k),
-                            vd + (uint64_t)(k * (16 * 128 >> 4)), idesc_o, i > 0 || h > 0 || k > 0 ? 1u : 0u);
-            tc_commit(smem_u32(&bar_pv[g][h]));
+            products(g, h, st, i > 0 || h > 0 ? 1u : 0u);
+            if (more) scores(g, h, st ^ 1);
+            if (h == 1 && (g == 1 || !two)) {
+              tc_commit(smem_u32(&bar_v_empty[st]));
+              if (more) tc_commit(smem_u32(&bar_k_empty[st ^ 1]));
+            }
           }
           __syncwarp();
-          if (i + 1 < tiles) scores(g, h, st ^ 1);
         }
-        if (!ok) break;
-        if (elect_one()) {
-          tc_commit(smem_u32(&bar_v_empty[st]));
-          if (i + 1 < tiles) tc_commit(smem_u32(&bar_k_empty[st ^ 1]));
-        }
-        __syncwarp();
       }
     }
   } else {
