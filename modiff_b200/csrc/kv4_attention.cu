@@ -120,77 +120,12 @@ kv4_attention_kernel(const Kv4Attention p) {
   const int32_t* table = p.table + (int64_t)b * p.max_pages;
   const int length = min(max(__ldg(p.lengths + b), 0), p.max_pages * p.c.page_size);
 
-  // ---- queries: one warp per row, brought to fp16 by a power of two, laid out as MMA fragments
-  uint32_t* q_frag = reinterpret_cast<uint32_t*>(smem);       // [plane][nt][k step][lane][2]
-  for (int r = warp; r < R; r += kWarps) {
-    float x[D / 32];
-    float top = 0.0f, sum = 0.0f;
-    const int rr = row0 + r;
-    const bool real = r < rows_here;
-    const T* src = static_cast<const T*>(p.q) + (int64_t)b * p.qb + (int64_t)(rr / p.group) * p.qt +
-                   (int64_t)(head * p.group + rr % p.group) * p.qh;
-#pragma unroll
-    for (int e = 0; e < D / 32; ++e) {
-      x[e] = real ? to_f32<T>(src[lane + 32 * e]) : 0.0f;
-      top = fmaxf(top, fabsf(x[e]));
-      sum += x[e];
-    }
-    for (int o = 16; o > 0; o >>= 1) {
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    }
-    // power of two that brings the largest element to [2^14, 2^15); in two factors, for fp32's range
-    int e2 = 0;
-    if (top > 0.0f && top < INFINITY) { frexpf(top, &e2); e2 = 15 - e2; }
-    const float f1 = ldexpf(1.0f, e2 / 2), f2 = ldexpf(1.0f, e2 - e2 / 2);
-    if (lane == 0) {
-      // score = a (s_k (q' . code') + m_k b) with q' the scaled query and code' = code * unit
-      row_a[r] = ((p.scale2 / kUnit) / f1) / f2;
-      row_b[r] = sum * f1 * f2 * kUnit;
-    }
-#pragma unroll
-    for (int e = 0; e < D / 32; ++e) {
-      const int ch = lane + 32 * e;
-      // thread j of an MMA holds channels [j D/4, (j + 1) D/4): word w, nibble n of them
-      const int tj = ch / (D / 4), w = ch % (D / 4) / 8, n = ch % 8;
-      const int step = 2 * w + ((n >> 1) & 1), reg = n & 1, half_at = n >> 2;
-      float v = x[e] * f1 * f2;
-      if (n & 1) v *= 0.0625f;
-      __half* dst = reinterpret_cast<__half*>(
-          &q_frag[(((r >> 3) * (D / 16) + step) * 32 + ((r & 7) * 4 + tj)) * 2 + reg]) + half_at;
-      const __half hi = __float2half_rn(v);
-      *dst = hi;
-      if (P == 2) dst[NT * (D / 16) * 32 * 2 * 2] = __float2half_rn(v - __half2float(hi));
-    }
-  }
-  __syncthreads();
-
   const int pos_lo = length - p.count + row0 / p.group;
   const int pos_hi = length - p.count + (row0 + rows_here - 1) / p.group;
   const TileRange range = tiles_of<kTile>(p, length, pos_lo, pos_hi);
   const int t_begin = (int)((int64_t)range.count * split / p.splits);
   const int t_end = (int)((int64_t)range.count * (split + 1) / p.splits);
 
-  float o[D / 16][NT][4];
-  float m_run[NT][2];
-  uint64_t l_run[NT], s_run[NT], ra[NT], rb[NT];   // pairs: query rows 2j and 2j + 1 of the eight
-  int pos[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[i][nt][e] = 0.0f;
-    const int r = 8 * nt + 2 * j;
-    l_run[nt] = s_run[nt] = 0ull;
-    ra[nt] = pack2(row_a[r], row_a[r + 1]);
-    rb[nt] = pack2(row_b[r], row_b[r + 1]);
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      m_run[nt][e] = -INFINITY;
-      pos[nt][e] = length - p.count + (row0 + r + e) / p.group;
-    }
-  }
   constexpr int kRow = D / 2;                     // bytes of a token's codes
   const uint8_t* k_lane = p.c.k_codes + g * kRow + j * (D / 8);
   const uint8_t* v_lane = p.c.v_codes + 2 * j * kRow + g * (D / 16);
@@ -230,6 +165,75 @@ kv4_attention_kernel(const Kv4Attention p) {
   if (ti < t_end) {
     place(range.tile(ti) * kTile, base);
     load_keys(base);
+  }
+
+  // ---- queries: one warp per row, brought to fp16 by a power of two, laid out as MMA fragments
+  uint32_t* q_frag = reinterpret_cast<uint32_t*>(smem);       // [plane][nt][k step][lane][2]
+  for (int r = warp; r < R; r += kWarps) {
+    float x[D / 32];
+    float top = 0.0f, sum = 0.0f;
+    const int rr = row0 + r;
+    const bool real = r < rows_here;
+    int member;
+    const int token = p.by_group.divmod(rr, member);
+    const T* src = static_cast<const T*>(p.q) + (int64_t)b * p.qb + (int64_t)token * p.qt +
+                   (int64_t)(head * p.group + member) * p.qh;
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) {
+      x[e] = real ? to_f32<T>(src[lane + 32 * e]) : 0.0f;
+      top = fmaxf(top, fabsf(x[e]));
+      sum += x[e];
+    }
+    for (int o = 16; o > 0; o >>= 1) {
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    }
+    // power of two that brings the largest element to [2^14, 2^15) (a subnormal one less far); in two
+    // factors, for fp32's range
+    int e2 = 0;
+    if (top > 0.0f && top < INFINITY) e2 = 141 - (int)(__float_as_uint(top) >> 23);
+    const float f1 = __int_as_float((127 + e2 / 2) << 23), f2 = __int_as_float((127 + e2 - e2 / 2) << 23);
+    if (lane == 0) {
+      // score = a (s_k (q' . code') + m_k b) with q' the scaled query and code' = code * unit
+      row_a[r] = p.scale2 / kUnit * __int_as_float((127 - e2 / 2) << 23) * __int_as_float((127 - (e2 - e2 / 2)) << 23);
+      row_b[r] = sum * f1 * f2 * kUnit;
+    }
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) {
+      const int ch = lane + 32 * e;
+      // thread j of an MMA holds channels [j D/4, (j + 1) D/4): word w, nibble n of them
+      const int tj = ch / (D / 4), w = ch % (D / 4) / 8, n = ch % 8;
+      const int step = 2 * w + ((n >> 1) & 1), reg = n & 1, half_at = n >> 2;
+      float v = x[e] * f1 * f2;
+      if (n & 1) v *= 0.0625f;
+      __half* dst = reinterpret_cast<__half*>(
+          &q_frag[(((r >> 3) * (D / 16) + step) * 32 + ((r & 7) * 4 + tj)) * 2 + reg]) + half_at;
+      const __half hi = __float2half_rn(v);
+      *dst = hi;
+      if (P == 2) dst[NT * (D / 16) * 32 * 2 * 2] = __float2half_rn(v - __half2float(hi));
+    }
+  }
+  __syncthreads();
+
+  float o[D / 16][NT][4];
+  float m_run[NT][2];
+  uint64_t l_run[NT], s_run[NT], ra[NT], rb[NT];   // pairs: query rows 2j and 2j + 1 of the eight
+  int pos[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][nt][e] = 0.0f;
+    const int r = 8 * nt + 2 * j;
+    l_run[nt] = s_run[nt] = 0ull;
+    ra[nt] = pack2(row_a[r], row_a[r + 1]);
+    rb[nt] = pack2(row_b[r], row_b[r + 1]);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      m_run[nt][e] = -INFINITY;
+      pos[nt][e] = length - p.count + (row0 + r + e) / p.group;
+    }
   }
   for (; ti < t_end; ti += kWarps) {
     const int t0 = range.tile(ti) * kTile;

@@ -14,14 +14,15 @@
 namespace modiff {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 
 struct NormRopeSide {
   const void* x;
   void* y;
   int64_t x_token, x_head, y_token, y_head;   // element strides
   const float* w;                             // [d] or NULL
-  int heads, groups;                          // groups of `step` heads
+  int heads;
+  FastDiv groups;                             // of `step` heads, per token
 };
 
 struct NormRopeParams {
@@ -29,7 +30,8 @@ struct NormRopeParams {
   const float* cos;
   const float* sin;
   const void* positions;     // int32 / int64 [tokens], or NULL: row = token
-  int64_t tokens, table_rows, items_q, items;
+  int64_t tokens, table_rows;
+  int items_q, items;
   int pos64, d, half, units, rot_units;
   float eps;
 };
@@ -39,13 +41,13 @@ template <typename T, int V, int NU, int LANES, int STEP, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads)
 qk_norm_rope_kernel(const NormRopeParams p) {
   const int lane = threadIdx.x % LANES;
-  const int64_t item = (int64_t)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
+  const int item = blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
   const bool is_q = item < p.items_q;
   const NormRopeSide& s = is_q ? p.q : p.k;
-  const int64_t local = is_q ? item : item - p.items_q;
   const bool live = item < p.items;
-  const int64_t token = live ? local / s.groups : 0;
-  const int head0 = live ? (int)(local % s.groups) * STEP : 0;
+  int group = 0;
+  const int64_t token = live ? s.groups.divmod(is_q ? item : item - p.items_q, group) : 0;
+  const int head0 = group * STEP;
   const int heads = live ? min(STEP, s.heads - head0) : 0;
 
   int64_t row = token;
@@ -91,18 +93,12 @@ qk_norm_rope_kernel(const NormRopeParams p) {
     for (int i = 0; i < V; ++i) { co[u][i] = 1.0f; si[u][i] = 0.0f; wa[u][i] = wb[u][i] = 1.0f; }
     if (live && mine[u]) {
       if (unit < p.rot_units && inside) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          co[u][i] = __ldg(p.cos + row * p.half + V * unit + i);
-          si[u][i] = __ldg(p.sin + row * p.half + V * unit + i);
-        }
+        load_f32<float, V>(p.cos + row * p.half + V * unit, co[u]);
+        load_f32<float, V>(p.sin + row * p.half + V * unit, si[u]);
       }
       if (s.w) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          wa[u][i] = __ldg(s.w + first[u] + i);
-          wb[u][i] = __ldg(s.w + second[u] + i);
-        }
+        load_f32<float, V>(s.w + first[u], wa[u]);
+        load_f32<float, V>(s.w + second[u], wb[u]);
       }
     }
   }
@@ -163,23 +159,25 @@ qk_norm_rope_kernel(const NormRopeParams p) {
 template <typename T, int V, int NU, int LANES, bool IL>
 int launch(NormRopeParams& p, cudaStream_t stream) {
   constexpr int kGroups = kThreads / LANES;
-  auto plan = [&](int step) {
-    p.q.groups = ceil_div(p.q.heads, step);
-    p.k.groups = ceil_div(p.k.heads, step);
-    p.items_q = p.tokens * p.q.groups;
-    p.items = p.items_q + p.tokens * p.k.groups;
-    return ceil_div64(p.items, kGroups);
+  auto plan = [&](int step) -> int64_t {
+    const int qg = p.q.heads ? ceil_div(p.q.heads, step) : 1, kg = p.k.heads ? ceil_div(p.k.heads, step) : 1;
+    p.q.groups = FastDiv(qg);
+    p.k.groups = FastDiv(kg);
+    const int64_t items_q = p.q.heads ? p.tokens * qg : 0, items = items_q + (p.k.heads ? p.tokens * kg : 0);
+    p.items_q = (int)items_q;
+    p.items = (int)items;
+    return items;
   };
   // several heads of a token per group once every SM still gets eight blocks
   constexpr int kStep = NU == 1 ? 4 : 1;
-  int64_t blocks = plan(kStep);
-  const bool wide = kStep > 1 && blocks >= 8 * (int64_t)device_sms();
-  if (!wide) blocks = plan(1);
-  MODIFF_CHECK_ARG(blocks <= 0x7fffffff, "too many tokens");
+  const bool wide = kStep > 1 && plan(kStep) >= 8ll * device_sms() * kGroups;
+  const int64_t items = plan(wide ? kStep : 1);
+  MODIFF_CHECK_ARG(items <= 0x7fffffff - kGroups, "too many tokens");
+  const unsigned blocks = (unsigned)ceil_div64(items, kGroups);
   if (wide)
-    qk_norm_rope_kernel<T, V, NU, LANES, kStep, IL><<<(unsigned)blocks, kThreads, 0, stream>>>(p);
+    qk_norm_rope_kernel<T, V, NU, LANES, kStep, IL><<<blocks, kThreads, 0, stream>>>(p);
   else
-    qk_norm_rope_kernel<T, V, NU, LANES, 1, IL><<<(unsigned)blocks, kThreads, 0, stream>>>(p);
+    qk_norm_rope_kernel<T, V, NU, LANES, 1, IL><<<blocks, kThreads, 0, stream>>>(p);
   MODIFF_LAUNCH_CHECK("qk_norm_rope_kernel");
   return MODIFF_OK;
 }
@@ -217,8 +215,8 @@ extern "C" int modiff_qk_norm_rope(const void* q, int64_t q_token, int64_t q_hea
   if (tokens == 0 || q_heads + k_heads == 0) return MODIFF_OK;
 
   NormRopeParams p = {};
-  p.q = NormRopeSide{q, q_out, q_token, q_head, q_out_token, q_out_head, q_weight, q_heads, 0};
-  p.k = NormRopeSide{k, k_out, k_token, k_head, k_out_token, k_out_head, k_weight, k_heads, 0};
+  p.q = NormRopeSide{q, q_out, q_token, q_head, q_out_token, q_out_head, q_weight, q_heads, FastDiv()};
+  p.k = NormRopeSide{k, k_out, k_token, k_head, k_out_token, k_out_head, k_weight, k_heads, FastDiv()};
   p.cos = cos;
   p.sin = sin;
   p.positions = rot ? positions : nullptr;
@@ -236,8 +234,12 @@ extern "C" int modiff_qk_norm_rope(const void* q, int64_t q_token, int64_t q_hea
     if (s->heads)
       align |= (uintptr_t)s->x | (uintptr_t)s->y |
                (uintptr_t)((s->x_token | s->x_head | s->y_token | s->y_head) * size);
+  // tables and weights are read as v fp32 values at a time: at most 16 bytes each
+  uintptr_t align4 = (uintptr_t)p.q.w | (uintptr_t)p.k.w;
+  if (rot) align4 |= (uintptr_t)cos | (uintptr_t)sin;
+  MODIFF_CHECK_ARG(align4 % 4 == 0, "misaligned table or weight");
   int v = 16 / size;
-  while (v > 1 && (align % (v * size) != 0 || (interleaved ? rot % (2 * v) != 0 || d % (2 * v) != 0
+  while (v > 1 && (align4 % (v >= 4 ? 16 : 4 * v) != 0 || align % (v * size) != 0 || (interleaved ? rot % (2 * v) != 0 || d % (2 * v) != 0
                                                            : p.half % v != 0 || (d - rot) % (2 * v) != 0)))
     v /= 2;
   MODIFF_CHECK_ARG(align % size == 0, "misaligned tensor");

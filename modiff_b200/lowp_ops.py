@@ -151,11 +151,11 @@ def fp8_linear(x, w, w_scale, bias=None):
         if bias.dtype != dtype or bias.shape != (n,):
             raise ModiffError(f"fp8_linear: bias of {n} values of {dtype}, got {tuple(bias.shape)} {bias.dtype}")
         bias = bias.contiguous()
+    if not ready:
+        return _fp8_linear_rows(device, x, w, n, k, w_pitch, w_scale, blocks, bias, dt)
     lead = tuple(src.shape[:-1])
     y = torch.empty(lead + (n,), dtype=dtype, device=src.device)
-    if y.numel() == 0:
-        return y
-    if ready:
+    if y.numel():
         kp = -(-k // 16) * 16
         rows = lead[0] if len(lead) == 1 else y.numel() // n
         if rows > 0x7fffffff:
@@ -170,16 +170,23 @@ def fp8_linear(x, w, w_scale, bias=None):
         _call(device, 'modiff_fp8_linear', src.data_ptr(), kp, x.scale.data_ptr(), row4, w.data_ptr(), w_pitch,
               w_scale.data_ptr(), blocks, _lib.ptr(bias), y.data_ptr(), n, rows, k, n, dt,
               nbytes=rows * kp + n * k + y.numel() * y.element_size(), nops=2 * rows * n * k)
-        return y
+    return y
+
+
+def _fp8_linear_rows(device, x, w, n, k, w_pitch, w_scale, blocks, bias, dt):
+    """`fp8_linear` of a tensor: quantised inside the product, or into a workspace before it."""
     at, pitch, rows, _, keep = _rows("fp8_linear", x)
     if rows > 0x7fffffff:
         raise ModiffError("fp8_linear: too many rows")
-    size = _lib.lib().modiff_fp8_linear_bytes(rows, k, n)
-    work = torch.empty(size, dtype=torch.uint8, device=src.device) if size else None
-    _call(device, 'modiff_fp8_linear_x', at, pitch, w.data_ptr(), w_pitch, w_scale.data_ptr(), blocks, _lib.ptr(bias),
-          y.data_ptr(), n, rows, k, n, dt, _lib.ptr(work),
-          nbytes=(rows * k + y.numel()) * y.element_size() + n * k, nops=2 * rows * n * k, more=int(size > 0))
-    return y
+    y = keep.new_empty((rows, n))
+    if rows:
+        size = _lib.lib().modiff_fp8_linear_bytes(rows, k, n)
+        work = keep.new_empty(size, dtype=torch.uint8) if size else None
+        _call(device, 'modiff_fp8_linear_x', at, pitch, w.data_ptr(), w_pitch, w_scale.data_ptr(), blocks,
+              None if bias is None else bias.data_ptr(), y.data_ptr(), n, rows, k, n, dt,
+              None if work is None else work.data_ptr(),
+              nbytes=rows * (k + n) * x.element_size() + n * k, nops=2 * rows * n * k, more=int(size > 0))
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], n)
 
 
 def _pitched(t, pitch, step):
