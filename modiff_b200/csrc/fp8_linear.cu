@@ -48,74 +48,116 @@ struct QuantParams {
   float* scale;
   int64_t scale_pitch;
   int64_t rows;
-  int k, blocks, col_groups;
+  int k, blocks;
+  FastDiv by_group;                         // groups of four blocks of a row
 };
 
-// x / s, correctly rounded, from r = 1 / s correctly rounded: two steps of Markstein's refinement (IBM J.
-// Res. Dev. 34, 1990): with q within one ulp the remainder x - q s is exact in a fused multiply-add, and
-// q + remainder * r rounds to the quotient.  Valid while nothing under- or overflows on the way.
-__device__ inline float divide_by(float x, float s, float r) {
-  float q = x * r;
-  q = fmaf(fmaf(-q, s, x), r, q);
-  return fmaf(fmaf(-q, s, x), r, q);
+// (x, y) / s, correctly rounded, from r = 1 / s correctly rounded: two steps of Markstein's refinement (IBM
+// J. Res. Dev. 34, 1990): with q within one ulp the remainder x - q s is exact in a fused multiply-add, and
+// q + remainder * r rounds to the quotient.  Valid while nothing under- or overflows on the way.  Five
+// instructions for two elements; the compiler's division alone was most of this kernel's time.
+__device__ inline float2 divide_pair(float x, float y, uint64_t r, uint64_t minus_s) {
+  uint64_t v, q, e;
+  float2 out;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(q) : "l"(v), "l"(r));
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(e) : "l"(q), "l"(minus_s), "l"(v));
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(q) : "l"(e), "l"(r));
+  }
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(out.x), "=f"(out.y) : "l"(q));
+  return out;
 }
 
-// Sixteen lanes own a block of 128 channels of one row, 8 each, and do kQuantBlocks blocks of that row one
-// after the other, all loads first; the sixteen groups of a CTA have neighbouring rows, whose scales
-// lie next to each other.  Bound: HBM, size + 1 bytes an element.
-constexpr int kQuantBlocks = 4;
+// Largest magnitude of the elements in a word (or a float): as integers, where a NaN is above infinity.
+template <typename T> __device__ inline uint32_t magnitude_max(uint32_t top, uint32_t w) {
+  if constexpr (sizeof(T) == 4) return max(top, w & 0x7fffffffu);
+  else return __vmaxu2(top, w & 0x7fff7fffu);
+}
+template <typename T> __device__ inline float magnitude_value(uint32_t top) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(top);
+  else {
+    const uint16_t h = (uint16_t)max(top & 0xffffu, top >> 16);
+    return to_f32<T>(*reinterpret_cast<const T*>(&h));
+  }
+}
+// The two elements of a word of 16-bit values, or of two fp32 words.
+template <typename T> __device__ inline float2 pair_of(const uint32_t* w, int i) {
+  if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+  else return make_float2(to_f32<T>(reinterpret_cast<const T*>(w)[2 * i]), to_f32<T>(reinterpret_cast<const T*>(w)[2 * i + 1]));
+}
+
+// Eight lanes own a block of 128 channels of one row, 16 each; a warp does four neighbouring blocks of ROWS
+// neighbouring rows, whose scales of a block it writes as one access.  All loads come first.  Bound: HBM,
+// size + 1 bytes an element.
+template <typename T> constexpr int kQuantRows = sizeof(T) == 4 ? 2 : 4;
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
 fp8_quantize_kernel(const QuantParams p) {
+  constexpr int kRows = kQuantRows<T>, kWords = 16 * sizeof(T) / 4;
   // a linear layer behind this kernel may bring its weights in meanwhile; it waits before it reads rows
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int lane = threadIdx.x & 15;
-  const int64_t row = (int64_t)(blockIdx.x / p.col_groups) * 16 + (threadIdx.x >> 4);
-  const int blk0 = (int)(blockIdx.x % p.col_groups) * kQuantBlocks;
-  const bool live = row < p.rows;
-  float x[kQuantBlocks][8];
+  const int lane = threadIdx.x & 7;
+  int group;
+  const int64_t row0 = (int64_t)kRows * p.by_group.divmod(blockIdx.x * 8 + (threadIdx.x >> 5), group);
+  const int blk = group * 4 + ((threadIdx.x >> 3) & 3);
+  const int c0 = blk * kBlock + 16 * lane;
+  const bool live = blk < p.blocks && row0 < p.rows;
+  uint32_t w[kRows][kWords];
 #pragma unroll
-  for (int u = 0; u < kQuantBlocks; ++u) {
-    const int c0 = (blk0 + u) * kBlock + 8 * lane;
+  for (int u = 0; u < kRows; ++u) {
+    const T* src = static_cast<const T*>(p.x) + (row0 + u) * p.x_pitch + c0;
+    const bool here = live && row0 + u < p.rows && c0 < p.k;
+    if (VEC && here && c0 + 16 <= p.k) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[u][e] = 0.0f;
-    if (live && c0 < p.k) {
-      const T* src = static_cast<const T*>(p.x) + row * p.x_pitch + c0;
-      if (VEC && c0 + 8 <= p.k) {
-        load_f32<T, 8>(src, x[u]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (c0 + e < p.k) x[u][e] = to_f32<T>(src[e]);
+      for (int i = 0; i < kWords / 4; ++i) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + i);
+        w[u][4 * i] = v.x; w[u][4 * i + 1] = v.y; w[u][4 * i + 2] = v.z; w[u][4 * i + 3] = v.w;
       }
+    } else {
+      T* t = reinterpret_cast<T*>(w[u]);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) t[e] = here && c0 + e < p.k ? src[e] : from_f32<T>(0.0f);
     }
   }
+  float scale[kRows];
 #pragma unroll
-  for (int u = 0; u < kQuantBlocks; ++u) {
-    float top = 0.0f;
+  for (int u = 0; u < kRows; ++u) {
+    uint32_t top = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) top = larger_or_nan(fabsf(x[u][e]), top);
+    for (int i = 0; i < kWords; ++i) top = magnitude_max<T>(top, w[u][i]);
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) top = larger_or_nan(__shfl_xor_sync(0xffffffffu, top, o), top);
-    const int c0 = (blk0 + u) * kBlock + 8 * lane;
-    if (!live || blk0 + u >= p.blocks) continue;
-    const float s = block_scale(top);
+    for (int o = 4; o > 0; o >>= 1) top = magnitude_max<T>(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float s = block_scale(magnitude_value<T>(top));
+    scale[u] = s;
+    if (!live || row0 + u >= p.rows) continue;
+    uint32_t codes[4];
     if (s > 1e-25f && s < 1e25f) {
+      uint64_t r2, ms2;
       const float r = __frcp_rn(s);
+      asm("mov.b64 %0, {%1, %1};" : "=l"(r2) : "f"(r));
+      asm("mov.b64 %0, {%1, %1};" : "=l"(ms2) : "f"(-s));
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[u][e] = divide_by(x[u][e], s, r);
+      for (int i = 0; i < 4; ++i) {
+        const float2 a = pair_of<T>(w[u], 2 * i), b = pair_of<T>(w[u], 2 * i + 1);
+        const float2 qa = divide_pair(a.x, a.y, r2, ms2), qb = divide_pair(b.x, b.y, r2, ms2);
+        codes[i] = e4m3_x4(qa.x, qa.y, qb.x, qb.y);
+      }
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[u][e] = __fdiv_rn(x[u][e], s);
+      for (int i = 0; i < 4; ++i) {
+        const float2 a = pair_of<T>(w[u], 2 * i), b = pair_of<T>(w[u], 2 * i + 1);
+        codes[i] = e4m3_x4(__fdiv_rn(a.x, s), __fdiv_rn(a.y, s), __fdiv_rn(b.x, s), __fdiv_rn(b.y, s));
+      }
     }
-    if (c0 < p.code_pitch) {                     // the pitch is a multiple of 16
-      uint2 w;
-      w.x = e4m3_x4(x[u][0], x[u][1], x[u][2], x[u][3]);
-      w.y = e4m3_x4(x[u][4], x[u][5], x[u][6], x[u][7]);
-      *reinterpret_cast<uint2*>(p.codes + row * p.code_pitch + c0) = w;
-    }
-    if (lane == 0) p.scale[(blk0 + u) * p.scale_pitch + row] = s;
+    if (c0 < p.code_pitch)                       // the pitch is a multiple of 16
+      *reinterpret_cast<uint4*>(p.codes + (row0 + u) * p.code_pitch + c0) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+  }
+  if (lane == 0 && live) {
+    float* dst = p.scale + blk * p.scale_pitch + row0;         // the pitch covers whole groups of four rows
+    store_f32<float, kRows>(dst, scale);
   }
 }
 
@@ -532,9 +574,11 @@ static int64_t scale_row(int rows) { return ((int64_t)rows + 3) / 4 * 4; }
 static int quantize_rows(const void* x, int64_t x_pitch, int64_t rows, int k, int dtype, uint8_t* codes,
                          int64_t code_pitch, float* scale, int64_t scale_pitch, cudaStream_t s) {
   const int size = dtype_bytes(dtype), blocks = ceil_div(k, kBlock);
-  QuantParams p{x, x_pitch, codes, code_pitch, scale, scale_pitch, rows, k, blocks, ceil_div(blocks, kQuantBlocks)};
-  const int64_t grid = ceil_div64(rows, 16) * p.col_groups;
-  MODIFF_CHECK_ARG(grid <= 0x7fffffff, "too many rows");
+  const int groups = ceil_div(blocks, 4), per = size == 4 ? kQuantRows<float> : kQuantRows<__half>;
+  QuantParams p{x, x_pitch, codes, code_pitch, scale, scale_pitch, rows, k, blocks, FastDiv(groups)};
+  const int64_t warps = ceil_div64(rows, per) * groups;
+  MODIFF_CHECK_ARG(warps <= 0x7fffffff - 8, "too many rows");
+  const int64_t grid = ceil_div64(warps, 8);
   const bool vec = (((uintptr_t)x | (uintptr_t)(x_pitch * size)) & 15) == 0;
   return with_dtype(dtype, [&](auto tag) {
     using T = decltype(tag);
