@@ -52,24 +52,6 @@ struct QuantParams {
   FastDiv by_group;                         // groups of four blocks of a row
 };
 
-// (x, y) / s, correctly rounded, from r = 1 / s correctly rounded: two steps of Markstein's refinement (IBM
-// J. Res. Dev. 34, 1990): with q within one ulp the remainder x - q s is exact in a fused multiply-add, and
-// q + remainder * r rounds to the quotient.  Valid while nothing under- or overflows on the way.  Five
-// instructions for two elements; the compiler's division alone was most of this kernel's time.
-__device__ inline float2 divide_pair(float x, float y, uint64_t r, uint64_t minus_s) {
-  uint64_t v, q, e;
-  float2 out;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(q) : "l"(v), "l"(r));
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(e) : "l"(q), "l"(minus_s), "l"(v));
-    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(q) : "l"(e), "l"(r));
-  }
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(out.x), "=f"(out.y) : "l"(q));
-  return out;
-}
-
 // Largest magnitude of the elements in a word (or a float): as integers, where a NaN is above infinity.
 template <typename T> __device__ inline uint32_t magnitude_max(uint32_t top, uint32_t w) {
   if constexpr (sizeof(T) == 4) return max(top, w & 0x7fffffffu);

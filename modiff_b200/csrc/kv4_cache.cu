@@ -13,12 +13,15 @@
 // Bound: HBM, one read of the new tokens and one write of d / 2 + 4 bytes per row (and launch latency
 // for a step of single tokens).  LANES lanes own a row, 8 channels each, in registers between the
 // extremes and the codes.
+#include <type_traits>
+
 #include "kv4.cuh"
 
 namespace modiff {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
+constexpr int64_t kMostRows = 0x7fffffff - kThreads;   // rows of one call: their numbers are 32-bit
 
 struct AppendParams {
   const void *k, *v;
@@ -26,70 +29,127 @@ struct AppendParams {
   Kv4Pages c;
   const int32_t* table;
   const int32_t* lengths;
-  int batch, count, max_pages;
-  int64_t rows;                       // batch * count * heads
+  int count, max_pages, rows;         // batch * count * heads
+  FastDiv by_heads, by_count;
 };
+
+// Smaller and larger of two numbers, a NaN if either is one.
+__device__ inline float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ inline float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// Extremes of a row whose channels LANES lanes hold eight each; 16-bit values two at a time, and between
+// lanes both extremes as one word (the smaller of the values and of their negatives).
+template <typename T, int LANES>
+__device__ inline void extremes(const Pack<T, 8>& x, bool mine, float& low, float& high) {
+  if constexpr (sizeof(T) == 4) {
+    low = INFINITY; high = -INFINITY;
+    if (mine) {
+      low = high = x.v[0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) { low = min_nan(low, x.v[e]); high = max_nan(high, x.v[e]); }
+    }
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) {
+      low = min_nan(low, __shfl_xor_sync(0xffffffffu, low, o));
+      high = max_nan(high, __shfl_xor_sync(0xffffffffu, high, o));
+    }
+  } else {
+    using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+    const T2* w = reinterpret_cast<const T2*>(x.v);
+    T2 both;
+    both.x = both.y = from_f32<T>(INFINITY);
+    if (mine) {
+      const T2 lo = __hmin2_nan(__hmin2_nan(w[0], w[1]), __hmin2_nan(w[2], w[3]));
+      const T2 hi = __hneg2(__hmax2_nan(__hmax2_nan(w[0], w[1]), __hmax2_nan(w[2], w[3])));
+      T2 a, b;
+      a.x = lo.x; a.y = hi.x; b.x = lo.y; b.y = hi.y;
+      both = __hmin2_nan(a, b);
+    }
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) both = __hmin2_nan(both, __shfl_xor_sync(0xffffffffu, both, o));
+    low = to_f32<T>(both.x);
+    high = -to_f32<T>(both.y);
+  }
+}
+
+// Eight values as codes; the scale and minimum of their row.
+template <typename T, int LANES>
+__device__ inline uint32_t encode(const Pack<T, 8>& in, bool mine, __half2& params) {
+  float low, high;
+  extremes<T, LANES>(in, mine, low, high);
+  float x[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = to_f32<T>(in.v[e]);
+  if (low < -65504.0f || high > 65504.0f) {
+    low = fminf(fmaxf(low, -65504.0f), 65504.0f);
+    high = fminf(fmaxf(high, -65504.0f), 65504.0f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = fminf(fmaxf(x[e], -65504.0f), 65504.0f);
+  }
+  const __half s = __float2half_rn(__fmul_rn(__fsub_rn(high, low), 1.0f / 15.0f)), m = __float2half_rn(low);
+  params = __halves2half2(s, m);
+  const float sf = __half2float(s), mf = __half2float(m);
+  if (!(sf > 0.0f)) return 0;
+  // s is a fp16 number above 0: nothing under- or overflows where the code is not 0 anyway
+  const float inv = __frcp_rn(sf);
+  const uint64_t r = pack2(inv, inv), minus_s = pack2(-sf, -sf), minus_m = pack2(-mf, -mf);
+  // adding 1.5 2^23 rounds to an integer, ties to even, and leaves it in the low bits
+  const uint64_t bias = pack2(12582912.0f, 12582912.0f);
+  uint32_t packed = 0;
+#pragma unroll
+  for (int e = 6; e >= 0; e -= 2) {
+    const float2 d = unpack2(add2(pack2(x[e], x[e + 1]), minus_m));
+    const float2 q = divide_pair(d.x, d.y, r, minus_s);
+    const float2 n = unpack2(add2(pack2(fminf(fmaxf(q.x, 0.0f), 15.0f), fminf(fmaxf(q.y, 0.0f), 15.0f)), bias));
+    packed = (packed << 4) + __float_as_uint(n.y);
+    packed = (packed << 4) + __float_as_uint(n.x);
+  }
+  // what 0x4b400000 of each of the eight adds up to, modulo 2^32
+  return packed - (0x4b400000u + 0xb4000000u + 0x40000000u);
+}
 
 template <typename T, int LANES, bool VEC>
 __global__ void __launch_bounds__(kThreads)
 kv4_append_kernel(const AppendParams p) {
   const int lane = threadIdx.x % LANES;
-  const int64_t item = (int64_t)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
-  const bool value = item >= p.rows;
-  const int64_t row = value ? item - p.rows : item;
+  const int row = blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
   bool live = row < p.rows;
-  const int head = live ? (int)(row % p.c.heads) : 0;
-  const int64_t bt = live ? row / p.c.heads : 0;
-  const int i = (int)(bt % p.count), b = (int)(bt / p.count);
-  const int at = live ? max(__ldg(p.lengths + b), 0) - p.count + i : -1;
-  const int64_t place = kv4_place(p.c, p.table + (int64_t)b * p.max_pages, p.max_pages, at, head);
-  live = live && place >= 0;
+  int head = 0, i = 0, b = 0;
+  if (live) b = p.by_heads.divmod(p.by_count.divmod(row, i), head);
   const bool mine = live && 8 * lane < p.c.dim;
-
-  float x[8];
-  float low = INFINITY, high = -INFINITY;
-  bool bad = false;
-  if (mine) {
-    const T* src = static_cast<const T*>(value ? p.v : p.k) +
-                   (value ? b * p.vb + i * p.vt + head * p.vh : b * p.kb + i * p.kt + head * p.kh) + 8 * lane;
-    if (VEC) {
-      load_f32<T, 8>(src, x);
-    } else {
+  Pack<T, 8> x[2];
+  if (mine) {                         // on their way before the page number is known
+    const T* src[2] = {static_cast<const T*>(p.k) + (b * p.kb + i * p.kt + head * p.kh) + 8 * lane,
+                       static_cast<const T*>(p.v) + (b * p.vb + i * p.vt + head * p.vh) + 8 * lane};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = to_f32<T>(src[e]);
-    }
+    for (int u = 0; u < 2; ++u) {
+      if (VEC) {
+        x[u] = *reinterpret_cast<const Pack<T, 8>*>(src[u]);
+      } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      bad |= isnan(x[e]);
-      x[e] = fminf(fmaxf(x[e], -65504.0f), 65504.0f);
-      low = fminf(low, x[e]);
-      high = fmaxf(high, x[e]);
+        for (int e = 0; e < 8; ++e) x[u].v[e] = src[u][e];
+      }
     }
   }
-  int any = bad;
+  int64_t place = -1;
+  if (live)
+    place = kv4_place(p.c, p.table + (int64_t)b * p.max_pages, p.max_pages, max(__ldg(p.lengths + b), 0) - p.count + i,
+                      head);
 #pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) {
-    low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
-    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
-    any |= __shfl_xor_sync(0xffffffffu, any, o);
-  }
-  if (!mine) return;
-  const __half s = __float2half_rn(any ? __int_as_float(0x7fc00000) : __fmul_rn(__fsub_rn(high, low), 1.0f / 15.0f));
-  const __half m = __float2half_rn(any ? __int_as_float(0x7fc00000) : low);
-  const float sf = __half2float(s), mf = __half2float(m);
-  uint32_t packed = 0;
-  if (sf > 0.0f) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float q = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[e], mf), sf)), 0.0f), 15.0f);
-      packed |= (uint32_t)q << (4 * e);
-    }
-  }
-  uint8_t* codes = value ? p.c.v_codes : p.c.k_codes;
-  *reinterpret_cast<uint32_t*>(codes + place * (p.c.dim / 2) + 4 * lane) = packed;
-  if (lane == 0) {
-    __half2* params = reinterpret_cast<__half2*>(value ? p.c.v_params : p.c.k_params);
-    params[place] = __halves2half2(s, m);
+  for (int u = 0; u < 2; ++u) {
+    __half2 sm;
+    const uint32_t packed = encode<T, LANES>(x[u], mine, sm);
+    if (!mine || place < 0) continue;
+    *reinterpret_cast<uint32_t*>((u ? p.c.v_codes : p.c.k_codes) + place * (p.c.dim / 2) + 4 * lane) = packed;
+    if (lane == 0) reinterpret_cast<__half2*>(u ? p.c.v_params : p.c.k_params)[place] = sm;
   }
 }
 
@@ -98,46 +158,54 @@ struct ReadParams {
   const int32_t* table;
   const int32_t* lengths;
   void *k, *v;                        // [batch][count][heads][dim]
-  int batch, count, max_pages;
-  int64_t items;                      // batch * count * heads * dim / 8
+  int count, max_pages, rows;         // batch * count * heads
+  FastDiv by_heads, by_count;
 };
 
-template <typename T>
+template <typename T, int LANES>
 __global__ void __launch_bounds__(kThreads)
 kv4_read_kernel(const ReadParams p) {
-  const int64_t item = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (item >= 2 * p.items) return;
-  const bool value = item >= p.items;
-  const int64_t local = value ? item - p.items : item;
-  const int chunks = p.c.dim / 8;
-  const int chunk = (int)(local % chunks);
-  const int64_t row = local / chunks;
-  const int head = (int)(row % p.c.heads);
-  const int64_t bt = row / p.c.heads;
-  const int i = (int)(bt % p.count), b = (int)(bt / p.count);
-  const int at = max(__ldg(p.lengths + b), 0) - p.count + i;
-  const int64_t place = kv4_place(p.c, p.table + (int64_t)b * p.max_pages, p.max_pages, at, head);
-  float x[8] = {};
+  const int lane = threadIdx.x % LANES;
+  const int row = blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
+  if (row >= p.rows || 8 * lane >= p.c.dim) return;
+  int head, i;
+  const int b = p.by_heads.divmod(p.by_count.divmod(row, i), head);
+  const int64_t place = kv4_place(p.c, p.table + (int64_t)b * p.max_pages, p.max_pages,
+                                  max(__ldg(p.lengths + b), 0) - p.count + i, head);
+  const int64_t to = (((int64_t)b * p.count + i) * p.c.heads + head) * p.c.dim;
+  uint32_t w[2] = {};
+  float2 sm[2] = {};
   if (place >= 0) {
-    const uint8_t* codes = value ? p.c.v_codes : p.c.k_codes;
-    const __half2* params = reinterpret_cast<const __half2*>(value ? p.c.v_params : p.c.k_params);
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(codes + place * (p.c.dim / 2) + 4 * chunk);
-    const float2 sm = __half22float2(params[place]);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = fmaf((float)((w >> (4 * e)) & 15u), sm.x, sm.y);
+    for (int u = 0; u < 2; ++u) {
+      w[u] = *reinterpret_cast<const uint32_t*>((u ? p.c.v_codes : p.c.k_codes) + place * (p.c.dim / 2) + 4 * lane);
+      sm[u] = __half22float2(reinterpret_cast<const __half2*>(u ? p.c.v_params : p.c.k_params)[place]);
+    }
   }
-  store_f32<T, 8>(static_cast<T*>(value ? p.v : p.k) + row * p.c.dim + 8 * chunk, x);
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = fmaf((float)((w[u] >> (4 * e)) & 15u), sm[u].x, sm[u].y);
+    store_f32<T, 8>(static_cast<T*>(u ? p.v : p.k) + to + 8 * lane, x);
+  }
 }
 
 template <typename T, int LANES>
 int launch_append(const AppendParams& p, bool vec, cudaStream_t s) {
-  const int64_t blocks = ceil_div64(2 * p.rows, kThreads / LANES);
-  MODIFF_CHECK_ARG(blocks <= 0x7fffffff, "too many tokens");
+  const unsigned blocks = (unsigned)ceil_div(p.rows, kThreads / LANES);
   if (vec)
-    kv4_append_kernel<T, LANES, true><<<(unsigned)blocks, kThreads, 0, s>>>(p);
+    kv4_append_kernel<T, LANES, true><<<blocks, kThreads, 0, s>>>(p);
   else
-    kv4_append_kernel<T, LANES, false><<<(unsigned)blocks, kThreads, 0, s>>>(p);
+    kv4_append_kernel<T, LANES, false><<<blocks, kThreads, 0, s>>>(p);
   MODIFF_LAUNCH_CHECK("kv4_append_kernel");
+  return MODIFF_OK;
+}
+
+template <typename T, int LANES>
+int launch_read(const ReadParams& p, cudaStream_t s) {
+  kv4_read_kernel<T, LANES><<<(unsigned)ceil_div(p.rows, kThreads / LANES), kThreads, 0, s>>>(p);
+  MODIFF_LAUNCH_CHECK("kv4_read_kernel");
   return MODIFF_OK;
 }
 
@@ -190,8 +258,12 @@ extern "C" int modiff_kv4_append(const modiff_kv4_cache* cache, const void* k, i
   p.vb = v_seq; p.vt = v_token; p.vh = v_head;
   p.c = kv4_pages(cache);
   p.table = table; p.lengths = lengths;
-  p.batch = batch; p.count = count; p.max_pages = max_pages;
-  p.rows = (int64_t)batch * count * cache->heads;
+  p.count = count; p.max_pages = max_pages;
+  const int64_t rows = (int64_t)batch * count * cache->heads;
+  MODIFF_CHECK_ARG((int64_t)batch * count <= kMostRows && rows <= kMostRows, "too many tokens");
+  p.rows = (int)rows;
+  p.by_heads = FastDiv(cache->heads);
+  p.by_count = FastDiv(count);
   const int size = dtype_bytes(dtype);
   const uintptr_t align = (uintptr_t)k | (uintptr_t)v |
                           (uintptr_t)((p.kb | p.kt | p.kh | p.vb | p.vt | p.vh) * size);
@@ -218,13 +290,17 @@ extern "C" int modiff_kv4_read(const modiff_kv4_cache* cache, const int32_t* tab
   p.c = kv4_pages(cache);
   p.table = table; p.lengths = lengths;
   p.k = k; p.v = v;
-  p.batch = batch; p.count = count; p.max_pages = max_pages;
-  p.items = (int64_t)batch * count * cache->heads * (cache->dim / 8);
-  const int64_t blocks = ceil_div64(2 * p.items, kThreads);
-  MODIFF_CHECK_ARG(blocks <= 0x7fffffff, "too many tokens");
+  p.count = count; p.max_pages = max_pages;
+  const int64_t rows = (int64_t)batch * count * cache->heads;
+  MODIFF_CHECK_ARG((int64_t)batch * count <= kMostRows && rows <= kMostRows, "too many tokens");
+  p.rows = (int)rows;
+  p.by_heads = FastDiv(cache->heads);
+  p.by_count = FastDiv(count);
+  cudaStream_t st = (cudaStream_t)stream;
   return with_dtype(dtype, [&](auto tag) {
-    kv4_read_kernel<decltype(tag)><<<(unsigned)blocks, kThreads, 0, (cudaStream_t)stream>>>(p);
-    MODIFF_LAUNCH_CHECK("kv4_read_kernel");
-    return MODIFF_OK;
+    using T = decltype(tag);
+    if (cache->dim == 64) return launch_read<T, 8>(p, st);
+    if (cache->dim == 128) return launch_read<T, 16>(p, st);
+    return launch_read<T, 32>(p, st);
   });
 }

@@ -39,6 +39,25 @@ __device__ inline void store_f32(T* dst, const float (&in)[N]) {
   for (int i = 0; i < N; ++i) p.v[i] = from_f32<T>(in[i]);
   *reinterpret_cast<Pack<T, N>*>(dst) = p;
 }
+
+// (x, y) / s, correctly rounded, from r = 1 / s correctly rounded: two steps of Markstein's refinement (IBM
+// J. Res. Dev. 34, 1990): with q within one ulp the remainder x - q s is exact in a fused multiply-add, and
+// q + remainder * r rounds to the quotient.  Valid while nothing under- or overflows on the way.  Five
+// instructions for two elements; the compiler's division alone was most of the
+// quantisers' time.
+__device__ inline float2 divide_pair(float x, float y, uint64_t r, uint64_t minus_s) {
+  uint64_t v, q, e;
+  float2 out;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(q) : "l"(v), "l"(r));
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(e) : "l"(q), "l"(minus_s), "l"(v));
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(q) : "l"(e), "l"(r));
+  }
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(out.x), "=f"(out.y) : "l"(q));
+  return out;
+}
 #endif
 
 // Calls `fn` with a value of the element type that `dtype` names.
