@@ -2,15 +2,15 @@
 //   out = sum_t p_t (s_v[t] code_v[t] + m_v[t]) / sum_t p_t,
 //   p_t = exp(scale * q . (s_k[t] code_k[t] + m_k[t])) over the tokens that the query sees.
 //
-// The codes go into the tensor cores as they are.  A nibble n in the low bits of an fp16 word is the
-// subnormal number n 2^-24, in bits 4 - 7 it is 16 n 2^-24, both exact, so that masks alone make MMA
-// operands out of eight packed codes' word (fp32 tensors: see codes_lower); the factors are taken out of
-// q and of the results.  Scale and minimum of a token leave the products:
+// The codes go into the tensor cores as they are, as small exact fp16 numbers (codes_lower below); the
+// factors are taken out of q and of the results.  Scale and minimum of a token leave the products:
 //   q . k_t = s_k (q . code) + m_k sum(q)            sum_t p_t v_t = sum_t (p_t s_v) code + sum_t p_t m_v
-// Queries are brought to fp16 by a power of two per row (exact for 16-bit types; fp32 queries and
-// weights travel as two fp16 planes, hi + lo, 22 bits).  p_t s_v is held in fp16 relative to the running
-// maximum of (score + exponent of s_v), so that it lies in [0, 2) 2^14 whatever the scales are.  Sums,
-// maxima and the output stay in fp32.
+// Queries are brought to fp16 by a power of two per row (exact for 16-bit types; fp32 queries travel as two
+// fp16 planes, hi + lo, 22 bits).  p_t s_v is held in fp16 relative to the running maximum of (score +
+// exponent of s_v), so that it lies in [0, 2) 2^14 whatever the scales are: in two planes for fp32 and fp16,
+// whose outputs then are as exact as their rounding, in one (2^-12 of each weight at most) for bf16, whose
+// outputs are rounded eight times as coarsely.  The second plane costs 28 % on 64 x 8192 cached tokens of 8
+// heads (148 us for 116).  Sums, maxima and the output stay in fp32.
 //
 // mma.m16n8k16 with the tokens (scores) or the channels (output) as the 16 rows and eight query rows as
 // the columns: S^T = K Q^T, O^T = V^T P^T.  One step of a conversation has as many query rows per
@@ -22,6 +22,8 @@
 // and head is split over `splits` blocks and the warps of each; partial results (numerator, sum,
 // maximum) are joined by kv4_join_kernel in a fixed order.
 #include <float.h>
+
+#include <type_traits>
 
 #include "kv4.cuh"
 
@@ -52,10 +54,10 @@ __device__ inline uint32_t transpose8(uint32_t v) {
   return r;
 }
 // Two channels of four codes out of a word: `even` the low halves of two bytes 16 bits apart, as n unit,
-// `odd` the high halves, as 16 n unit.  For 16-bit types unit is 2^-24 and the masked bits are the subnormal
+// `odd` the high halves, as 16 n unit.  For bf16 unit is 2^-24 and the masked bits are the subnormal
 // numbers; the even ones of the upper bytes come from a subtraction (exact), because logic instructions,
 // of half the rate of additions, are what this kernel has most of.  The tensor cores align the products
-// of subnormal numbers as if they had a leading bit, which leaves sums of them some 17 bits: fp32 takes
+// of subnormal numbers as if they had a leading bit, which leaves sums of them some 17 bits: fp16 and fp32 take
 // unit 1 (0x6400 | x is the number 1024 + x), and n - 8 for n, so that sums over tokens or channels do not
 // meet a large common part that the minima take out again (the accumulation truncates).
 __device__ inline uint32_t half_minus(uint32_t v, float c) {
@@ -96,8 +98,10 @@ constexpr int smem_bytes() {
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kThreads, NT > 1 || D > 128 ? 2 : kBlocksPerSm)
 kv4_attention_kernel(const Kv4Attention p) {
-  constexpr int P = sizeof(T) == 4 ? 2 : 1;       // fp16 planes of q and of the weights
-  constexpr float kUnit = P == 1 ? 0x1p-24f : 1.0f;  // what a code of 1 is to the tensor cores
+  constexpr int P = sizeof(T) == 4 ? 2 : 1;       // fp16 planes of q
+  constexpr bool kCoarse = std::is_same_v<T, __nv_bfloat16>;
+  constexpr int W = kCoarse ? 1 : 2;              // fp16 planes of the weights
+  constexpr float kUnit = kCoarse ? 0x1p-24f : 1.0f;  // what a code of 1 is to the tensor cores
   constexpr int R = 8 * NT;
   constexpr int KW = D / 32;                      // words of a key row that a thread holds
   constexpr int VW = D / 64;                      // words of a value row that a thread holds
@@ -284,11 +288,11 @@ kv4_attention_kernel(const Kv4Attention p) {
         for (int u = 0; u < kSub; ++u) {
           uint32_t e0, o0, e1, o1;
           if (h) {
-            codes_upper<P == 1>(kw[u][0][w], e0, o0);
-            codes_upper<P == 1>(kw[u][1][w], e1, o1);
+            codes_upper<kCoarse>(kw[u][0][w], e0, o0);
+            codes_upper<kCoarse>(kw[u][1][w], e1, o1);
           } else {
-            codes_lower<P == 1>(kw[u][0][w], e0, o0);
-            codes_lower<P == 1>(kw[u][1][w], e1, o1);
+            codes_lower<kCoarse>(kw[u][0][w], e0, o0);
+            codes_lower<kCoarse>(kw[u][1][w], e1, o1);
           }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
@@ -304,7 +308,7 @@ kv4_attention_kernel(const Kv4Attention p) {
       for (int e = 0; e < 2; ++e) {
         kf[u][e] = half_values(kp[u][e]);
         vf[u][e] = half_values(vp[u][e]);
-        if (P == 2) {                             // the minimum that belongs to n - 8
+        if (!kCoarse) {                           // the minimum that belongs to n - 8
           kf[u][e].y = fmaf(8.0f, kf[u][e].x, kf[u][e].y);
           vf[u][e].y = fmaf(8.0f, vf[u][e].x, vf[u][e].y);
         }
@@ -322,7 +326,7 @@ kv4_attention_kernel(const Kv4Attention p) {
     }
 
     // ---- softmax: scores in units of log2, reference = running maximum of score + exponent of s_v
-    uint32_t pw[P][kSub][NT][2];                  // weights times s_v, fp16 pairs
+    uint32_t pw[W][kSub][NT][2];                  // weights times s_v, fp16 pairs
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float top[2] = {-INFINITY, -INFINITY};
@@ -393,9 +397,9 @@ kv4_attention_kernel(const Kv4Attention p) {
           const float2 q = unpack2(mul2(w2, pack2(vx, vx1)));
           const uint32_t h = half_pair(q.x, q.y);
           pw[0][u][nt][e] = h;
-          if (P == 2) {
+          if (W == 2) {
             const float2 f = half_values(h);
-            pw[P - 1][u][nt][e] = half_pair(q.x - f.x, q.y - f.y);
+            pw[W - 1][u][nt][e] = half_pair(q.x - f.x, q.y - f.y);
           }
         }
     }
@@ -410,9 +414,9 @@ kv4_attention_kernel(const Kv4Attention p) {
           load_words<4 * VW>(v_lane + at * kRow + ((e & 1) + 8 * (e >> 1)) * kRow, vw[0][e]);
       }
       const auto& vu = vw[kAllValues ? u : 0];
-      uint32_t b0[P][NT], b1[P][NT];
+      uint32_t b0[W][NT], b1[W][NT];
 #pragma unroll
-      for (int pl = 0; pl < P; ++pl)
+      for (int pl = 0; pl < W; ++pl)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           b0[pl][nt] = transpose8(pw[pl][u][nt][0]);
@@ -428,16 +432,16 @@ kv4_attention_kernel(const Kv4Attention p) {
           for (int h2 = 0; h2 < 2; ++h2) {
             uint32_t e0, o0, e1, o1;
             if (h2) {
-              codes_upper<P == 1>(z0, e0, o0);
-              codes_upper<P == 1>(z1, e1, o1);
+              codes_upper<kCoarse>(z0, e0, o0);
+              codes_upper<kCoarse>(z1, e1, o1);
             } else {
-              codes_lower<P == 1>(z0, e0, o0);
-              codes_lower<P == 1>(z1, e1, o1);
+              codes_lower<kCoarse>(z0, e0, o0);
+              codes_lower<kCoarse>(z1, e1, o1);
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int pl = 0; pl < P; ++pl)
+              for (int pl = 0; pl < W; ++pl)
                 mma_f16(o[4 * w + 2 * h + h2][nt], e0, o0, e1, o1, b0[pl][nt], b1[pl][nt]);
           }
         }

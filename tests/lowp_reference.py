@@ -144,11 +144,12 @@ def attention(q, cache, table, lengths, scale, causal=True, window=0, sinks=0):
                 # a score: d exact products and the row's sum in fp32 (or q in 22 bits), scale and minimum
                 off = abs(scale) * (d + 16) * 2.0 ** -22 * (
                     ks_ * (rows.abs() @ kq_.t()) + km_.abs() * rows.abs().sum(-1, keepdim=True)).amax(-1)
-                # its weight: exp2 (2^-21) and, against the codes, one rounding to fp16 (22 bits for
-                # fp32); the sums over the tokens
+                # its weight: exp2 (2^-21) and, against the codes, one rounding to fp16 for bf16 (22 bits
+                # otherwise); the sums over the tokens
                 much = p @ (vs[sees, None] * vq[sees] + vm[sees, None].abs())
-                weight = 2.0 ** -20 + (2.0 ** -21 if dtype == torch.float32 else 2.0 ** -11)
-                if dtype != torch.float32 and n * group >= 64 and d <= 128:
+                many = dtype != torch.float32 and n * group >= 64 and d <= 128
+                weight = 2.0 ** -20 + (2.0 ** -11 if many or dtype == torch.bfloat16 else 2.0 ** -21)
+                if many:
                     # many rows: keys and values as fp16 numbers, one rounding (half a step, 2^-11) each, and
                     # weights that fp16's smallest step, 2^-24, may round by 2^-25 where 2^6 stands for 1
                     k = ks_[:, None] * kq_ + km_[:, None]
