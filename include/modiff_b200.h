@@ -642,7 +642,7 @@ int modiff_attention_i8(const int8_t* q_codes, const int8_t* k_codes, const int8
 #define MODIFF_BF16 2
 
 /* Linear layer in 8-bit floating point (e4m3), one fp32 scale per block of 128 channels:
- *   modiff_fp8_quantize     rows x [rows][k] -> codes [rows][code_pitch] (zeros from k to the pitch),
+ *   modiff_fp8_quantize     rows x [rows][k] -> codes [rows][code_pitch] (zeros from k to the next multiple of 16),
  *                           scale [ceil(k / 128)][scale_pitch >= rows, a multiple of 4] = max|x| * (1.0f / 448.0f) of the
  *                           block, 1 where that is 0; code = e4m3(x / scale).  code_pitch a multiple of 16
  *   modiff_fp8_pack_weight  w [n][k] -> codes [n][round_up(k, 16)], scale [ceil(n/128)][ceil(k/128)]

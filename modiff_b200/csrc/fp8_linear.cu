@@ -16,6 +16,7 @@ int read_device_status_fp8(int* status, int reset) { return read_status_this_uni
 namespace {
 
 constexpr int kBlock = kFp8Block;
+constexpr int kMostRows = 0x7fffff00;          // sizes are rounded up to tiles in 32 bits
 constexpr float kInvE4m3Max = 1.0f / 448.0f;   // the scale is a product with this fp32 number
 
 __device__ inline void tc_mma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
@@ -134,7 +135,7 @@ fp8_quantize_kernel(const QuantParams p) {
         codes[i] = e4m3_x4(__fdiv_rn(a.x, s), __fdiv_rn(a.y, s), __fdiv_rn(b.x, s), __fdiv_rn(b.y, s));
       }
     }
-    if (c0 < p.code_pitch)                       // the pitch is a multiple of 16
+    if (c0 < p.k)                                // up to the next multiple of 16, zeros from k on
       *reinterpret_cast<uint4*>(p.codes + (row0 + u) * p.code_pitch + c0) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
   }
   if (lane == 0 && live) {
@@ -535,6 +536,7 @@ int check_weight(const uint8_t* w, int64_t w_pitch, const float* w_scale, int64_
                  const void* y, int64_t y_pitch, int rows, int k, int n, int dtype) {
   MODIFF_CHECK_ARG(dtype_ok(dtype), "unknown element type %d", dtype);
   MODIFF_CHECK_ARG(rows >= 0 && k > 0 && n > 0, "bad shape");
+  MODIFF_CHECK_ARG(rows <= kMostRows && k <= kMostRows && n <= kMostRows, "more than %d rows or channels", kMostRows);
   if (rows == 0) return MODIFF_OK;
   const int size = dtype_bytes(dtype);
   MODIFF_CHECK_ARG(w && w_scale && y, "NULL pointer argument");
@@ -576,7 +578,7 @@ static int quantize_rows(const void* x, int64_t x_pitch, int64_t rows, int k, in
 extern "C" int modiff_fp8_quantize(const void* x, int64_t x_pitch, int64_t rows, int k, int dtype, uint8_t* codes,
                                    int64_t code_pitch, float* scale, int64_t scale_pitch, void* stream) {
   MODIFF_CHECK_ARG(dtype_ok(dtype), "unknown element type %d", dtype);
-  MODIFF_CHECK_ARG(rows >= 0 && k > 0, "bad shape");
+  MODIFF_CHECK_ARG(rows >= 0 && k > 0 && k <= kMostRows, "bad shape");
   if (rows == 0) return MODIFF_OK;
   MODIFF_CHECK_ARG(x && codes && scale, "NULL pointer argument");
   MODIFF_CHECK_ARG(code_pitch >= k && code_pitch % 16 == 0 && (uintptr_t)codes % 16 == 0,
@@ -590,7 +592,7 @@ extern "C" int modiff_fp8_quantize(const void* x, int64_t x_pitch, int64_t rows,
 extern "C" int modiff_fp8_pack_weight(const void* w, int64_t w_pitch, int n, int k, int dtype, uint8_t* codes,
                                       int64_t code_pitch, float* scale, int64_t scale_pitch, void* stream) {
   MODIFF_CHECK_ARG(dtype_ok(dtype), "unknown element type %d", dtype);
-  MODIFF_CHECK_ARG(n > 0 && k > 0, "bad shape");
+  MODIFF_CHECK_ARG(n > 0 && k > 0 && n <= kMostRows && k <= kMostRows, "bad shape");
   MODIFF_CHECK_ARG(w && codes && scale, "NULL pointer argument");
   MODIFF_CHECK_ARG(code_pitch >= k && code_pitch <= round_up(k, 16) && code_pitch % 16 == 0 && (uintptr_t)codes % 16 == 0,
                    "rows of codes need 16-byte alignment and the next multiple of 16 as pitch");
@@ -624,7 +626,7 @@ extern "C" int modiff_fp8_linear(const uint8_t* codes, int64_t code_pitch, const
 }
 
 extern "C" int64_t modiff_fp8_linear_bytes(int rows, int k, int n) {
-  if (rows <= 0 || k <= 0 || n <= 0 || fused_wanted(rows, k, n)) return 0;
+  if (rows <= 0 || k <= 0 || n <= 0 || rows > kMostRows || k > kMostRows || n > kMostRows || fused_wanted(rows, k, n)) return 0;
   return (int64_t)rows * round_up(k, 16) + 4ll * scale_row(rows) * ceil_div(k, kBlock);
 }
 

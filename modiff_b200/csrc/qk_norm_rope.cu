@@ -212,6 +212,7 @@ extern "C" int modiff_qk_norm_rope(const void* q, int64_t q_token, int64_t q_hea
   MODIFF_CHECK_ARG(k_heads == 0 || (k && k_out), "NULL pointer argument");
   MODIFF_CHECK_ARG(positions || rot == 0 || table_rows >= tokens, "tables of %lld rows for %lld tokens",
                    (long long)table_rows, (long long)tokens);
+  MODIFF_CHECK_ARG((uintptr_t)positions % (positions64 ? 8 : 4) == 0, "misaligned positions");
   if (tokens == 0 || q_heads + k_heads == 0) return MODIFF_OK;
 
   NormRopeParams p = {};

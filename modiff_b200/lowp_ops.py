@@ -158,7 +158,7 @@ def fp8_linear(x, w, w_scale, bias=None):
     if y.numel():
         kp = -(-k // 16) * 16
         rows = lead[0] if len(lead) == 1 else y.numel() // n
-        if rows > 0x7fffffff:
+        if rows > 0x7fffff00:
             raise ModiffError("fp8_linear: too many rows")
         _device("fp8_linear", src, x.scale)
         if x.scale.dtype != torch.float32 or tuple(x.scale.shape) != lead + (blocks,):
@@ -176,7 +176,7 @@ def fp8_linear(x, w, w_scale, bias=None):
 def _fp8_linear_rows(device, x, w, n, k, w_pitch, w_scale, blocks, bias, dt):
     """`fp8_linear` of a tensor: quantised inside the product, or into a workspace before it."""
     at, pitch, rows, _, keep = _rows("fp8_linear", x)
-    if rows > 0x7fffffff:
+    if rows > 0x7fffff00:
         raise ModiffError("fp8_linear: too many rows")
     y = keep.new_empty((rows, n))
     if rows:
@@ -317,7 +317,7 @@ def _cache(name, cache, table, lengths):
     """(the cache as the entry points take it, its heads and channels, table and lengths without gaps)"""
     kc, kp, vc, vp = cache
     shape, par = kc.shape, kp.shape
-    if (len(shape) != 4 or kc.dtype is not torch.uint8 or vc.dtype is not torch.uint8 or vc.shape != shape
+    if (len(shape) != 4 or shape[1] == 0 or kc.dtype is not torch.uint8 or vc.dtype is not torch.uint8 or vc.shape != shape
             or kp.dtype is not torch.float16 or vp.dtype is not torch.float16 or par != (*shape[:3], 2) or vp.shape != par
             or not (kc.is_contiguous() and vc.is_contiguous() and kp.is_contiguous() and vp.is_contiguous())):
         raise ModiffError(f"{name}: a cache is contiguous uint8 codes [pages, heads, page_size, d / 2] and fp16 "

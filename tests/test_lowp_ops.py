@@ -97,6 +97,25 @@ def test_entry_points_refuse_bad_arguments_without_a_device():
     assert lib.modiff_kv4_append(cache(), a, *s3, a, *s3, a, a, 1, 0, 1, 0, None) == 0
 
 
+def test_entry_points_refuse_sizes_beyond_their_index_types():
+    lib = _lib.lib()
+    a, most = 1 << 20, 0x7fffff00
+    s2, s3 = (64, 64), (64, 64, 64)
+    cache = C.byref(_lib.Kv4CacheStruct(a, a, a, a, 4, 1 << 20, 16, 64))
+    for rc in (lib.modiff_fp8_linear(a, 16, a, most + 4, a, 16, a, 1, None, a, 1, most + 1, 16, 1, 0, None),
+               lib.modiff_fp8_linear_x(a, 16, a, 16, a, 1, None, a, 1, most + 1, 16, 1, 0, a, None),
+               lib.modiff_fp8_quantize(a, 16, 1 << 40, 16, 0, a, 16, a, 1 << 40, None),
+               lib.modiff_fp8_quantize(a, 1 << 31, 1, most + 1, 0, a, 1 << 31, a, 4, None),
+               lib.modiff_kv4_append(cache, a, *s3, a, *s3, a, a, 64, 32, 1, 0, None),
+               lib.modiff_kv4_read(cache, a, a, 64, 32, 1, a, a, 0, None),
+               lib.modiff_qk_norm_rope(a, *s2, a, *s2, 1, None, *s2, None, *s2, 0, None, None, a, a, 8, a, 0, 1 << 31, 64, 64,
+                                       0, 1e-6, 0, None),
+               lib.modiff_qk_norm_rope(a, *s2, a, *s2, 1, None, *s2, None, *s2, 0, None, None, a, a, 8, a + 4, 1, 1, 64, 64,
+                                       0, 1e-6, 0, None)):
+        assert rc == 1 and lib.modiff_last_error()
+    assert lib.modiff_fp8_linear_bytes(most + 1, 16, 1) == 0
+
+
 @gpu
 def test_arguments_are_checked(cuda):
     x = torch.randn(4, 256, device=cuda)
@@ -353,6 +372,23 @@ def test_kv4_append_odd_inputs(cuda):
     bad_rows = torch.isnan(rk).any(-1)
     assert bool(torch.isnan(rk[0, 0, 0]).all()) and int(bad_rows.sum()) == 1
     assert ops.kv4_append(cache, k[:, :0], v[:, :0], table, lens) is None
+
+
+@gpu
+@pytest.mark.parametrize("k", [1, 100, 128, 300])
+def test_fp8_quantize_writes_nothing_beyond_its_rows(cuda, k):
+    """Codes as a part of wider rows: zeros up to the next multiple of 16, nothing behind that."""
+    rows, pitch, k16 = 5, 512, -(-k // 16) * 16
+    x = torch.randn(rows, k, generator=_gen(k)).to(cuda)
+    codes = torch.full((rows + 1, pitch), 0x55, dtype=torch.uint8, device=cuda)
+    scale = torch.full((-(-k // 128) + 1, 8), -1.0, device=cuda)
+    assert _lib.lib().modiff_fp8_quantize(x.data_ptr(), k, rows, k, 0, codes.data_ptr(), pitch, scale.data_ptr(), 8,
+                                          torch.cuda.current_stream().cuda_stream) == 0
+    want = ops.fp8_quantize(x)
+    assert torch.equal(codes[:rows, :k], want.codes.view(torch.uint8))
+    assert torch.equal(scale[:-1, :rows].t(), want.scale)
+    assert not codes[:rows, k:k16].any() and (codes[:rows, k16:] == 0x55).all() and (codes[rows] == 0x55).all()
+    assert (scale[-1] == -1).all()
 
 
 # ------------------------------------------------------------------------------ cached attention
