@@ -19,6 +19,8 @@
 //
 // Bound: tensor pipe (2048 cycles a tile of 128 keys and 256 rows of 128 channels); the loaders need about
 // 500 issue slots of a scheduler for it, the softmax about 1000.
+#include <type_traits>
+
 #include "kv4.cuh"
 #include "tc_common.cuh"
 
@@ -460,17 +462,21 @@ kv4_attention_tc_kernel(const Kv4Attention p) {
         const float ref = m_ref == -INFINITY ? 0.0f : kRoom - m_ref;
         const uint64_t ref2 = pack2(ref, ref);
         uint32_t w[kHalf / 2];
+        auto weigh = [&](auto all) {
 #pragma unroll
-        for (int j = 0; j < kHalf; j += 2) {
-          float2 a = unpack2(fma2(pack2(__int_as_float(v[j]), __int_as_float(v[j + 1])), ra2, ref2));
-          if (!whole) {                                        // 0 * inf where the scale is 0
-            if (v[j] == __float_as_int(-INFINITY)) a.x = -INFINITY;
-            if (v[j + 1] == __float_as_int(-INFINITY)) a.y = -INFINITY;
+          for (int j = 0; j < kHalf; j += 2) {
+            float2 a = unpack2(fma2(pack2(__int_as_float(v[j]), __int_as_float(v[j + 1])), ra2, ref2));
+            if (!decltype(all)::value) {                       // 0 * inf where the scale is 0
+              if (v[j] == __float_as_int(-INFINITY)) a.x = -INFINITY;
+              if (v[j + 1] == __float_as_int(-INFINITY)) a.y = -INFINITY;
+            }
+            const float2 e = make_float2(exp2_fast(a.x), exp2_fast(a.y));
+            l2 = add2(l2, pack2(e.x, e.y));
+            w[j / 2] = half_pair(e.x, e.y);
           }
-          const float2 e = make_float2(exp2_fast(a.x), exp2_fast(a.y));
-          l2 = add2(l2, pack2(e.x, e.y));
-          w[j / 2] = half_pair(e.x, e.y);
-        }
+        };
+        if (whole) weigh(std::true_type());
+        else weigh(std::false_type());
         tc_st16(t_sh, reinterpret_cast<uint32_t(&)[16]>(w[0]));
         tc_st16(t_sh + 16, reinterpret_cast<uint32_t(&)[16]>(w[16]));
         tc_wait_st();
