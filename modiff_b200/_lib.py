@@ -5,6 +5,7 @@ wrapper raises `ModiffError` when an entry point returns a non-zero status.
 """
 import ctypes as C
 import os
+import struct
 
 import torch
 
@@ -64,7 +65,8 @@ class Kv4CacheStruct(C.Structure):
 
 _P = C.c_void_p
 _G = C.POINTER(ConvGeom)
-_KV4 = C.POINTER(Kv4CacheStruct)
+_KV4 = C.c_void_p               # a Kv4CacheStruct by reference, or its bytes (KV4_PACK: a third of the time)
+KV4_PACK = struct.Struct("4Q4i").pack
 
 # name -> (restype, argtypes); one entry per declaration of include/modiff_b200.h
 SIGNATURES = {

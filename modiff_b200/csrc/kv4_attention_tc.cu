@@ -10,8 +10,8 @@
 //   one warp issues S = Q K^T into tensor memory (128 columns a group) and O += P V, with P read from
 //   tensor memory, where the softmax has put it in place of S;
 //   four softmax warps a group, a thread per row, no exchange between threads: maximum, then weights.
-//   O is rescaled only when a row's maximum has grown by more than 2^8; weights are fp16 in units of
-//   2^(reference - 6), at most 2^14.
+//   O is rescaled only when a row's maximum has grown by more than 2^10; weights are fp16 in units of
+//   2^(reference - 5), at most 2^15.
 // While one group's softmax runs the tensor pipe works for the other.
 //
 // Queries are brought to fp16 by a power of two per row (exact for bf16).  A value that is not finite is
@@ -40,8 +40,8 @@ constexpr int kThreads = 32 * 20;           // the last three warps only complet
 constexpr int kRegsAtLaunch = 96, kRegsLoad = 72, kRegsSoftmax = 136, kRegsMma = 56;
 static_assert(5 * kRegsAtLaunch >= 2 * kRegsLoad + 2 * kRegsSoftmax + kRegsMma, "register split");
 constexpr int kChunk = kKeys * 128;         // bytes of 128 rows of 64 channels
-constexpr float kGrowth = 8.0f;             // of a row's maximum, in powers of two, before O is rescaled
-constexpr float kRoom = 6.0f;               // weights are at most 2^(kGrowth + kRoom)
+constexpr float kGrowth = 10.0f;            // of a row's maximum, in powers of two, before O is rescaled
+constexpr float kRoom = 5.0f;               // weights are at most 2^(kGrowth + kRoom)
 constexpr int kBitSlots = 4;
 
 // fp16 x fp16 -> fp32; descriptors as low words and the high word they share.  A from shared or tensor memory.
@@ -412,35 +412,46 @@ kv4_attention_tc_kernel(const Kv4Attention p) {
         bool whole = (there.x & there.y) == 0xffffffffu && (bad.x | bad.y) == 0;
         if (p.causal) whole &= t0 + kHalf <= pos_lo + 1;
         if (p.window > 0) whole &= t0 > pos_hi - p.window || t0 + kHalf <= p.sinks;
-        tc_wait_ld();
+        // the keys that this row sees, one bit each; where that is not all of them the scores are left as they
+        // are and passed over below
+        whole = __all_sync(0xffffffffu, whole) != 0;
+        uint32_t vis[2] = {0xffffffffu, 0xffffffffu};
         if (!whole) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             const int tb = t0 + 32 * c;
-            uint32_t vis = c ? there.y : there.x;
-            if (p.causal) vis &= low_bits(pos - tb + 1);
-            if (p.window > 0) vis &= ~low_bits(pos - p.window + 1 - tb) | low_bits(p.sinks - tb);
-            poisoned |= (vis & (c ? bad.y : bad.x)) != 0;
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (!(vis >> j & 1u)) v[32 * c + j] = __float_as_int(-INFINITY);
+            vis[c] = c ? there.y : there.x;
+            if (p.causal) vis[c] &= low_bits(pos - tb + 1);
+            if (p.window > 0) vis[c] &= ~low_bits(pos - p.window + 1 - tb) | low_bits(p.sinks - tb);
+            poisoned |= (vis[c] & (c ? bad.y : bad.x)) != 0;
           }
         }
-        float top = max3(__int_as_float(v[0]), __int_as_float(v[1]), -INFINITY);
-        float top2 = max3(__int_as_float(v[2]), __int_as_float(v[3]), -INFINITY);
+        tc_wait_ld();
+        float top, top2;
+        auto largest = [&](auto all) {
+          auto score = [&](int j) {
+            return decltype(all)::value || (vis[j >> 5] >> (j & 31) & 1u) ? __int_as_float(v[j]) : -INFINITY;
+          };
+          top = max3(score(0), score(1), -INFINITY);
+          top2 = max3(score(2), score(3), -INFINITY);
 #pragma unroll
-        for (int j = 4; j < kHalf; j += 4) {
-          top = max3(__int_as_float(v[j]), __int_as_float(v[j + 1]), top);
-          top2 = max3(__int_as_float(v[j + 2]), __int_as_float(v[j + 3]), top2);
-        }
+          for (int j = 4; j < kHalf; j += 4) {
+            top = max3(score(j), score(j + 1), top);
+            top2 = max3(score(j + 2), score(j + 3), top2);
+          }
+        };
+        if (whole) largest(std::true_type());
+        else largest(std::false_type());
         top = fmaxf(top, top2);
         const float m_new = top == -INFINITY ? -INFINITY : top * ra;
         const bool grow = m_new > m_ref + kGrowth || (m_ref == -INFINITY && m_new > -INFINITY);
         if (__any_sync(0xffffffffu, grow)) {
-          const float alpha = grow ? exp2_fast(m_ref - m_new) : 1.0f;       // 0 while nothing was seen
+          // nothing was seen before: nothing to rescale, the sum and O are 0
+          const bool rescale = grow && m_ref > -INFINITY;
+          const float alpha = rescale ? exp2_fast(m_ref - m_new) : 1.0f;
           if (grow) m_ref = m_new;
           l2 = mul2(l2, pack2(alpha, alpha));
-          if (step > 0) {
+          if (__any_sync(0xffffffffu, rescale)) {
             // O may be rewritten once the products of the step before are in it; those of two steps before
             // are, this step's scores were multiplied behind them
             ok = mbar_wait(smem_u32(&bar_pv[g][h ^ 1]), (uint32_t)((step - 1) >> 1) & 1u, abort_flag);
@@ -466,9 +477,9 @@ kv4_attention_tc_kernel(const Kv4Attention p) {
 #pragma unroll
           for (int j = 0; j < kHalf; j += 2) {
             float2 a = unpack2(fma2(pack2(__int_as_float(v[j]), __int_as_float(v[j + 1])), ra2, ref2));
-            if (!decltype(all)::value) {                       // 0 * inf where the scale is 0
-              if (v[j] == __float_as_int(-INFINITY)) a.x = -INFINITY;
-              if (v[j + 1] == __float_as_int(-INFINITY)) a.y = -INFINITY;
+            if (!decltype(all)::value) {
+              if (!(vis[j >> 5] >> (j & 31) & 1u)) a.x = -INFINITY;
+              if (!(vis[j >> 5] >> (j & 31) & 2u)) a.y = -INFINITY;
             }
             const float2 e = make_float2(exp2_fast(a.x), exp2_fast(a.y));
             l2 = add2(l2, pack2(e.x, e.y));

@@ -6,7 +6,6 @@ Tensors are CUDA tensors of fp32, fp16 or bf16, all of a call on one device; a c
 device's current stream.  Sums, statistics and softmax are fp32, the result is rounded once.  There is no
 backward pass: inputs that ask for gradients are refused while gradients are recorded.
 """
-import ctypes as C
 from typing import NamedTuple
 
 import torch
@@ -19,7 +18,8 @@ _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
 _Tensor, _grad_enabled = torch.Tensor, torch.is_grad_enabled
-_stream = torch._C._cuda_getCurrentRawStream       # what torch.cuda.current_stream(device).cuda_stream wraps
+# what torch.cuda.current_stream(device).cuda_stream and torch.cuda.current_device() wrap
+_stream, _current = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
 def _device(name, *tensors):
@@ -52,11 +52,11 @@ def _dtype(name, x):
 def _call(device, entry, *args, nbytes=0, nops=0, more=0):
     """One entry point on `device`'s current stream, whatever the current device is; `more` kernels
     beyond its first."""
-    if device != torch.cuda.current_device():
+    if device == _current():
+        _lib.call(entry, *args, _stream(device), nbytes=nbytes, nops=nops)
+    else:
         with torch.cuda.device(device):
             _lib.call(entry, *args, _stream(device), nbytes=nbytes, nops=nops)
-    else:
-        _lib.call(entry, *args, _stream(device), nbytes=nbytes, nops=nops)
     _lib.LAUNCHES[0] += more
 
 
@@ -91,9 +91,9 @@ def fp8_quantize(x):
     at, pitch, rows, k, keep = _rows("fp8_quantize", x)
     blocks, kp = -(-k // FP8_BLOCK), -(-k // 16) * 16
     lead = tuple(x.shape[:-1])
-    codes = torch.empty(lead + (kp,), dtype=torch.float8_e4m3fn, device=x.device)
+    codes = x.new_empty(lead + (kp,), dtype=torch.float8_e4m3fn)
     row4 = -(-rows // 4) * 4
-    scale = torch.empty((blocks, row4), dtype=torch.float32, device=x.device)
+    scale = x.new_empty((blocks, row4), dtype=torch.float32)
     if rows:
         _call(device, 'modiff_fp8_quantize', at, pitch, rows, k, dt, codes.data_ptr(), kp, scale.data_ptr(), row4,
               nbytes=rows * (k * x.element_size() + kp + 4 * blocks))
@@ -328,8 +328,8 @@ def _cache(name, cache, table, lengths):
         raise ModiffError(f"{name}: int32 table [batch, pages] and lengths [batch], got {tuple(table.shape)} "
                           f"{table.dtype} and {tuple(lengths.shape)} {lengths.dtype}")
     pages, heads, size, half = shape
-    return (C.byref(_lib.Kv4CacheStruct(kc.data_ptr(), vc.data_ptr(), kp.data_ptr(), vp.data_ptr(), pages, heads, size,
-                                        2 * half)), heads, 2 * half, table.contiguous(), lengths.contiguous())
+    return (_lib.KV4_PACK(kc.data_ptr(), vc.data_ptr(), kp.data_ptr(), vp.data_ptr(), pages, heads, size, 2 * half),
+            heads, 2 * half, table.contiguous(), lengths.contiguous())
 
 
 def kv4_append(cache, k, v, table, lengths):
@@ -369,7 +369,7 @@ def kv4_read(cache, table, lengths, n, dtype=torch.float32):
     if dtype not in _DTYPES or n < 0:
         raise ModiffError(f"{name}: n >= 0 tokens as fp32, fp16 or bf16, got {n} and {dtype}")
     b, per = table.shape
-    k = torch.empty((b, n, heads, dim), dtype=dtype, device=table.device)
+    k = table.new_empty((b, n, heads, dim), dtype=dtype)
     v = torch.empty_like(k)
     rows = b * n * heads
     if rows:
@@ -407,7 +407,7 @@ def kv4_attention(q, cache, table, lengths, scale=None, causal=True, window=0, s
     if b * n:
         window, sinks = min(window, 1 << 30), min(sinks, 1 << 30)
         size = _lib.lib().modiff_kv4_attention_bytes(c, b, n, heads, per, window, sinks, dt)
-        work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+        work = q.new_empty(size, dtype=torch.uint8) if size else None
         _call(device, 'modiff_kv4_attention', q.data_ptr(), *q.stride()[:3], c, table.data_ptr(), lengths.data_ptr(),
               out.data_ptr(), b, n, heads, per, dim ** -0.5 if scale is None else scale, 1 if causal else 0, window,
               sinks, dt, None if work is None else work.data_ptr(), more=int(size > 0))

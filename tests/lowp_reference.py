@@ -151,12 +151,12 @@ def attention(q, cache, table, lengths, scale, causal=True, window=0, sinks=0):
                 weight = 2.0 ** -20 + (2.0 ** -11 if many or dtype == torch.bfloat16 else 2.0 ** -21)
                 if many:
                     # many rows: keys and values as fp16 numbers, one rounding (half a step, 2^-11) each, and
-                    # weights that fp16's smallest step, 2^-24, may round by 2^-25 where 2^6 stands for 1
+                    # weights that fp16's smallest step, 2^-24, may round by 2^-25 where 2^5 stands for 1
                     k = ks_[:, None] * kq_ + km_[:, None]
                     off = off + abs(scale) * 2.0 ** -11 * (rows.abs() @ k.abs().t()).amax(-1)
                     much = torch.maximum(much, p @ v.abs())
                     weight = weight + 2.0 ** -11
-                    tol[i, r, h * group:(h + 1) * group] = len(k) * 2.0 ** -31 * v.abs().amax(0)
+                    tol[i, r, h * group:(h + 1) * group] = len(k) * 2.0 ** -30 * v.abs().amax(0)
                 err = (2 * off + weight + (len(p[0]) + 8) * 2.0 ** -23)[:, None] * much
                 tol[i, r, h * group:(h + 1) * group] += err + (p @ v).abs() * half_step(dtype)
     # what fp16 cannot hold: outputs below its normal range
