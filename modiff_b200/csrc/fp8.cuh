@@ -29,7 +29,7 @@ struct Fp8Params {
 };
 
 // Kernel for many rows (fp8_linear_pair.cu)
-bool fp8_pair_wanted(int rows, int k, int n);
+bool fp8_pair_wanted(int rows, int n);
 int fp8_launch_pair(const Fp8Operands& o, const Fp8Params& p, int dtype, cudaStream_t s);
 
 namespace {

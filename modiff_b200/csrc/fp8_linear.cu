@@ -472,20 +472,30 @@ fp8_linear_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_c
   }
 }
 
-// Channels split over up to eight CTAs while the grid leaves SMs idle and every CTA keeps two blocks
+// Channels split over up to eight CTAs of a cluster.  Of tiles of 128 tokens an SM holds one: all of them run at
+// once (a second round costs more than the split gains: 128 x 8192 x 8192, us for 1 : 2 : 4 parts, 37.6 : 23.6 :
+// 27.8), and clusters of eight, of which fewer fit, leave a third of the SMs free (96 x 2048 x 2048, 4 : 8 parts,
+// 7.9 : 13.0).  Narrower tiles share an SM: split while the grid leaves SMs idle and every CTA keeps two blocks
+// (64 x 8192 x 8192, 2 : 4 : 8 parts, 18.7 : 14.9 : 22.1).
 int rows_split(int rows, int n, int kb, int tn) {
   const int64_t tiles = (int64_t)ceil_div(n, 128) * ceil_div(rows, tn);
+  const int sms = device_sms();
   int split = 1;
-  while (split < 8 && tiles * split < device_sms() && kb >= 4 * split) split *= 2;
+  if (tn >= 128)
+    while (split < 8 && 2 * split * tiles <= (split == 4 ? 2 * sms / 3 : sms) && kb >= 2 * split) split *= 2;
+  else
+    while (split < 8 && tiles * split < sms && kb >= 4 * split) split *= 2;
   return split;
 }
 
-// Rows few enough to be quantised by the CTAs that multiply them: every CTA of a column of tiles repeats
-// that work, so it has to stay small beside the CTA's weights.
+// Rows few enough to be quantised by the CTAs that multiply them, in one launch: every CTA of a column of tiles
+// repeats that work.  Device time against two kernels (us): 1 x 4096 x 4096 (8 row blocks a CTA) 7.4 : 7.9, 1 x
+// 8192 x 8192 (16) 13.4 : 12.5, 8 x 1024 x 4096 (16) 8.2 : 6.6, 2 x 8192 x 8192 (32) 16.4 : 12.1; the second
+// launch and its workspace cost the host about 5 us.
 bool fused_wanted(int rows, int k, int n) {
   const int kb = ceil_div(k, kBlock);
   const int blocks = ceil_div(kb, rows_split(rows, n, kb, kFusedRows));
-  return rows <= kFusedRows && blocks <= kFusedBlocks && rows * blocks <= 64;
+  return rows <= kFusedRows && blocks <= kFusedBlocks && rows * blocks <= 16;
 }
 
 template <typename T, int TN, bool FUSED>
@@ -522,7 +532,7 @@ int launch_rows(const Fp8Operands& o, Fp8Params p, cudaStream_t s) {
 }
 
 int launch_linear(const Fp8Operands& o, const Fp8Params& p, int dtype, cudaStream_t s) {
-  if (fp8_pair_wanted(p.rows, o.k, p.n)) return fp8_launch_pair(o, p, dtype, s);
+  if (fp8_pair_wanted(p.rows, p.n)) return fp8_launch_pair(o, p, dtype, s);
   return with_dtype(dtype, [&](auto tag) {
     using T = decltype(tag);
     if (p.rows <= 16) return launch_rows<T, 16, false>(o, p, s);

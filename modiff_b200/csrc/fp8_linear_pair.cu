@@ -384,9 +384,12 @@ int launch(const Fp8Operands& o, const Fp8Params& p, cudaStream_t s) {
 
 }  // namespace
 
-bool fp8_pair_wanted(int rows, int k, int n) {
-  (void)k;
-  return (int64_t)ceil_div(rows, kTile) * ceil_div(n, kTile) >= device_sms() / 4;
+// Above 64 rows, once tiles of 128 x 128 fill more than half of the SMs: below that the other kernel splits the
+// channels (us, this kernel : that one; 256 x 4096 x 4096 19.2 : 15.4, 1000 x 8192 x 1000 31.8 : 23.8), above it
+// cannot (200 x 8192 x 8192 32.5 : 42.6, 4096 x 512 x 512 7.8 : 8.9).  Up to 64 rows that one's narrow tiles are
+// faster whatever the weights' size is (64 x 5120 x 25600 41.7 : 28.3, 8 x 1024 x 40000 19.1 : 8.5).
+bool fp8_pair_wanted(int rows, int n) {
+  return rows > 64 && 2 * (int64_t)ceil_div(rows, 128) * ceil_div(n, 128) > device_sms();
 }
 
 int fp8_launch_pair(const Fp8Operands& o, const Fp8Params& p, int dtype, cudaStream_t s) {
