@@ -89,21 +89,45 @@ fp8_quantize_kernel(const QuantParams p) {
   const int c0 = blk * kBlock + 16 * lane;
   const bool live = blk < p.blocks && row0 < p.rows;
   uint32_t w[kRows][kWords];
+  if constexpr (VEC) {
 #pragma unroll
-  for (int u = 0; u < kRows; ++u) {
-    const T* src = static_cast<const T*>(p.x) + (row0 + u) * p.x_pitch + c0;
-    const bool here = live && row0 + u < p.rows && c0 < p.k;
-    if (VEC && here && c0 + 16 <= p.k) {
+    for (int u = 0; u < kRows; ++u) {
+      const T* src = static_cast<const T*>(p.x) + (row0 + u) * p.x_pitch + c0;
+      const bool here = live && row0 + u < p.rows && c0 < p.k;
+      if (here && c0 + 16 <= p.k) {
+#pragma unroll
+        for (int i = 0; i < kWords / 4; ++i) {
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + i);
+          w[u][4 * i] = v.x; w[u][4 * i + 1] = v.y; w[u][4 * i + 2] = v.z; w[u][4 * i + 3] = v.w;
+        }
+      } else {
+        T* t = reinterpret_cast<T*>(w[u]);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) t[e] = here && c0 + e < p.k ? src[e] : from_f32<T>(0.0f);
+      }
+    }
+  } else {
+    // rows that do not start on 16 bytes: neighbouring lanes load neighbouring elements, shared memory deals
+    // them out (the layer 13578 x 1660 -> 135, bf16: 62 us with every lane at its own 16, 33 so)
+    __shared__ __align__(16) T staged[8][kRows][4 * kBlock];
+    T(&mine)[kRows][4 * kBlock] = staged[threadIdx.x >> 5];
+    const int w0 = group * 4 * kBlock + (threadIdx.x & 31);
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+      const T* src = static_cast<const T*>(p.x) + (row0 + u) * p.x_pitch;
+      const bool here = row0 + u < p.rows;
+#pragma unroll
+      for (int i = 0; i < 4 * kBlock / 32; ++i)
+        mine[u][32 * i + (threadIdx.x & 31)] = here && w0 + 32 * i < p.k ? src[w0 + 32 * i] : from_f32<T>(0.0f);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int u = 0; u < kRows; ++u)
 #pragma unroll
       for (int i = 0; i < kWords / 4; ++i) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + i);
+        const uint4 v = *reinterpret_cast<const uint4*>(&mine[u][16 * (threadIdx.x & 31) + i * (16 / sizeof(T))]);
         w[u][4 * i] = v.x; w[u][4 * i + 1] = v.y; w[u][4 * i + 2] = v.z; w[u][4 * i + 3] = v.w;
       }
-    } else {
-      T* t = reinterpret_cast<T*>(w[u]);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) t[e] = here && c0 + e < p.k ? src[e] : from_f32<T>(0.0f);
-    }
   }
   float scale[kRows];
 #pragma unroll

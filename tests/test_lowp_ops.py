@@ -205,7 +205,8 @@ def test_fp8_pack_weight_bits(cuda, n, k, dtype):
 @pytest.mark.parametrize("rows,k,n", [
     (1, 1, 1), (1, 16, 8), (2, 128, 128), (15, 77, 130), (16, 1280, 640), (17, 300, 33), (31, 2001, 129),
     (64, 5120, 320), (65, 640, 1280), (100, 33, 7), (154, 768, 640), (129, 129, 257), (257, 1000, 520),
-    (1000, 320, 2560), (2500, 1411, 1030), (4096, 640, 768)])
+    (1000, 320, 2560), (2500, 1411, 1030), (4096, 640, 768), (1300, 129, 1001), (65, 136, 20000), (64, 256, 9600),
+    (512, 1000, 1000), (70, 4200, 2049), (8, 2048, 130)])
 def test_fp8_linear(cuda, rows, k, n, dtype):
     g = _gen(rows + 3 * k + 7 * n)
     x = (torch.randn(rows, k, generator=g) * torch.randn(1, k, generator=g).exp()).to(dtype)
@@ -221,6 +222,24 @@ def test_fp8_linear(cuda, rows, k, n, dtype):
     again = ops.fp8_linear(x.to(cuda), codes, scale)
     assert torch.equal(got, again)                         # no order that changes from call to call
     assert _lib.device_status() == 0
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("pitch", [1001, 1002, 1004, 1016])
+@pytest.mark.parametrize("rows", [3, 100, 1300])
+def test_fp8_linear_writes_nothing_beside_its_rows(cuda, rows, pitch, dtype):
+    """Results as a part of wider rows, on every alignment that a row can start on."""
+    k, n = 200, 1001
+    x = torch.randn(rows, k, generator=_gen(rows)).to(cuda, dtype)
+    w, s = ops.fp8_pack_weight(torch.randn(n, k, generator=_gen(1)).to(cuda))
+    y = torch.full((rows + 1, pitch), 7.0, dtype=dtype, device=cuda)
+    q = ops.fp8_quantize(x)
+    assert _lib.lib().modiff_fp8_linear(
+        q.codes.data_ptr(), 208, q.scale.data_ptr(), -(-rows // 4) * 4, w.data_ptr(), 208, s.data_ptr(), 2, None,
+        y.data_ptr(), pitch, rows, k, n, TYPES.index(dtype), torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(y[:rows, :n], ops.fp8_linear(q, w, s))
+    assert (y[:rows, n:] == 7).all() and (y[rows] == 7).all()
 
 
 @gpu
