@@ -569,7 +569,14 @@ int launch(const Kv4Attention& p, cudaStream_t s) {
 
 }  // namespace
 
-bool kv4_tc_wanted(int rows, int dim, int dtype) { return dtype != MODIFF_FP32 && dim <= 128 && rows >= 64; }
+// From 17 rows per key head on (bf16, us, kv4_attention.cu : this kernel; 4 sequences of up to 8000 tokens, 8 key
+// heads: 16 rows 31 : 45, 24 rows 57 : 45, 48 rows 84 : 47; 61 prompts of 39 tokens 114 : 48).  In fp16 from 64:
+// keys, values and weights are rounded to fp16 here, once each, which leaves outputs off by 4 - 7e-4, two or three
+// times their own rounding, and the other kernel's are as exact as that (24 rows 53 : 38, 64 rows about 85 : 38).
+// An exact split of all three would double this kernel's products.
+bool kv4_tc_wanted(int rows, int dim, int dtype) {
+  return dtype != MODIFF_FP32 && dim <= 128 && rows > (dtype == MODIFF_BF16 ? 16 : 63);
+}
 int kv4_tc_rows() { return kRows; }
 
 int kv4_launch_tc(const Kv4Attention& p, int dtype, cudaStream_t s) {
