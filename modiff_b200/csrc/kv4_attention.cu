@@ -576,12 +576,16 @@ kv4_join_kernel(const float* __restrict__ part, T* __restrict__ out, int64_t row
 }
 
 // Parts of the tokens of one sequence and key head: one round of blocks over all SMs if there are few of
-// them, else several, so that sequences of other lengths even out; every part at least `least` tokens.  The
-// lengths are on the device, so the table's width stands for the longest.
+// them, else two, so that sequences of other lengths even out (64 sequences of up to 8192 tokens, us for 1 : 2 :
+// 3 : 4 rounds, 117 : 113 : 116 : 120; 200 of 2000 88 : 87 : 109 : 108).  Every part at least `least` tokens: a
+// tile for every warp (2000 tokens of 8 heads, 128 : 512 tokens a part, 7.4 : 10.4; 131072 of 4 heads 27.2 :
+// 27.2), two tiles of the many-row kernel (100 queries, 4000 tokens, 256 : 1024, 33 : 49); fewer than four parts
+// are not worth the second launch (200 tokens 7.2 split, 6.9 not).  The lengths are on the device, so the table's
+// width stands for the longest.
 int splits_for(int64_t units, int max_tokens, int per_sm, int least) {
   const int64_t slots = (int64_t)per_sm * device_sms();
-  const int64_t want = 2 * units <= slots ? slots / units : ceil_div64(3 * slots, units);
-  const int64_t most = max_tokens / least;
+  const int64_t want = 2 * units <= slots ? slots / units : ceil_div64(2 * slots, units);
+  const int64_t most = max_tokens < 4 * least ? 1 : max_tokens / least;
   const int64_t s = want < most ? want : most;
   return (int)(s < 1 ? 1 : (s > kMaxSplits ? kMaxSplits : s));
 }
@@ -604,7 +608,7 @@ Plan plan_of(const modiff_kv4_cache* c, int batch, int count, int heads, int max
   const int64_t units = (int64_t)batch * c->heads * pl.row_tiles;
   int64_t tokens = (int64_t)max_pages * c->page_size;
   if (window > 0 && (int64_t)window + sinks + tile < tokens) tokens = (int64_t)window + sinks + tile;
-  pl.splits = splits_for(units, (int)tokens, pl.tc ? 1 : kBlocksPerSm, pl.tc ? 1024 : 4 * kTile * kWarps);
+  pl.splits = splits_for(units, (int)tokens, pl.tc ? 1 : kBlocksPerSm, pl.tc ? 256 : kTile * kWarps);
   pl.blocks = units * pl.splits;
   return pl;
 }
