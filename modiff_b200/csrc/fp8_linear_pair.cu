@@ -12,10 +12,10 @@
 //
 // Bound: the epilogue warps, about 1000 cycles per block of which the tensor pipe works 512: 256 go to the
 // additions, the rest to waits and tensor-memory loads one after the other.  16384 x 5120 -> 5120, codes
-// to bf16: 389 us, 2.2 PFLOP/s.  What it took: cluster-scope release / acquire on the barriers between the
+// to bf16: 376 us, 2.3 PFLOP/s.  What it took: cluster-scope release / acquire on the barriers between the
 // two CTAs 1001 us, default scope 430 (nothing but tensor memory passes through them, which tcgen05's own
 // fences order); scales through shared memory, bulk store 407; eight warps of 128 columns with 224
-// registers, loads and additions overlapped 389.  Not better: sixteen warps of 64 columns (407), four
+// registers, loads and additions overlapped 389, with the present ring and register split 376.  Not better: sixteen warps of 64 columns (407), four
 // buffers of 128 columns (442), one CTA per 128 x 256 tile (410).
 #include "fp8.cuh"
 
@@ -408,9 +408,9 @@ int launch(const Fp8Operands& o, const Fp8Params& p, cudaStream_t s) {
 }  // namespace
 
 // Above 64 rows, once tiles of 128 x 128 fill more than half of the SMs: below that the other kernel splits the
-// channels (us, this kernel : that one; 256 x 4096 x 4096 19.2 : 15.4, 1000 x 8192 x 1000 31.8 : 23.8), above it
-// cannot (200 x 8192 x 8192 32.5 : 42.6, 4096 x 512 x 512 7.8 : 8.9).  Up to 64 rows that one's narrow tiles are
-// faster whatever the weights' size is (64 x 5120 x 25600 41.7 : 28.3, 8 x 1024 x 40000 19.1 : 8.5).
+// channels (us, this kernel : that one; 256 x 4096 x 4096 19.2 : 15.7, 1000 x 8192 x 1000 32.0 : 23.8), above it
+// cannot as much (200 x 8192 x 8192 33.1 : 38.0, 4096 x 512 x 512 7.9 : 8.1).  Up to 64 rows that one's narrow tiles
+// are faster whatever the weights' size is (64 x 5120 x 25600 41.7 : 28.3, 8 x 1024 x 40000 19.1 : 8.5).
 bool fp8_pair_wanted(int rows, int n) {
   return rows > 64 && 2 * (int64_t)ceil_div(rows, 128) * ceil_div(n, 128) > device_sms();
 }

@@ -17,10 +17,14 @@
 // key head as query heads share it, mostly 1 to 8, which fills the narrow side.  All operands come
 // straight from global memory into the registers of the thread that multiplies them: which channel is
 // which column of an MMA is free as long as both operands agree, so a thread takes consecutive bytes.
+// More rows are more blocks, next to each other, which meet the codes in L2 (16 rows over 64 x 8192 tokens,
+// bf16: 212 us, as two groups of eight in one block 291).
 //
-// Bound: HBM (d + 8 bytes per cached token and head) for single tokens.  The cache of one sequence
-// and head is split over `splits` blocks and the warps of each; partial results (numerator, sum,
-// maximum) are joined by kv4_join_kernel in a fixed order.
+// Bound: instruction issue (22 instructions of a warp per 32 tokens' worth of a token and head), then HBM (d + 8
+// bytes per cached token and head).  64 sequences of up to 8192 tokens, 8 key heads of 128, bf16: 113 us, 3.8 TB/s;
+// one of 131072, 4 heads: 27 us.  The cache of one sequence and head is split over `splits` blocks and the warps of
+// each; partial results (numerator, sum, maximum) are joined by kv4_join_kernel in a fixed order.  Not better: tiles
+// of 64 tokens, five blocks an SM.
 #include <float.h>
 
 #include <type_traits>
@@ -32,6 +36,7 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
+constexpr int kQueries = 8;               // query rows of a block
 constexpr int kTile = 32;                 // tokens a warp takes at a time
 constexpr int kSub = kTile / 16;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -85,27 +90,27 @@ __device__ inline void codes_upper(uint32_t w, uint32_t& even, uint32_t& odd) {
   }
 }
 
-template <typename T, int D, int NT>
+template <typename T, int D>
 constexpr int smem_bytes() {
   constexpr int planes = sizeof(T) == 4 ? 2 : 1;
-  const int q = NT * (D / 16) * 32 * 8 * planes;               // query fragments
-  const int o = kWarps * NT * 8 * (D + 4) * 4;                 // the warps' outputs, joined at the end
+  const int q = (D / 16) * 32 * 8 * planes;               // query fragments
+  const int o = kWarps * kQueries * (D + 4) * 4;                 // the warps' outputs, joined at the end
   return q > o ? q : o;
 }
 
-// One block: 8 * NT query rows (query, head of the group) of one sequence and key head, one part of
+// One block: eight query rows (query, head of the group) of one sequence and key head, one part of
 // the tokens.
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreads, NT > 1 || D > 128 ? 2 : kBlocksPerSm)
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, D > 128 ? 2 : kBlocksPerSm)
 kv4_attention_kernel(const Kv4Attention p) {
   constexpr int P = sizeof(T) == 4 ? 2 : 1;       // fp16 planes of q
   constexpr bool kCoarse = std::is_same_v<T, __nv_bfloat16>;
   constexpr int W = kCoarse ? 1 : 2;              // fp16 planes of the weights
   constexpr float kUnit = kCoarse ? 0x1p-24f : 1.0f;  // what a code of 1 is to the tensor cores
-  constexpr int R = 8 * NT;
+  constexpr int R = kQueries;
   constexpr int KW = D / 32;                      // words of a key row that a thread holds
   constexpr int VW = D / 64;                      // words of a value row that a thread holds
-  constexpr bool kAllValues = NT == 1 && D <= 128;  // registers for a whole tile's values
+  constexpr bool kAllValues = D <= 128;  // registers for a whole tile's values
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float row_a[R], row_b[R];            // factor of a score, sum of the scaled query
   __shared__ float join_m[kWarps][R], join_l[kWarps][R], join_s[kWarps][R];
@@ -172,7 +177,7 @@ kv4_attention_kernel(const Kv4Attention p) {
   }
 
   // ---- queries: one warp per row, brought to fp16 by a power of two, laid out as MMA fragments
-  uint32_t* q_frag = reinterpret_cast<uint32_t*>(smem);       // [plane][nt][k step][lane][2]
+  uint32_t* q_frag = reinterpret_cast<uint32_t*>(smem);       // [plane][k step][lane][2]
   for (int r = warp; r < R; r += kWarps) {
     float x[D / 32];
     float top = 0.0f, sum = 0.0f;
@@ -211,33 +216,30 @@ kv4_attention_kernel(const Kv4Attention p) {
       float v = x[e] * f1 * f2;
       if (n & 1) v *= 0.0625f;
       __half* dst = reinterpret_cast<__half*>(
-          &q_frag[(((r >> 3) * (D / 16) + step) * 32 + ((r & 7) * 4 + tj)) * 2 + reg]) + half_at;
+          &q_frag[(step * 32 + r * 4 + tj) * 2 + reg]) + half_at;
       const __half hi = __float2half_rn(v);
       *dst = hi;
-      if (P == 2) dst[NT * (D / 16) * 32 * 2 * 2] = __float2half_rn(v - __half2float(hi));
+      if (P == 2) dst[(D / 16) * 32 * 2 * 2] = __float2half_rn(v - __half2float(hi));
     }
   }
   __syncthreads();
 
-  float o[D / 16][NT][4];
-  float m_run[NT][2];
-  uint64_t l_run[NT], s_run[NT], ra[NT], rb[NT];   // pairs: query rows 2j and 2j + 1 of the eight
-  int pos[NT][2];
+  float o[D / 16][4];
+  float m_run[2];
+  uint64_t l_run, s_run, ra, rb;   // pairs: query rows 2j and 2j + 1 of the eight
+  int pos[2];
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
+  for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i)
+    for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
+  const int r = 2 * j;
+  l_run = s_run = 0ull;
+  ra = pack2(row_a[r], row_a[r + 1]);
+  rb = pack2(row_b[r], row_b[r + 1]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[i][nt][e] = 0.0f;
-    const int r = 8 * nt + 2 * j;
-    l_run[nt] = s_run[nt] = 0ull;
-    ra[nt] = pack2(row_a[r], row_a[r + 1]);
-    rb[nt] = pack2(row_b[r], row_b[r + 1]);
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      m_run[nt][e] = -INFINITY;
-      pos[nt][e] = length - p.count + (row0 + r + e) / p.group;
-    }
+  for (int e = 0; e < 2; ++e) {
+    m_run[e] = -INFINITY;
+    pos[e] = length - p.count + (row0 + r + e) / p.group;
   }
   for (; ti < t_end; ti += kWarps) {
     const int t0 = range.tile(ti) * kTile;
@@ -266,24 +268,20 @@ kv4_attention_kernel(const Kv4Attention p) {
     }
 
     // ---- scores, in units of 1 / a
-    float s[kSub][NT][4];
+    float s[kSub][4];
 #pragma unroll
     for (int u = 0; u < kSub; ++u)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[u][nt][e] = 0.0f;
+      for (int e = 0; e < 4; ++e) s[u][e] = 0.0f;
 #pragma unroll
     for (int w = 0; w < KW; ++w)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        uint2 qf[P][NT];
+        uint2 qf[P];
 #pragma unroll
         for (int pl = 0; pl < P; ++pl)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            qf[pl][nt] = *reinterpret_cast<const uint2*>(
-                &q_frag[(((pl * NT + nt) * (D / 16) + 2 * w + h) * 32 + lane) * 2]);
+          qf[pl] = *reinterpret_cast<const uint2*>(
+              &q_frag[((pl * (D / 16) + 2 * w + h) * 32 + lane) * 2]);
 #pragma unroll
         for (int u = 0; u < kSub; ++u) {
           uint32_t e0, o0, e1, o1;
@@ -295,10 +293,8 @@ kv4_attention_kernel(const Kv4Attention p) {
             codes_lower<kCoarse>(kw[u][1][w], e1, o1);
           }
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int pl = 0; pl < P; ++pl)
-              mma_f16(s[u][nt], e0, e1, o0, o1, qf[pl][nt].x, qf[pl][nt].y);
+          for (int pl = 0; pl < P; ++pl)
+            mma_f16(s[u], e0, e1, o0, o1, qf[pl].x, qf[pl].y);
         }
       }
     float2 kf[kSub][2], vf[kSub][2];
@@ -326,83 +322,80 @@ kv4_attention_kernel(const Kv4Attention p) {
     }
 
     // ---- softmax: scores in units of log2, reference = running maximum of score + exponent of s_v
-    uint32_t pw[W][kSub][NT][2];                  // weights times s_v, fp16 pairs
+    uint32_t pw[W][kSub][2];                  // weights times s_v, fp16 pairs
+    float top[2] = {-INFINITY, -INFINITY};
+    uint64_t x[kSub][2];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float top[2] = {-INFINITY, -INFINITY};
-      uint64_t x[kSub][2];
+    for (int u = 0; u < kSub; ++u)
 #pragma unroll
-      for (int u = 0; u < kSub; ++u)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          x[u][e] = fma2(pack2(s[u][nt][2 * e], s[u][nt][2 * e + 1]), pack2(kf[u][e].x, kf[u][e].x),
-                         mul2(pack2(kf[u][e].y, kf[u][e].y), rb[nt]));
-          // 32 + the exponent field of the fp16 scale, as a float: its true exponent + 47 (less for subnormal
-          // scales, which then only leave the weights some of their room)
-          const float ev = __uint_as_float(((vp[u][e] << 8) & 0x007c0000u) | 0x42000000u);
-          float2 r = unpack2(fma2(x[u][e], ra[nt], pack2(ev, ev)));
-          if (!whole) {
-            const int t = t0 + 16 * u + g + 8 * e;
-            const bool there = here[u] >= 0 && t < length;
-            if (!(there && sees(p, t, pos[nt][0]))) r.x = -INFINITY;
-            if (!(there && sees(p, t, pos[nt][1]))) r.y = -INFINITY;
-          }
-          top[0] = fmaxf(top[0], r.x);
-          top[1] = fmaxf(top[1], r.y);
+      for (int e = 0; e < 2; ++e) {
+        x[u][e] = fma2(pack2(s[u][2 * e], s[u][2 * e + 1]), pack2(kf[u][e].x, kf[u][e].x),
+                       mul2(pack2(kf[u][e].y, kf[u][e].y), rb));
+        // 32 + the exponent field of the fp16 scale, as a float: its true exponent + 47 (less for subnormal
+        // scales, which then only leave the weights some of their room)
+        const float ev = __uint_as_float(((vp[u][e] << 8) & 0x007c0000u) | 0x42000000u);
+        float2 r = unpack2(fma2(x[u][e], ra, pack2(ev, ev)));
+        if (!whole) {
+          const int t = t0 + 16 * u + g + 8 * e;
+          const bool there = here[u] >= 0 && t < length;
+          if (!(there && sees(p, t, pos[0]))) r.x = -INFINITY;
+          if (!(there && sees(p, t, pos[1]))) r.y = -INFINITY;
         }
+        top[0] = fmaxf(top[0], r.x);
+        top[1] = fmaxf(top[1], r.y);
+      }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 4));
+      top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 8));
+      top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 16));
+    }
+    if (top[0] > m_run[0] || top[1] > m_run[1]) {
+      float alpha[2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 4));
-        top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 8));
-        top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 16));
+        const bool more = top[c] > m_run[c];
+        alpha[c] = more ? exp2_fast(m_run[c] - top[c]) : 1.0f;      // 0 while nothing was seen
+        m_run[c] = more ? top[c] : m_run[c];
       }
-      if (top[0] > m_run[nt][0] || top[1] > m_run[nt][1]) {
-        float alpha[2];
+      const uint64_t a2 = pack2(alpha[0], alpha[1]);
+      l_run = mul2(l_run, a2);
+      s_run = mul2(s_run, a2);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const bool more = top[c] > m_run[nt][c];
-          alpha[c] = more ? exp2_fast(m_run[nt][c] - top[c]) : 1.0f;      // 0 while nothing was seen
-          m_run[nt][c] = more ? top[c] : m_run[nt][c];
-        }
-        const uint64_t a2 = pack2(alpha[0], alpha[1]);
-        l_run[nt] = mul2(l_run[nt], a2);
-        s_run[nt] = mul2(s_run[nt], a2);
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          o[i][nt][0] *= alpha[0];
-          o[i][nt][1] *= alpha[1];
-          o[i][nt][2] *= alpha[0];
-          o[i][nt][3] *= alpha[1];
-        }
+      for (int i = 0; i < D / 16; ++i) {
+        o[i][0] *= alpha[0];
+        o[i][1] *= alpha[1];
+        o[i][2] *= alpha[0];
+        o[i][3] *= alpha[1];
       }
-      const uint64_t ref = pack2(m_run[nt][0] == -INFINITY ? 0.0f : kExponentBias - m_run[nt][0],
-                                 m_run[nt][1] == -INFINITY ? 0.0f : kExponentBias - m_run[nt][1]);
-#pragma unroll
-      for (int u = 0; u < kSub; ++u)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float2 a = unpack2(fma2(x[u][e], ra[nt], ref));
-          float2 w = make_float2(exp2_fast(a.x), exp2_fast(a.y));
-          float vx = vf[u][e].x * 16384.0f, vx1 = vx, vy = vf[u][e].y, vy1 = vy;
-          if (!whole) {
-            // a hidden token's scale and minimum may be anything: its weight of 0 must not meet them
-            const int t = t0 + 16 * u + g + 8 * e;
-            const bool there = here[u] >= 0 && t < length;
-            if (!(there && sees(p, t, pos[nt][0]))) { w.x = 0.0f; vx = vy = 0.0f; }
-            if (!(there && sees(p, t, pos[nt][1]))) { w.y = 0.0f; vx1 = vy1 = 0.0f; }
-          }
-          const uint64_t w2 = pack2(w.x, w.y);
-          l_run[nt] = add2(l_run[nt], w2);
-          s_run[nt] = fma2(w2, pack2(vy, vy1), s_run[nt]);
-          const float2 q = unpack2(mul2(w2, pack2(vx, vx1)));
-          const uint32_t h = half_pair(q.x, q.y);
-          pw[0][u][nt][e] = h;
-          if (W == 2) {
-            const float2 f = half_values(h);
-            pw[W - 1][u][nt][e] = half_pair(q.x - f.x, q.y - f.y);
-          }
-        }
     }
+    const uint64_t ref = pack2(m_run[0] == -INFINITY ? 0.0f : kExponentBias - m_run[0],
+                               m_run[1] == -INFINITY ? 0.0f : kExponentBias - m_run[1]);
+#pragma unroll
+    for (int u = 0; u < kSub; ++u)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float2 a = unpack2(fma2(x[u][e], ra, ref));
+        float2 w = make_float2(exp2_fast(a.x), exp2_fast(a.y));
+        float vx = vf[u][e].x * 16384.0f, vx1 = vx, vy = vf[u][e].y, vy1 = vy;
+        if (!whole) {
+          // a hidden token's scale and minimum may be anything: its weight of 0 must not meet them
+          const int t = t0 + 16 * u + g + 8 * e;
+          const bool there = here[u] >= 0 && t < length;
+          if (!(there && sees(p, t, pos[0]))) { w.x = 0.0f; vx = vy = 0.0f; }
+          if (!(there && sees(p, t, pos[1]))) { w.y = 0.0f; vx1 = vy1 = 0.0f; }
+        }
+        const uint64_t w2 = pack2(w.x, w.y);
+        l_run = add2(l_run, w2);
+        s_run = fma2(w2, pack2(vy, vy1), s_run);
+        const float2 q = unpack2(mul2(w2, pack2(vx, vx1)));
+        const uint32_t h = half_pair(q.x, q.y);
+        pw[0][u][e] = h;
+        if (W == 2) {
+          const float2 f = half_values(h);
+          pw[W - 1][u][e] = half_pair(q.x - f.x, q.y - f.y);
+        }
+      }
 
     // ---- output
 #pragma unroll
@@ -414,14 +407,12 @@ kv4_attention_kernel(const Kv4Attention p) {
           load_words<4 * VW>(v_lane + at * kRow + ((e & 1) + 8 * (e >> 1)) * kRow, vw[0][e]);
       }
       const auto& vu = vw[kAllValues ? u : 0];
-      uint32_t b0[W][NT], b1[W][NT];
+      uint32_t b0[W], b1[W];
 #pragma unroll
-      for (int pl = 0; pl < W; ++pl)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          b0[pl][nt] = transpose8(pw[pl][u][nt][0]);
-          b1[pl][nt] = transpose8(pw[pl][u][nt][1]);
-        }
+      for (int pl = 0; pl < W; ++pl) {
+        b0[pl] = transpose8(pw[pl][u][0]);
+        b1[pl] = transpose8(pw[pl][u][1]);
+      }
 #pragma unroll
       for (int w = 0; w < VW; ++w)
 #pragma unroll
@@ -439,10 +430,8 @@ kv4_attention_kernel(const Kv4Attention p) {
               codes_lower<kCoarse>(z1, e1, o1);
             }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int pl = 0; pl < W; ++pl)
-                mma_f16(o[4 * w + 2 * h + h2][nt], e0, o0, e1, o1, b0[pl][nt], b1[pl][nt]);
+            for (int pl = 0; pl < W; ++pl)
+              mma_f16(o[4 * w + 2 * h + h2], e0, o0, e1, o1, b0[pl], b1[pl]);
           }
         }
     }
@@ -450,35 +439,30 @@ kv4_attention_kernel(const Kv4Attention p) {
 
   // ---- the warps' results joined: numerators in units of 2^m
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-    for (int sh = 4; sh < 32; sh <<= 1) {
-      l_run[nt] = add2(l_run[nt], __shfl_xor_sync(0xffffffffu, l_run[nt], sh));
-      s_run[nt] = add2(s_run[nt], __shfl_xor_sync(0xffffffffu, s_run[nt], sh));
-    }
-    if (g == 0) {
-      const int r = 8 * nt + 2 * j;
-      const float2 l = unpack2(l_run[nt]), sm = unpack2(s_run[nt]);
-      join_m[warp][r] = m_run[nt][0];
-      join_m[warp][r + 1] = m_run[nt][1];
-      join_l[warp][r] = l.x;
-      join_l[warp][r + 1] = l.y;
-      join_s[warp][r] = sm.x;
-      join_s[warp][r + 1] = sm.y;
-    }
+  for (int sh = 4; sh < 32; sh <<= 1) {
+    l_run = add2(l_run, __shfl_xor_sync(0xffffffffu, l_run, sh));
+    s_run = add2(s_run, __shfl_xor_sync(0xffffffffu, s_run, sh));
+  }
+  if (g == 0) {
+    const int r = 2 * j;
+    const float2 l = unpack2(l_run), sm = unpack2(s_run);
+    join_m[warp][r] = m_run[0];
+    join_m[warp][r + 1] = m_run[1];
+    join_l[warp][r] = l.x;
+    join_l[warp][r + 1] = l.y;
+    join_s[warp][r] = sm.x;
+    join_s[warp][r + 1] = sm.y;
   }
   __syncthreads();                                            // also: the query fragments are read
   float* o_sh = reinterpret_cast<float*>(smem);               // [warp][row][D + 4]
 #pragma unroll
   for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float* dst = o_sh + (size_t)(warp * R + 8 * nt + 2 * j + c) * (D + 4) + g * (D / 8) + 2 * i;
-        dst[0] = o[i][nt][c] * (0x1p-14f / kUnit);
-        dst[1] = o[i][nt][2 + c] * (0x1p-18f / kUnit);        // codes of odd channels stood for 16 n
-      }
+    for (int c = 0; c < 2; ++c) {
+      float* dst = o_sh + (size_t)(warp * R + 2 * j + c) * (D + 4) + g * (D / 8) + 2 * i;
+      dst[0] = o[i][c] * (0x1p-14f / kUnit);
+      dst[1] = o[i][2 + c] * (0x1p-18f / kUnit);        // codes of odd channels stood for 16 n
+    }
   __syncthreads();
   for (int idx = threadIdx.x; idx < rows_here * (D / 4); idx += kThreads) {
     const int r = idx / (D / 4), c4 = idx % (D / 4) * 4;
@@ -577,23 +561,23 @@ kv4_join_kernel(const float* __restrict__ part, T* __restrict__ out, int64_t row
 
 // Parts of the tokens of one sequence and key head: one round of blocks over all SMs if there are few of
 // them, else two, so that sequences of other lengths even out (64 sequences of up to 8192 tokens, us for 1 : 2 :
-// 3 : 4 rounds, 117 : 113 : 116 : 120; 200 of 2000 88 : 87 : 109 : 108).  Every part at least `least` tokens: a
-// tile for every warp (2000 tokens of 8 heads, 128 : 512 tokens a part, 7.4 : 10.4; 131072 of 4 heads 27.2 :
-// 27.2), two tiles of the many-row kernel (100 queries, 4000 tokens, 256 : 1024, 33 : 49); fewer than four parts
-// are not worth the second launch (200 tokens 7.2 split, 6.9 not).  The lengths are on the device, so the table's
-// width stands for the longest.
-int splits_for(int64_t units, int max_tokens, int per_sm, int least) {
-  const int64_t slots = (int64_t)per_sm * device_sms();
-  const int64_t want = 2 * units <= slots ? slots / units : ceil_div64(2 * slots, units);
+// 3 : 4 rounds, 117 : 113 : 116 : 120; 200 of 2000 88 : 87 : 109 : 108), but one of the many-row kernel, whose
+// blocks take 8 us to begin and end (32 sequences of 1000 tokens, 24 rows, 43 : 67).  Every part at least `least`
+// tokens: a tile for every warp (2000 tokens of 8 heads, 128 : 512 tokens a part, 7.4 : 10.4; 131072 of 4 heads
+// 27.2 : 27.2), two tiles of the many-row kernel (100 queries, 4000 tokens, 256 : 1024, 33 : 49); fewer than four
+// parts are not worth the second launch (200 tokens 7.2 split, 6.9 not).  The lengths are on the device, so the
+// table's width stands for the longest.
+int splits_for(int64_t units, int max_tokens, bool many) {
+  const int64_t slots = (int64_t)(many ? 1 : kBlocksPerSm) * device_sms();
+  const int least = many ? 256 : kTile * kWarps;
+  const int64_t want = many || 2 * units <= slots ? slots / units : ceil_div64(2 * slots, units);
   const int64_t most = max_tokens < 4 * least ? 1 : max_tokens / least;
   const int64_t s = want < most ? want : most;
   return (int)(s < 1 ? 1 : (s > kMaxSplits ? kMaxSplits : s));
 }
 
-int row_block(int rows, int dim) { return rows <= 8 ? 1 : (rows <= 16 || dim > 128 ? 2 : 4); }
-
 struct Plan {
-  int nt, row_tiles, splits;
+  int row_tiles, splits;
   bool tc;                              // the tensor-core kernel for many rows
   int64_t blocks;
 };
@@ -602,13 +586,12 @@ Plan plan_of(const modiff_kv4_cache* c, int batch, int count, int heads, int max
   Plan pl;
   const int rows = count * (heads / c->heads);
   pl.tc = kv4_tc_wanted(rows, c->dim, dtype);
-  pl.nt = row_block(rows, c->dim);
-  const int tile = pl.tc ? kv4_tc_rows() : 8 * pl.nt;
+  const int tile = pl.tc ? kv4_tc_rows() : kQueries;
   pl.row_tiles = ceil_div(rows, tile);
   const int64_t units = (int64_t)batch * c->heads * pl.row_tiles;
   int64_t tokens = (int64_t)max_pages * c->page_size;
   if (window > 0 && (int64_t)window + sinks + tile < tokens) tokens = (int64_t)window + sinks + tile;
-  pl.splits = splits_for(units, (int)tokens, pl.tc ? 1 : kBlocksPerSm, pl.tc ? 256 : kTile * kWarps);
+  pl.splits = splits_for(units, (int)tokens, pl.tc);
   pl.blocks = units * pl.splits;
   return pl;
 }
@@ -630,12 +613,12 @@ int join(const Kv4Attention& p, cudaStream_t s) {
   return MODIFF_OK;
 }
 
-template <typename T, int D, int NT>
+template <typename T, int D>
 int launch_attention(const Kv4Attention& p, int64_t blocks, cudaStream_t s) {
-  constexpr int smem = smem_bytes<T, D, NT>();
+  constexpr int smem = smem_bytes<T, D>();
   static SmemLimit limit;
-  MODIFF_CUDA(raise_smem_limit(kv4_attention_kernel<T, D, NT>, smem, limit));
-  kv4_attention_kernel<T, D, NT><<<(unsigned)blocks, kThreads, smem, s>>>(p);
+  MODIFF_CUDA(raise_smem_limit(kv4_attention_kernel<T, D>, smem, limit));
+  kv4_attention_kernel<T, D><<<(unsigned)blocks, kThreads, smem, s>>>(p);
   MODIFF_LAUNCH_CHECK("kv4_attention_kernel");
   return join<T, D>(p, s);
 }
@@ -646,10 +629,7 @@ int by_rows(const Kv4Attention& p, const Plan& pl, int dtype, cudaStream_t s) {
     const int rc = kv4_launch_tc(p, dtype, s);
     return rc ? rc : join<T, D>(p, s);
   }
-  if (pl.nt == 1) return launch_attention<T, D, 1>(p, pl.blocks, s);
-  if (pl.nt == 2) return launch_attention<T, D, 2>(p, pl.blocks, s);
-  if constexpr (D <= 128) return launch_attention<T, D, 4>(p, pl.blocks, s);
-  return MODIFF_ERR_INVALID;
+  return launch_attention<T, D>(p, pl.blocks, s);
 }
 
 int check_shape(const modiff_kv4_cache* c, int batch, int count, int heads) {

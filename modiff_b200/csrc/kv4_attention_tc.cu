@@ -14,11 +14,17 @@
 //   2^(reference - 5), at most 2^15.
 // While one group's softmax runs the tensor pipe works for the other.
 //
-// Queries are brought to fp16 by a power of two per row (exact for bf16).  A value that is not finite is
+// Queries are brought to fp16 by a power of two per row (exact).  A value that is not finite is
 // replaced by zero and makes the rows that see it NaN, so that rows that do not see it never meet it.
 //
-// Bound: tensor pipe (2048 cycles a tile of 128 keys and 256 rows of 128 channels); the loaders need about
-// 500 issue slots of a scheduler for it, the softmax about 1000.
+// Bound: tensor pipe and exponentials alike, 2048 cycles a tile of 128 keys and 256 rows of 128 channels.  4
+// pieces of 1000 queries over up to 8000 tokens, window 2048, 32 / 8 heads of 128, bf16: 255 us, of which 34 are
+// the blocks' beginnings and ends, 32 the steps with hidden keys; without exponentials, maxima and dequantisation
+// it would be 178: what is left are the roles' waits for each other.  What it took: one group of warps for loading
+// and weighing 447, loaders of their own 310, half tiles of 64 keys with the next scores multiplied meanwhile 299,
+// queries laid out in 16-byte chunks 274, masks out of the steps that need none 264, by bit 255.  Not better:
+// exponentials before the maximum is known (278), scores fetched a step ahead by four loader warps (323), one
+// straight copy of the step for each kind of mask (281, spills).
 #include <type_traits>
 
 #include "kv4.cuh"
@@ -569,13 +575,13 @@ int launch(const Kv4Attention& p, cudaStream_t s) {
 
 }  // namespace
 
-// From 17 rows per key head on (bf16, us, kv4_attention.cu : this kernel; 4 sequences of up to 8000 tokens, 8 key
-// heads: 16 rows 31 : 45, 24 rows 57 : 45, 48 rows 84 : 47; 61 prompts of 39 tokens 114 : 48).  In fp16 from 64:
+// From 41 rows per key head on (bf16, us, kv4_attention.cu : this kernel; 4 sequences of up to 8000 tokens, 8 key
+// heads: 24 rows 30 : 45, 32 rows 38 : 45, 48 rows 51 : 46; 64 of 8192 tokens, 32 rows 373 : 405).  In fp16 from 64:
 // keys, values and weights are rounded to fp16 here, once each, which leaves outputs off by 4 - 7e-4, two or three
-// times their own rounding, and the other kernel's are as exact as that (24 rows 53 : 38, 64 rows about 85 : 38).
-// An exact split of all three would double this kernel's products.
+// times their own rounding, and the other kernel's are as exact as that (48 rows 59 : 40, 64 rows 72 : 42).  An
+// exact split of all three would double this kernel's products.
 bool kv4_tc_wanted(int rows, int dim, int dtype) {
-  return dtype != MODIFF_FP32 && dim <= 128 && rows > (dtype == MODIFF_BF16 ? 16 : 63);
+  return dtype != MODIFF_FP32 && dim <= 128 && rows > (dtype == MODIFF_BF16 ? 40 : 63);
 }
 int kv4_tc_rows() { return kRows; }
 

@@ -8,7 +8,8 @@
 // Bound: HBM, every value read and written once.  A group of lanes owns one token's row of one head:
 // a lane holds V pairs (two accesses of V elements), so that both members of a pair meet in one
 // thread and only the sum of squares crosses lanes.  A group walks several heads of its token with
-// the angles and weights in registers, loads of all of them issued first.
+// the angles and weights in registers, loads of all of them issued first.  65536 tokens, 16 heads of 40, fp32:
+// 69 us, 5.0 TB/s; one token 2.6 us.
 #include "types.cuh"
 
 namespace modiff {
@@ -168,7 +169,8 @@ int launch(NormRopeParams& p, cudaStream_t stream) {
     p.items = (int)items;
     return items;
   };
-  // several heads of a token per group once every SM still gets eight blocks
+  // Several heads of a token per group once every SM still gets eight blocks (32 + 8 heads of 128, bf16, us for one
+  // : four heads a group: 300 tokens 3.6 : 4.2, 1000 tokens 7.3 : 6.7, 16000 tokens 92 : 73).
   constexpr int kStep = NU == 1 ? 4 : 1;
   const bool wide = kStep > 1 && plan(kStep) >= 8ll * device_sms() * kGroups;
   const int64_t items = plan(wide ? kStep : 1);

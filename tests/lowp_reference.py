@@ -147,7 +147,7 @@ def attention(q, cache, table, lengths, scale, causal=True, window=0, sinks=0):
                 # its weight: exp2 (2^-21) and, against the codes, one rounding to fp16 for bf16 (22 bits
                 # otherwise); the sums over the tokens
                 much = p @ (vs[sees, None] * vq[sees] + vm[sees, None].abs())
-                many = d <= 128 and n * group > {torch.bfloat16: 16, torch.float16: 63}.get(dtype, n * group)
+                many = d <= 128 and n * group > {torch.bfloat16: 40, torch.float16: 63}.get(dtype, n * group)
                 weight = 2.0 ** -20 + (2.0 ** -11 if many or dtype == torch.bfloat16 else 2.0 ** -21)
                 if many:
                     # many rows: keys and values as fp16 numbers, one rounding (half a step, 2^-11) each, and
