@@ -180,7 +180,8 @@ kv4_attention_kernel(const Kv4Attention p) {
   uint32_t* q_frag = reinterpret_cast<uint32_t*>(smem);       // [plane][k step][lane][2]
   for (int r = warp; r < R; r += kWarps) {
     float x[D / 32];
-    float top = 0.0f, sum = 0.0f;
+    uint32_t top = 0;                             // largest magnitude, by its bits: a NaN is above infinity
+    float sum = 0.0f;
     const int rr = row0 + r;
     const bool real = r < rows_here;
     int member;
@@ -190,21 +191,23 @@ kv4_attention_kernel(const Kv4Attention p) {
 #pragma unroll
     for (int e = 0; e < D / 32; ++e) {
       x[e] = real ? to_f32<T>(src[lane + 32 * e]) : 0.0f;
-      top = fmaxf(top, fabsf(x[e]));
+      top = max(top, __float_as_uint(fabsf(x[e])));
       sum += x[e];
     }
     for (int o = 16; o > 0; o >>= 1) {
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
       sum += __shfl_xor_sync(0xffffffffu, sum, o);
     }
     // power of two that brings the largest element to [2^14, 2^15) (a subnormal one less far); in two
     // factors, for fp32's range
+    const bool finite = top < 0x7f800000u;
     int e2 = 0;
-    if (top > 0.0f && top < INFINITY) e2 = 141 - (int)(__float_as_uint(top) >> 23);
+    if (top > 0 && finite) e2 = 141 - (int)(top >> 23);
     const float f1 = __int_as_float((127 + e2 / 2) << 23), f2 = __int_as_float((127 + e2 - e2 / 2) << 23);
     if (lane == 0) {
       // score = a (s_k (q' . code') + m_k b) with q' the scaled query and code' = code * unit
-      row_a[r] = p.scale2 / kUnit * __int_as_float((127 - e2 / 2) << 23) * __int_as_float((127 - (e2 - e2 / 2)) << 23);
+      // (not a number for a query that is not finite: its scores may all be -inf, which stands for hidden)
+      row_a[r] = (finite ? p.scale2 / kUnit : __int_as_float(0x7fc00000)) * __int_as_float((127 - e2 / 2) << 23) * __int_as_float((127 - (e2 - e2 / 2)) << 23);
       row_b[r] = sum * f1 * f2 * kUnit;
     }
 #pragma unroll

@@ -243,23 +243,26 @@ kv4_attention_tc_kernel(const Kv4Attention p) {
 #pragma unroll
   for (int u = 0; u < kBatch; ++u) {
     const int r = q_row + u * kPass;
-    float x[8], top = 0.0f;
+    float x[8];
+    uint32_t top = 0;                             // largest magnitude, by its bits: a NaN is above infinity
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       x[e] = to_f32<T>(raw[u].v[e]);
-      top = fmaxf(top, fabsf(x[e]));
+      top = max(top, __float_as_uint(fabsf(x[e])));
     }
 #pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int o = kLanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
     // power of two that brings the largest element to [2^14, 2^15) (a subnormal one less far); in two
     // factors, for bf16's range
+    const bool finite = top < 0x7f800000u;
     int e2 = 0;
-    if (top > 0.0f && top < INFINITY) e2 = 141 - (int)(__float_as_uint(top) >> 23);
+    if (top > 0 && finite) e2 = 141 - (int)(top >> 23);
     const float f1 = sign * __int_as_float((127 + e2 / 2) << 23), f2 = __int_as_float((127 + e2 - e2 / 2) << 23);
     if (r < kRows) {
-      // divided by both (powers of two, exactly)
+      // divided by both (powers of two, exactly); not a number for a query that is not finite: its scores may all
+      // be -inf, which stands for hidden
       if (chunk == 0)
-        row_a[r] = fabsf(p.scale2) * __int_as_float((127 - e2 / 2) << 23) * __int_as_float((127 - (e2 - e2 / 2)) << 23);
+        row_a[r] = (finite ? fabsf(p.scale2) : __int_as_float(0x7fc00000)) * __int_as_float((127 - e2 / 2) << 23) * __int_as_float((127 - (e2 - e2 / 2)) << 23);
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = x[e] * f1 * f2;
       *reinterpret_cast<uint4*>(q_sh + (r >> 7) * kQTile + (chunk >> 3) * kChunk + (r & 127) * 128 +

@@ -1,7 +1,9 @@
 """Thin Python wrappers over the fp32 graph kernels of libmodiff_b200.so.
 
 Each function allocates its output with torch (device memory plumbing) and launches one
-hand-written kernel on the current CUDA stream.  CUDA float32 tensors only.
+hand-written kernel on the current CUDA stream.  CUDA float32 tensors only, but for the operators of
+a transformer in low precision (`fp8_linear`, `qk_norm_rope`, `kv4_attention` and theirs), which take
+fp16 and bf16 as well (`lowp_ops.py`).
 """
 import ctypes as C
 import math

@@ -578,6 +578,27 @@ def test_kv4_attention_strided_queries_and_empty_batches(cuda):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("n,page", [(2, 16), (100, 64)])
+def test_kv4_attention_of_queries_that_are_not_finite(cuda, n, page, value, dtype):
+    """All keys of one sign, so that every score of such a query is the same infinity: not a number where
+    the query sees anything, 0 where it does not, nothing in the rows beside it."""
+    d, lens = 128, torch.tensor([150, 1], dtype=torch.int32, device=cuda)
+    cache = ops.kv4_cache(-(-150 // page) * 2, 2, page, d, cuda)
+    table = torch.arange(cache.k_codes.shape[0], dtype=torch.int32, device=cuda).view(2, -1)
+    k = 0.5 + torch.rand(2, 150, 2, d, generator=_gen(4)).to(cuda)
+    ops.kv4_append(cache, k, k, table, torch.tensor([150, 150], dtype=torch.int32, device=cuda))
+    q = torch.randn(2, n, 4, d, generator=_gen(5)).to(dtype).to(cuda)
+    clean = ops.kv4_attention(q, cache, table, lens)
+    q[0, 1, 2, 5] = q[1, 0, 3, 7] = value                  # the second one stands before its sequence begins
+    got = ops.kv4_attention(q, cache, table, lens)
+    assert torch.isnan(got[0, 1, 2]).all() and not got[1, 0, 3].any()
+    clean[0, 1, 2] = got[0, 1, 2] = 0
+    assert torch.equal(got, clean)
+
+
+@gpu
 def test_kv4_cache_beyond_32_bits(cuda):
     """Pages whose bytes lie more than 2^32 behind the cache's beginning."""
     pages = 140000
