@@ -5,7 +5,6 @@ wrapper raises `ModiffError` when an entry point returns a non-zero status.
 """
 import ctypes as C
 import os
-import struct
 
 import torch
 
@@ -65,8 +64,7 @@ class Kv4CacheStruct(C.Structure):
 
 _P = C.c_void_p
 _G = C.POINTER(ConvGeom)
-_KV4 = C.c_void_p               # a Kv4CacheStruct by reference, or its bytes (KV4_PACK: a third of the time)
-KV4_PACK = struct.Struct("4Q4i").pack
+_KV4 = C.POINTER(Kv4CacheStruct)
 
 # name -> (restype, argtypes); one entry per declaration of include/modiff_b200.h
 SIGNATURES = {
@@ -170,6 +168,7 @@ SIGNATURES = {
                           [C.c_int] * 4 + [_P]),
     "modiff_kv4_read": (C.c_int, [_KV4, _P, _P, C.c_int, C.c_int, C.c_int, _P, _P, C.c_int, _P]),
     "modiff_kv4_attention_bytes": (C.c_int64, [_KV4] + [C.c_int] * 7),
+    "modiff_packed_call": (C.c_int64, [C.c_int, C.c_char_p]),
     "modiff_kv4_attention": (C.c_int, [_P, C.c_int64, C.c_int64, C.c_int64, _KV4, _P, _P, _P, C.c_int,
                                        C.c_int, C.c_int, C.c_int,
                                        C.c_float, C.c_int, C.c_int, C.c_int, C.c_int, _P, _P]),
@@ -198,6 +197,10 @@ def lib():
         _lib = l
     return _lib
 
+
+# entry points that `modiff_packed_call` knows (each launches one kernel, or as many more as its caller says)
+PACKED = {"modiff_fp8_quantize": 0, "modiff_fp8_linear": 1, "modiff_fp8_linear_x": 2, "modiff_qk_norm_rope": 3,
+          "modiff_kv4_append": 4, "modiff_kv4_read": 5, "modiff_kv4_attention": 6, "modiff_kv4_attention_bytes": 7}
 
 # kernels one successful call of an entry point launches (for launch accounting)
 KERNELS_PER_CALL = {
@@ -274,6 +277,24 @@ def call(name, *args, nbytes=0, tag=None, nops=0):
     if rc != 0:
         check(rc)
     LAUNCHES[0] += KERNELS_PER_CALL.get(name, 0)
+
+
+def call_words(name, words, nbytes=0, nops=0, more=0):
+    """`call` of an entry point of PACKED with its arguments as bytes of 64-bit words; `more` kernels
+    beyond its first."""
+    fn = lib().modiff_packed_call
+    if TIMER is None:
+        rc = fn(PACKED[name], words)
+    else:
+        start = torch.cuda.Event(enable_timing=True)
+        end = torch.cuda.Event(enable_timing=True)
+        start.record()
+        rc = fn(PACKED[name], words)
+        end.record()
+        TIMER.add(name, start, end, nbytes, None, nops)
+    if rc != 0:
+        check(rc)
+    LAUNCHES[0] += 1 + more
 
 
 def check(rc):

@@ -6,6 +6,7 @@ Tensors are CUDA tensors of fp32, fp16 or bf16, all of a call on one device; a c
 device's current stream.  Sums, statistics and softmax are fp32, the result is rounded once.  There is no
 backward pass: inputs that ask for gradients are refused while gradients are recorded.
 """
+import struct
 from typing import NamedTuple
 
 import torch
@@ -49,15 +50,24 @@ def _dtype(name, x):
     return dt
 
 
+# the arguments of the entry points as 64-bit words, without the stream, which is the last
+_CACHE = "4Q4i"
+_PACK = {name: struct.Struct(words + "q").pack for name, words in (
+    ("modiff_fp8_quantize", "9q"), ("modiff_fp8_linear", "15q"), ("modiff_fp8_linear_x", "14q"),
+    ("modiff_qk_norm_rope", "25qdq"), ("modiff_kv4_append", _CACHE + "14q"), ("modiff_kv4_read", _CACHE + "8q"),
+    ("modiff_kv4_attention", _CACHE + "11qd5q"))}
+_PACK_BYTES = struct.Struct(_CACHE + "7q").pack
+
+
 def _call(device, entry, *args, nbytes=0, nops=0, more=0):
     """One entry point on `device`'s current stream, whatever the current device is; `more` kernels
     beyond its first."""
+    words = _PACK[entry](*args, _stream(device))
     if device == _current():
-        _lib.call(entry, *args, _stream(device), nbytes=nbytes, nops=nops)
+        _lib.call_words(entry, words, nbytes, nops, more)
     else:
         with torch.cuda.device(device):
-            _lib.call(entry, *args, _stream(device), nbytes=nbytes, nops=nops)
-    _lib.LAUNCHES[0] += more
+            _lib.call_words(entry, words, nbytes, nops, more)
 
 
 # ------------------------------------------------------------------------------- 8-bit linear layers
@@ -114,8 +124,9 @@ def fp8_pack_weight(w):
     kp = -(-k // 16) * 16
     codes = torch.empty((n, kp), dtype=torch.float8_e4m3fn, device=w.device)
     scale = torch.empty((-(-n // FP8_BLOCK), -(-k // FP8_BLOCK)), dtype=torch.float32, device=w.device)
-    _call(device, 'modiff_fp8_pack_weight', at, pitch, n, k, dt, codes.data_ptr(), kp, scale.data_ptr(),
-          scale.shape[1], nbytes=n * (k * w.element_size() + kp))
+    with torch.cuda.device(device):
+        _lib.call('modiff_fp8_pack_weight', at, pitch, n, k, dt, codes.data_ptr(), kp, scale.data_ptr(),
+                  scale.shape[1], _stream(device), nbytes=n * (k * w.element_size() + kp))
     return codes[:, :k], scale
 
 
@@ -168,7 +179,7 @@ def fp8_linear(x, w, w_scale, bias=None):
                 or x.scale.data_ptr() % 16 or not _pitched(x.scale, 1, row4)):
             raise ModiffError("fp8_linear: rows of codes as fp8_quantize lays them out")
         _call(device, 'modiff_fp8_linear', src.data_ptr(), kp, x.scale.data_ptr(), row4, w.data_ptr(), w_pitch,
-              w_scale.data_ptr(), blocks, _lib.ptr(bias), y.data_ptr(), n, rows, k, n, dt,
+              w_scale.data_ptr(), blocks, 0 if bias is None else bias.data_ptr(), y.data_ptr(), n, rows, k, n, dt,
               nbytes=rows * kp + n * k + y.numel() * y.element_size(), nops=2 * rows * n * k)
     return y
 
@@ -183,8 +194,8 @@ def _fp8_linear_rows(device, x, w, n, k, w_pitch, w_scale, blocks, bias, dt):
         size = _lib.lib().modiff_fp8_linear_bytes(rows, k, n)
         work = keep.new_empty(size, dtype=torch.uint8) if size else None
         _call(device, 'modiff_fp8_linear_x', at, pitch, w.data_ptr(), w_pitch, w_scale.data_ptr(), blocks,
-              None if bias is None else bias.data_ptr(), y.data_ptr(), n, rows, k, n, dt,
-              None if work is None else work.data_ptr(),
+              0 if bias is None else bias.data_ptr(), y.data_ptr(), n, rows, k, n, dt,
+              0 if work is None else work.data_ptr(),
               nbytes=rows * (k + n) * x.element_size() + n * k, nops=2 * rows * n * k, more=int(size > 0))
     return y if x.dim() == 2 else y.view(*x.shape[:-1], n)
 
@@ -213,7 +224,7 @@ def _tokens(name, x):
 def _norm_weight(name, w, d):
     """Address of a weight, and the tensor that holds it."""
     if w is None:
-        return None, None
+        return 0, None
     if w.dtype is not torch.float32 or w.shape != (d,):
         raise ModiffError(f"{name}: fp32 weights of {d} values, got {tuple(w.shape)} {w.dtype}")
     w = w.contiguous()
@@ -270,10 +281,10 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6, i
     rows, half = shape
     q3, q_out, q_args = _norm_side(name, q, None if out is None else out[0])
     n = q3.shape[0]
-    k3, k_out, k_args = None, None, (None, 0, 0, None, 0, 0, 0)
+    k3, k_out, k_args = None, None, (0, 0, 0, 0, 0, 0, 0)
     if k is not None:
         k3, k_out, k_args = _norm_side(name, k, None if out is None else out[1])
-    wide, at = 0, None
+    wide, at = 0, 0
     if positions is not None:
         wide = int(positions.dtype is torch.int64)
         if not (wide or positions.dtype is torch.int32) or positions.numel() != n:
@@ -328,8 +339,8 @@ def _cache(name, cache, table, lengths):
         raise ModiffError(f"{name}: int32 table [batch, pages] and lengths [batch], got {tuple(table.shape)} "
                           f"{table.dtype} and {tuple(lengths.shape)} {lengths.dtype}")
     pages, heads, size, half = shape
-    return (_lib.KV4_PACK(kc.data_ptr(), vc.data_ptr(), kp.data_ptr(), vp.data_ptr(), pages, heads, size, 2 * half),
-            heads, 2 * half, table.contiguous(), lengths.contiguous())
+    return ((kc.data_ptr(), vc.data_ptr(), kp.data_ptr(), vp.data_ptr(), pages, heads, size, 2 * half), heads, 2 * half,
+            table.contiguous(), lengths.contiguous())
 
 
 def kv4_append(cache, k, v, table, lengths):
@@ -356,7 +367,7 @@ def kv4_append(cache, k, v, table, lengths):
         vs = v.stride()
     rows = b * shape[1] * heads
     if rows:
-        _call(device, 'modiff_kv4_append', c, k.data_ptr(), *ks[:3], v.data_ptr(), *vs[:3], table.data_ptr(),
+        _call(device, 'modiff_kv4_append', *c, k.data_ptr(), *ks[:3], v.data_ptr(), *vs[:3], table.data_ptr(),
               lengths.data_ptr(), b, shape[1], per, dt, nbytes=2 * rows * (dim * k.element_size() + dim // 2 + 4))
 
 
@@ -373,7 +384,7 @@ def kv4_read(cache, table, lengths, n, dtype=torch.float32):
     v = torch.empty_like(k)
     rows = b * n * heads
     if rows:
-        _call(device, 'modiff_kv4_read', c, table.data_ptr(), lengths.data_ptr(), b, n, per, k.data_ptr(), v.data_ptr(),
+        _call(device, 'modiff_kv4_read', *c, table.data_ptr(), lengths.data_ptr(), b, n, per, k.data_ptr(), v.data_ptr(),
               _DTYPES[dtype], nbytes=2 * rows * (dim * k.element_size() + dim // 2 + 4))
     return k, v
 
@@ -406,9 +417,9 @@ def kv4_attention(q, cache, table, lengths, scale=None, causal=True, window=0, s
     n, heads = shape[1], shape[2]
     if b * n:
         window, sinks = min(window, 1 << 30), min(sinks, 1 << 30)
-        size = _lib.lib().modiff_kv4_attention_bytes(c, b, n, heads, per, window, sinks, dt)
+        size = _lib.lib().modiff_packed_call(7, _PACK_BYTES(*c, b, n, heads, per, window, sinks, dt))
         work = q.new_empty(size, dtype=torch.uint8) if size else None
-        _call(device, 'modiff_kv4_attention', q.data_ptr(), *q.stride()[:3], c, table.data_ptr(), lengths.data_ptr(),
+        _call(device, 'modiff_kv4_attention', *c, q.data_ptr(), *q.stride()[:3], table.data_ptr(), lengths.data_ptr(),
               out.data_ptr(), b, n, heads, per, dim ** -0.5 if scale is None else scale, 1 if causal else 0, window,
-              sinks, dt, None if work is None else work.data_ptr(), more=int(size > 0))
+              sinks, dt, 0 if work is None else work.data_ptr(), more=int(size > 0))
     return out

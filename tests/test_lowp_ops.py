@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import lowp_reference as ref
-from modiff_b200 import ModiffError, _lib, ops
+from modiff_b200 import ModiffError, _lib, lowp_ops, ops
 
 TYPES = [torch.float32, torch.float16, torch.bfloat16]
 gpu = pytest.mark.gpu
@@ -95,6 +95,20 @@ def test_entry_points_refuse_bad_arguments_without_a_device():
     # nothing to do is not an error, and touches nothing
     assert lib.modiff_fp8_quantize(None, 64, 0, 64, 0, None, 64, None, 1, None) == 0
     assert lib.modiff_kv4_append(cache(), a, *s3, a, *s3, a, a, 1, 0, 1, 0, None) == 0
+
+
+def test_arguments_as_words():
+    """Words for every entry of the packed call, and its refusals."""
+    lib = _lib.lib()
+    cache = {"modiff_kv4_append", "modiff_kv4_read", "modiff_kv4_attention", "modiff_kv4_attention_bytes"}
+    for name in _lib.PACKED:
+        pack = lowp_ops._PACK.get(name, lowp_ops._PACK_BYTES).__self__
+        assert pack.size == 8 * len(_lib.SIGNATURES[name][1]) + (40 if name in cache else 0)
+    assert lib.modiff_packed_call(0, None) == 1 and lib.modiff_packed_call(99, bytes(8 * 30)) == 1
+    assert lib.modiff_packed_call(0, bytes(80)) == 1 and lib.modiff_last_error()      # no shape
+    words = lowp_ops._PACK_BYTES(0, 0, 0, 0, 64, 2, 64, 128, 1, 1, 8, 64, 0, 0, 1)
+    c = C.byref(_lib.Kv4CacheStruct(None, None, None, None, 64, 2, 64, 128))
+    assert lib.modiff_packed_call(7, words) == lib.modiff_kv4_attention_bytes(c, 1, 1, 8, 64, 0, 0, 1) > 0
 
 
 def test_entry_points_refuse_sizes_beyond_their_index_types():
