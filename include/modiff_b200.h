@@ -711,6 +711,12 @@ int modiff_kv4_attention(const void* q, int64_t q_seq, int64_t q_token, int64_t 
                          int heads, int max_pages, float scale, int causal, int window, int sinks,
                          int dtype, void* workspace, void* stream);
 
+/* The operators above with their arguments as 64-bit words, in the order of their declarations (floats as doubles;
+ * a modiff_kv4_cache, by value, before all others), for callers whose every argument costs a conversion.  `entry`:
+ * 0 fp8_quantize, 1 fp8_linear, 2 fp8_linear_x, 3 qk_norm_rope, 4 kv4_append, 5 kv4_read, 6 kv4_attention,
+ * 7 kv4_attention_bytes.  Returns what the entry point returns. */
+int64_t modiff_packed_call(int entry, const int64_t* words);
+
 /* Tensor-pipe probe of tcgen05.mma kind::i8 (measurement aid; no counterpart in the reference,
  * whose convolutions are PyTorch fp32, qdiff/quant_layer.py:345-365).  Every unit holds a
  * 128-row A tile per CTA and the B tile in shared memory (K = 128 bytes) and repeats the four

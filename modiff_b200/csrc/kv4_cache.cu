@@ -14,7 +14,7 @@
 // issue; launch latency for a step of single tokens (4 us).  LANES lanes own a row, 8 channels each, of the key and
 // of the value, in registers between the extremes and the codes.  4 x 2048 tokens of 8 heads of 128, fp16: 17.4 us,
 // 2.5 TB/s (21.1 with extremes in fp32, 35.4 with the compiler's divisions and 64-bit indexes as well); reading
-// them back as fp32 20.5 us, 3.7 TB/s, nearly all of it writes.
+// them back as fp32 13.7 us, 5.5 TB/s, nearly all of it writes (20.5 with two accesses of a lane side by side).
 #include <type_traits>
 
 #include "kv4.cuh"
@@ -164,33 +164,43 @@ struct ReadParams {
   FastDiv by_heads, by_count;
 };
 
+// A lane's stores are 16 bytes next to its neighbour's: eight channels of 16-bit values, four of fp32 twice.
 template <typename T, int LANES>
 __global__ void __launch_bounds__(kThreads)
 kv4_read_kernel(const ReadParams p) {
+  constexpr int E = 16 / sizeof(T), kPieces = 8 / E;
+  using Codes = std::conditional_t<E == 8, uint32_t, uint16_t>;
   const int lane = threadIdx.x % LANES;
   const int row = blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
-  if (row >= p.rows || 8 * lane >= p.c.dim) return;
+  if (row >= p.rows) return;
   int head, i;
   const int b = p.by_heads.divmod(p.by_count.divmod(row, i), head);
   const int64_t place = kv4_place(p.c, p.table + (int64_t)b * p.max_pages, p.max_pages,
                                   max(__ldg(p.lengths + b), 0) - p.count + i, head);
   const int64_t to = (((int64_t)b * p.count + i) * p.c.heads + head) * p.c.dim;
-  uint32_t w[2] = {};
+  uint32_t w[2][kPieces] = {};
   float2 sm[2] = {};
   if (place >= 0) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      w[u] = *reinterpret_cast<const uint32_t*>((u ? p.c.v_codes : p.c.k_codes) + place * (p.c.dim / 2) + 4 * lane);
+      const uint8_t* codes = (u ? p.c.v_codes : p.c.k_codes) + place * (p.c.dim / 2);
+#pragma unroll
+      for (int q = 0; q < kPieces; ++q)
+        if (const int c = (q * LANES + lane) * E; c < p.c.dim) w[u][q] = *reinterpret_cast<const Codes*>(codes + c / 2);
       sm[u] = __half22float2(reinterpret_cast<const __half2*>(u ? p.c.v_params : p.c.k_params)[place]);
     }
   }
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    float x[8];
+  for (int u = 0; u < 2; ++u)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = fmaf((float)((w[u] >> (4 * e)) & 15u), sm[u].x, sm[u].y);
-    store_f32<T, 8>(static_cast<T*>(u ? p.v : p.k) + to + 8 * lane, x);
-  }
+    for (int q = 0; q < kPieces; ++q) {
+      const int c = (q * LANES + lane) * E;
+      if (c >= p.c.dim) continue;
+      float x[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] = fmaf((float)((w[u][q] >> (4 * e)) & 15u), sm[u].x, sm[u].y);
+      store_f32<T, E>(static_cast<T*>(u ? p.v : p.k) + to + c, x);
+    }
 }
 
 template <typename T, int LANES>
