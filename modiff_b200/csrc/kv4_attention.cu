@@ -20,8 +20,8 @@
 // More rows are more blocks, next to each other, which meet the codes in L2 (16 rows over 64 x 8192 tokens,
 // bf16: 212 us, as two groups of eight in one block 291).
 //
-// Bound: instruction issue (22 instructions of a warp per 32 tokens' worth of a token and head), then HBM (d + 8
-// bytes per cached token and head).  64 sequences of up to 8192 tokens, 8 key heads of 128, bf16: 113 us, 3.8 TB/s;
+// Bound: dependent instructions of few warps (22 of a warp per cached token and head; issue 56 %, DRAM 47 %), then
+// HBM (d + 8 bytes per cached token and head).  64 sequences of up to 8192 tokens, 8 key heads of 128, bf16: 113 us, 3.8 TB/s;
 // one of 131072, 4 heads: 27 us.  The cache of one sequence and head is split over `splits` blocks and the warps of
 // each; partial results (numerator, sum, maximum) are joined by kv4_join_kernel in a fixed order.  Not better: tiles
 // of 64 tokens, five blocks an SM.
