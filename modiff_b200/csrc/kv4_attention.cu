@@ -432,9 +432,20 @@ kv4_attention_kernel(const Kv4Attention p) {
               codes_lower<kCoarse>(z0, e0, o0);
               codes_lower<kCoarse>(z1, e1, o1);
             }
+            float(&acc)[4] = o[4 * w + 2 * h + h2];
+            if constexpr (sizeof(T) == 4) {
+              // The tensor cores cut off what they add: over thousands of tokens that is 1e-5 of the sum, so
+              // sixteen tokens' products are added to the others by rounding additions.
+              float part[4] = {};
 #pragma unroll
-            for (int pl = 0; pl < W; ++pl)
-              mma_f16(o[4 * w + 2 * h + h2], e0, o0, e1, o1, b0[pl], b1[pl]);
+              for (int pl = 0; pl < W; ++pl) mma_f16(part, e0, o0, e1, o1, b0[pl], b1[pl]);
+              const float2 lo = unpack2(add2(pack2(acc[0], acc[1]), pack2(part[0], part[1])));
+              const float2 hi = unpack2(add2(pack2(acc[2], acc[3]), pack2(part[2], part[3])));
+              acc[0] = lo.x; acc[1] = lo.y; acc[2] = hi.x; acc[3] = hi.y;
+            } else {
+#pragma unroll
+              for (int pl = 0; pl < W; ++pl) mma_f16(acc, e0, o0, e1, o1, b0[pl], b1[pl]);
+            }
           }
         }
     }

@@ -451,12 +451,14 @@ def test_kv4_attention(cuda, lengths, n, heads, kv_heads, page, d, dtype):
 @gpu
 @pytest.mark.parametrize("dtype,gain", [(torch.float32, 2.0), (torch.float16, 2.0), (torch.float16, 0.01)])
 @pytest.mark.parametrize("lengths,n,heads,kv_heads,d", [
-    ([4000], 1, 8, 2, 128), ([900, 10], 2, 10, 5, 64), ([1, 30], 1, 7, 1, 256), ([600], 7, 8, 1, 128)])
+    ([4000], 1, 8, 2, 128), ([900, 10], 2, 10, 5, 64), ([1, 30], 1, 7, 1, 256), ([600], 7, 8, 1, 128),
+    ([16000] * 4, 1, 64, 64, 64)])
 def test_kv4_attention_is_as_exact_as_its_type(cuda, lengths, n, heads, kv_heads, d, dtype, gain):
     """Few query rows.  Root mean squares: weights of 22 bits (2^-23 of each), scores of magnitude 16 at most
     from products and sums in fp32 that are cut at 2^-23 of sums no larger than 16 times the score (their error
     is that of the weight: 16 * 16 * 2^-23 = 2^-15 at worst, in the mean over signs and sizes an eighth), sums
-    of numbers of both signs.  So 2^-18 in all; beside fp16's rounding, 0.84 * 2^-12 in the mean over a binade,
+    of numbers of both signs, rounded at every sixteen tokens (the errors of 16000 tokens' sums, of either sign,
+    are 2^-24 sqrt(16000 / 16) = 2^-19 of a part of the sum at worst).  So 2^-18 in all; beside fp16's rounding, 0.84 * 2^-12 in the mean over a binade,
     that adds less than a thousandth, and the test leaves a tenth."""
     q, cache, table, lens, got = _attend(cuda, lengths, n, heads, kv_heads, 16, d, dtype, seed=11, gain=gain)
     want, _ = ref.attention(q, cache, table, lens, d ** -0.5)
