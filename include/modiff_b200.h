@@ -690,8 +690,9 @@ int modiff_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, void* q_
  *   modiff_kv4_read       the last `count` positions as values, zeros where there is none
  *   modiff_kv4_attention  out[b][i][h] = sum_t softmax_t(scale * q[b][i][h] . k_t) v_t over the positions
  *                         t < lengths[b] and, if `causal`, t <= lengths[b] - count + i, with window > 0
- *                         also t > that - window or t < sinks; 0 where nothing is seen.  `heads` query
- *                         heads share the cache's heads in order.  workspace:
+ *                         also t > that - window or t < sinks; 0 where nothing is seen.  A key whose scale
+ *                         or minimum is not finite makes the rows that see it NaN, such a value makes
+ *                         them not finite.  `heads` query heads share the cache's heads in order.  workspace:
  *                         modiff_kv4_attention_bytes (0: may be NULL), not shared by calls that overlap */
 typedef struct modiff_kv4_cache {
   uint8_t *k_codes, *v_codes;

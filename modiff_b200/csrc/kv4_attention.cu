@@ -58,6 +58,13 @@ __device__ inline uint32_t transpose8(uint32_t v) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
+// An infinite scale or minimum of a key becomes NaN, so that rows that see it are NaN: its score might be -inf, which
+// would hide the key.  (inf 0 + inf; finite numbers stay as they are.)
+__device__ inline uint32_t nan_unless_finite(uint32_t params) {
+  const __half2 h = *reinterpret_cast<const __half2*>(&params);
+  const __half2 r = __hfma2(h, __float2half2_rn(0.0f), h);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
 // Two channels of four codes out of a word: `even` the low halves of two bytes 16 bits apart, as n unit,
 // `odd` the high halves, as 16 n unit.  For bf16 unit is 2^-24 and the masked bits are the subnormal
 // numbers; the even ones of the upper bytes come from a subtraction (exact), because logic instructions,
@@ -305,7 +312,7 @@ kv4_attention_kernel(const Kv4Attention p) {
     for (int u = 0; u < kSub; ++u)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        kf[u][e] = half_values(kp[u][e]);
+        kf[u][e] = half_values(nan_unless_finite(kp[u][e]));
         vf[u][e] = half_values(vp[u][e]);
         if (!kCoarse) {                           // the minimum that belongs to n - 8
           kf[u][e].y = fmaf(8.0f, kf[u][e].x, kf[u][e].y);

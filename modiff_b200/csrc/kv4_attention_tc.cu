@@ -14,8 +14,9 @@
 //   2^(reference - 5), at most 2^15.
 // While one group's softmax runs the tensor pipe works for the other.
 //
-// Queries are brought to fp16 by a power of two per row (exact).  A value that is not finite is
-// replaced by zero and makes the rows that see it NaN, so that rows that do not see it never meet it.
+// Queries are brought to fp16 by a power of two per row (exact).  A key whose scale or minimum is not finite is
+// NaN, and so are its scores; such a value is replaced by zero and makes the rows that see it NaN, so that rows
+// that do not see it never meet it.
 //
 // Bound: tensor pipe and exponentials alike, 2048 cycles a tile of 128 keys and 256 rows of 128 channels.  4
 // pieces of 1000 queries over up to 8000 tokens, window 2048, 32 / 8 heads of 128, bf16: 255 us, of which 34 are
@@ -300,9 +301,10 @@ kv4_attention_tc_kernel(const Kv4Attention p) {
       const int st = i & 1, slot = i % kBitSlots;
       if (!mbar_wait(empty0 + 8 * st, ((uint32_t)(i >> 1) & 1u) ^ 1u, abort_flag)) break;
       bool there = place >= 0;
+      // exponent field of all ones: infinity or NaN
+      const bool bad = there && ((sm & 0x7c00u) == 0x7c00u || (sm & 0x7c000000u) == 0x7c000000u);
+      if (!value && bad) sm = 0x7fff7fffu;                     // its scores are NaN, not what an infinity clamps to
       if (value) {
-        // exponent field of all ones: infinity or NaN
-        const bool bad = there && ((sm & 0x7c00u) == 0x7c00u || (sm & 0x7c000000u) == 0x7c000000u);
         const uint32_t there_bits = __ballot_sync(0xffffffffu, there), bad_bits = __ballot_sync(0xffffffffu, bad);
         if (lane == 0) {
           there_sh[slot][warp - kLoaders] = there_bits;

@@ -395,7 +395,9 @@ def kv4_attention(q, cache, table, lengths, scale=None, causal=True, window=0, s
     heads, which consecutive query heads share.  Query i of sequence b stands at position
     lengths[b] - n + i and sees the positions up to its own; with `window` > 0 only the last `window` of
     them and the first `sinks` of the sequence (tokens outside are not read).  causal=False: every query
-    sees all lengths[b] tokens.  A row that sees nothing is 0.  scale defaults to d ** -0.5."""
+    sees all lengths[b] tokens.  A row that sees nothing is 0.  A cached scale or minimum that is not finite
+    (`kv4_append` writes NaN for a row that holds one) makes the rows that see its key NaN, those that see its
+    value not finite, and no others.  scale defaults to d ** -0.5."""
     name = "kv4_attention"
     device = _device(name, q, table, lengths, *cache)
     c, kv_heads, dim, table, lengths = _cache(name, cache, table, lengths)
