@@ -635,7 +635,8 @@ int modiff_attention_i8(const int8_t* q_codes, const int8_t* k_codes, const int8
 
 /* ---- Operators of a transformer served in low precision.  The reference has none of them; they stand
  * beside its int8 layers and attention (qdiff/quant_layer.py:257-392, qdiff/quant_block.py:181-369).
- * Tensors are fp32, fp16 or bf16 (`dtype`), sums and statistics fp32, with one rounding at the end.
+ * Tensors are fp32, fp16 or bf16 (`dtype`), sums and statistics fp32, with one rounding at the end (what
+ * modiff_kv4_attention rounds before is said there).
  * Strides and pitches count elements (bytes for code rows). */
 #define MODIFF_FP32 0
 #define MODIFF_FP16 1
@@ -693,7 +694,10 @@ int modiff_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, void* q_
  *                         also t > that - window or t < sinks; 0 where nothing is seen.  A key whose scale
  *                         or minimum is not finite makes the rows that see it NaN, such a value makes
  *                         them not finite.  `heads` query heads share the cache's heads in order.  workspace:
- *                         modiff_kv4_attention_bytes (0: may be NULL), not shared by calls that overlap */
+ *                         modiff_kv4_attention_bytes (0: may be NULL), not shared by calls that overlap.
+ *                         fp32, fp16: queries and weights with 22 bits, exact codes.  bf16: weights rounded to
+ *                         fp16, sums of query times code in 17 bits; from 41 query rows per key head on (dim <=
+ *                         128) keys and values rounded to fp16, once each */
 typedef struct modiff_kv4_cache {
   uint8_t *k_codes, *v_codes;
   uint16_t *k_params, *v_params;

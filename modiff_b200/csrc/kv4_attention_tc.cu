@@ -1,24 +1,34 @@
 // Attention over the 4-bit cache for many query rows per key head (prompts and pieces of them), on the
-// 5th-generation tensor cores.  Same result as kv4_attention.cu, fp16 and bf16 tensors.
+// 5th-generation tensor cores.  fp16 and bf16 tensors; fp16 results are as exact as those of kv4_attention.cu.
 //
 // A block owns 256 query rows (query, head of the group) of one sequence and key head, as two groups of
 // 128, and walks the keys in tiles of 128 that both groups share:
-//   four warps each read the codes of keys and of values through the page table and write fp16 numbers
-//   s code + m, rounded once, as operands of an MMA (128-byte swizzle; a key's channels stay in its row,
-//   which is K-major for the scores and N-major for the output; eight channels of a word lie in the
-//   order 0 4 1 5 2 6 3 7, in which they come out of it, and so do the queries');
+//   four warps each read the codes of keys and of values through the page table and write them as fp16 operands of
+//   an MMA (128-byte swizzle; a key's channels stay in its row, which is K-major for the scores and N-major for the
+//   output; eight channels of a word lie in the order 0 4 1 5 2 6 3 7, in which they come out of it, and so do the
+//   queries');
 //   one warp issues S = Q K^T into tensor memory (128 columns a group) and O += P V, with P read from
 //   tensor memory, where the softmax has put it in place of S;
 //   four softmax warps a group, a thread per row, no exchange between threads: maximum, then weights.
-//   O is rescaled only when a row's maximum has grown by more than 2^10; weights are fp16 in units of
-//   2^(reference - 5), at most 2^15.
+//   O is rescaled only when a row's maximum has grown by more than 2^10.
 // While one group's softmax runs the tensor pipe works for the other.
+//
+// What the operands are:
+//   bf16 calls  s code + m, rounded to fp16 once (2^-11 of it at most), for keys and values; weights in fp16, in units
+//               of 2^(reference - 5), at most 2^15.  So a score is off by up to scale 2^-11 sum |q k|, one weight by
+//               2^-11.  Beside the rounding of bf16 outputs (1.66e-3 of them in the mean) that is little while scores
+//               are not large: 1.77e-3 in all on the case below.
+//   fp16 calls  codes as the exact numbers n - 8, scales and minima outside the products (kExact):
+//                 score = s (q . (n - 8)) + (m + 8 s) sum(q),  sum_t p v = sum_t (p s) (n - 8) + sum_t p (m + 8 s),
+//               p s as two fp16 numbers (22 bits) relative to the largest score + exponent of s.  Half as many products
+//               again and twice the softmax's instructions: 423 us where bf16 takes 257, for errors of the output's
+//               own rounding (2.1e-4); with bf16's operands they were 4e-4 to 8.6e-4, and 2.6e-3 where scores reach 60.
 //
 // Queries are brought to fp16 by a power of two per row (exact).  A key whose scale or minimum is not finite is
 // NaN, and so are its scores; such a value is replaced by zero and makes the rows that see it NaN, so that rows
 // that do not see it never meet it.
 //
-// Bound: tensor pipe and exponentials alike, 2048 cycles a tile of 128 keys and 256 rows of 128 channels.  4
+// Bound (bf16): tensor pipe and exponentials alike, 2048 cycles a tile of 128 keys and 256 rows of 128 channels.  4
 // pieces of 1000 queries over up to 8000 tokens, window 2048, 32 / 8 heads of 128, bf16: 255 us, of which 34 are
 // the blocks' beginnings and ends, 32 the steps with hidden keys; without exponentials, maxima and dequantisation
 // it would be 178: what is left are the roles' waits for each other.  What it took: one group of warps for loading
@@ -44,11 +54,15 @@ constexpr int kLoaders = 4;                 // warps 0 .. 3 keys, 4 .. 7 values;
 constexpr int kSoftmaxWarp = 8, kMmaWarp = 16;
 constexpr int kThreads = 32 * 20;           // the last three warps only complete the MMA warp's group
 // Registers: 96 a thread at launch, dealt out anew by group of four warps.
-constexpr int kRegsAtLaunch = 96, kRegsLoad = 72, kRegsSoftmax = 136, kRegsMma = 56;
-static_assert(5 * kRegsAtLaunch >= 2 * kRegsLoad + 2 * kRegsSoftmax + kRegsMma, "register split");
+constexpr int kRegsAtLaunch = 96, kRegsMma = 56;
+template <bool EXACT> constexpr int kRegsLoad = EXACT ? 64 : 72;
+template <bool EXACT> constexpr int kRegsSoftmax = EXACT ? 144 : 136;
+static_assert(5 * kRegsAtLaunch >= 2 * kRegsLoad<false> + 2 * kRegsSoftmax<false> + kRegsMma &&
+                  5 * kRegsAtLaunch >= 2 * kRegsLoad<true> + 2 * kRegsSoftmax<true> + kRegsMma, "register split");
 constexpr int kChunk = kKeys * 128;         // bytes of 128 rows of 64 channels
 constexpr float kGrowth = 10.0f;            // of a row's maximum, in powers of two, before O is rescaled
-constexpr float kRoom = 5.0f;               // weights are at most 2^(kGrowth + kRoom)
+// Weights (times the scale of their value, in fp16 calls) are at most 2^15, kGrowth included.
+template <bool EXACT> constexpr float kRoom = EXACT ? 4.0f : 5.0f;
 constexpr int kBitSlots = 4;
 
 // fp16 x fp16 -> fp32; descriptors as low words and the high word they share.  A from shared or tensor memory.
@@ -118,8 +132,21 @@ __device__ inline uint4 dequantise(uint32_t w, __half2 s, __half2 m) {
   return make_uint4(as_u32(v[0]), as_u32(v[1]), as_u32(v[2]), as_u32(v[3]));
 }
 
+// One word of eight codes as the numbers n - 8.
+__device__ inline uint4 centred(uint32_t w) {
+  const __half2 k1032 = as_half2(0x64086408u), k16th = as_half2(0x2c002c00u), k72 = as_half2(0xd480d480u);   // 1032, 1/16, -72
+  __half2 v[4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t x = i ? w >> 8 : w;
+    v[2 * i] = __hsub2(as_half2((x & 0x000f000fu) | 0x64006400u), k1032);
+    v[2 * i + 1] = __hfma2(as_half2((x & 0x00f000f0u) | 0x64006400u), k16th, k72);
+  }
+  return make_uint4(as_u32(v[0]), as_u32(v[1]), as_u32(v[2]), as_u32(v[3]));
+}
+
 // A row of codes into its place of an operand tile.
-template <int D>
+template <int D, bool EXACT>
 __device__ inline void store_row(uint8_t* tile, int row, const uint32_t (&w)[D / 8], uint32_t params, bool there) {
   const __half2 sm = as_half2(params);
   const __half2 s = __low2half2(sm), m = __high2half2(sm);
@@ -127,7 +154,10 @@ __device__ inline void store_row(uint8_t* tile, int row, const uint32_t (&w)[D /
   const bool edge = fabsf(f.y) > 65000.0f || fabsf(fmaf(15.0f, f.x, f.y)) > 65000.0f;
   uint8_t* base = tile + row * 128;
   auto place = [&](int i) { return reinterpret_cast<uint4*>(base + (i >> 3) * kChunk + (((i & 7) ^ (row & 7)) << 4)); };
-  if (!there) {
+  if (EXACT) {
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) *place(i) = centred(w[i]);
+  } else if (!there) {
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) *place(i) = make_uint4(0u, 0u, 0u, 0u);
   } else if (edge) {
@@ -162,11 +192,14 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
 kv4_attention_tc_kernel(const Kv4Attention p) {
   constexpr int kQTile = 128 * D * 2, kKvTile = kKeys * D * 2;
+  constexpr bool kExact = std::is_same_v<T, __half>;
   extern __shared__ __align__(1024) uint8_t smem[];          // Q [2], K [2], V [2]
   __shared__ __align__(8) uint64_t bar_k_full[2], bar_k_empty[2], bar_v_full[2], bar_v_empty[2];
   __shared__ __align__(8) uint64_t bar_s_full[2][2], bar_p_ready[2][2], bar_pv[2][2], bar_bits[kBitSlots];   // [group][half]
   __shared__ __align__(16) uint32_t there_sh[kBitSlots][4], bad_sh[kBitSlots][4];   // tokens that exist; values that are not finite
-  __shared__ float row_a[kRows];
+  // kExact: of a tile's keys the scale and minimum, of its values the scale's exponent, scale and minimum
+  __shared__ __align__(16) float factor_sh[kExact ? kBitSlots : 1][5][kExact ? kKeys : 4];
+  __shared__ float row_a[kRows], row_b[kExact ? kRows : 1];
   __shared__ uint32_t tmem_base_sh;
   __shared__ int abort_sh;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -207,7 +240,7 @@ kv4_attention_tc_kernel(const Kv4Attention p) {
         mbar_init(smem_u32(&bar_pv[i][h]), 1);
       }
     }
-    for (int i = 0; i < kBitSlots; ++i) mbar_init(smem_u32(&bar_bits[i]), kLoaders);
+    for (int i = 0; i < kBitSlots; ++i) mbar_init(smem_u32(&bar_bits[i]), kExact ? 2 * kLoaders : kLoaders);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kMmaWarp) {
@@ -259,13 +292,20 @@ kv4_attention_tc_kernel(const Kv4Attention p) {
     int e2 = 0;
     if (top > 0 && finite) e2 = 141 - (int)(top >> 23);
     const float f1 = sign * __int_as_float((127 + e2 / 2) << 23), f2 = __int_as_float((127 + e2 - e2 / 2) << 23);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = x[e] * f1 * f2;
+    float sum = 0.0f;
+    if constexpr (kExact) {
+      sum = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    }
     if (r < kRows) {
+      if (kExact && chunk == 0) row_b[kExact ? r : 0] = sum;
       // divided by both (powers of two, exactly); not a number for a query that is not finite: its scores may all
       // be -inf, which stands for hidden
       if (chunk == 0)
         row_a[r] = (finite ? fabsf(p.scale2) : __int_as_float(0x7fc00000)) * __int_as_float((127 - e2 / 2) << 23) * __int_as_float((127 - (e2 - e2 / 2)) << 23);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = x[e] * f1 * f2;
       *reinterpret_cast<uint4*>(q_sh + (r >> 7) * kQTile + (chunk >> 3) * kChunk + (r & 127) * 128 +
                                 (((chunk & 7) ^ (r & 7)) << 4)) =
           make_uint4(half_pair(x[0], x[4]), half_pair(x[1], x[5]), half_pair(x[2], x[6]), half_pair(x[3], x[7]));
@@ -279,7 +319,7 @@ kv4_attention_tc_kernel(const Kv4Attention p) {
 
   if (warp < kSoftmaxWarp) {
     // ------------------------------------------------------------ keys (warps 0 .. 3), values (4 .. 7)
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLoad<kExact>));
     const bool value = warp >= kLoaders;
     const int key = threadIdx.x & 127;
     const uint8_t* codes = value ? p.c.v_codes : p.c.k_codes;
@@ -310,11 +350,21 @@ kv4_attention_tc_kernel(const Kv4Attention p) {
           there_sh[slot][warp - kLoaders] = there_bits;
           bad_sh[slot][warp - kLoaders] = bad_bits;
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&bar_bits[slot]));
         there = there && !bad;
       }
-      store_row<D>(stages + st * kKvTile, key, w, sm, there);
+      if constexpr (kExact) {
+        // what n - 8 stands for is scale (n - 8) + (minimum + 8 scale)
+        const float2 f = there ? half_values(sm) : make_float2(0.0f, 0.0f);
+        float* to = &factor_sh[slot][value ? 3 : 0][key];
+        to[0] = f.x;
+        to[kKeys] = fmaf(8.0f, f.x, f.y);
+        if (value) to[-kKeys] = (float)((int)((sm >> 10) & 31u) - 15);   // f.x is below 2^(that + 1)
+      }
+      if (value || kExact) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bar_bits[slot]));
+      }
+      store_row<D, kExact>(stages + st * kKvTile, key, w, sm, there);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(full0 + 8 * st);
@@ -323,7 +373,7 @@ kv4_attention_tc_kernel(const Kv4Attention p) {
     __syncwarp();
   } else if (warp >= kMmaWarp) {
     // ------------------------------------------------------------ MMAs
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsMma));
     if (warp == kMmaWarp) {
       // This warp's instructions are the critical path (about five cycles each beside the other warps): the
       // descriptors' low words are added to 32-bit constants, waits that come together are one.
@@ -348,9 +398,9 @@ kv4_attention_tc_kernel(const Kv4Attention p) {
       auto products = [&](int g, int h, int st, uint32_t accumulate) {
         const uint32_t vd = v_lo + (uint32_t)(st * (kKvTile >> 4) + h * (kHalf * 128 >> 4));
 #pragma unroll
-        for (int k = 0; k < kHalf / 16; ++k)
+        for (int k = 0; k < (kExact ? 2 : 1) * kHalf / 16; ++k)
           tc_mma_f16_ta(tmem_base + (uint32_t)(256 + 128 * g), tmem_base + (uint32_t)(128 * g + kHalf * h + 8 * k),
-                        vd + (uint32_t)(k * (16 * 128 >> 4)), desc_hi, idesc_o, k > 0 ? 1u : accumulate);
+                        vd + (uint32_t)(k % (kHalf / 16) * (16 * 128 >> 4)), desc_hi, idesc_o, k > 0 ? 1u : accumulate);
         tc_commit(smem_u32(&bar_pv[g][h]));
       };
       const uint32_t k_full0 = smem_u32(&bar_k_full[0]), v_full0 = smem_u32(&bar_v_full[0]);
@@ -395,7 +445,7 @@ kv4_attention_tc_kernel(const Kv4Attention p) {
     }
   } else {
     // ------------------------------------------------------------ softmax, output
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax<kExact>));
     const int g = (warp - kSoftmaxWarp) >> 2, quarter = warp & 3;
     const int r = 128 * g + 32 * quarter + lane;
     const uint32_t t_lane = tmem_base + ((uint32_t)(quarter * 32) << 16);
@@ -403,9 +453,11 @@ kv4_attention_tc_kernel(const Kv4Attention p) {
     if (g == 0 || two) {
       const float ra = row_a[r];
       const uint64_t ra2 = pack2(ra, ra);
+      const float rb = kExact ? row_b[kExact ? r : 0] : 0.0f;
+      const uint64_t rb2 = pack2(rb, rb);
       const int pos = length - p.count + (row0 + r) / p.group;
       float m_ref = -INFINITY;                                 // the row's reference, in units of log2
-      uint64_t l2 = 0ull;                                      // sums of even and odd columns
+      uint64_t l2 = 0ull, s2 = 0ull;                           // sums of even and odd columns; kExact: of weights times minima
       bool ok = true, poisoned = false;
       for (int step = 0; step < 2 * tiles; ++step) {
         const int i = step >> 1, h = step & 1, slot = i % kBitSlots;
@@ -437,24 +489,38 @@ kv4_attention_tc_kernel(const Kv4Attention p) {
             poisoned |= (vis[c] & (c ? bad.y : bad.x)) != 0;
           }
         }
+        // factors of four columns, as two pairs
+        auto factors = [&](int which, int j) {
+          return *reinterpret_cast<const ulonglong2*>(&factor_sh[kExact ? slot : 0][which][kExact ? kHalf * h + j : 0]);
+        };
         tc_wait_ld();
-        float top, top2;
+        float top = -INFINITY, top2 = -INFINITY;
         auto largest = [&](auto all) {
-          auto score = [&](int j) {
-            return decltype(all)::value || (vis[j >> 5] >> (j & 31) & 1u) ? __int_as_float(v[j]) : -INFINITY;
-          };
-          top = max3(score(0), score(1), -INFINITY);
-          top2 = max3(score(2), score(3), -INFINITY);
+          auto seen = [&](int j, float x) { return decltype(all)::value || (vis[j >> 5] >> (j & 31) & 1u) ? x : -INFINITY; };
 #pragma unroll
-          for (int j = 4; j < kHalf; j += 4) {
-            top = max3(score(j), score(j + 1), top);
-            top2 = max3(score(j + 2), score(j + 3), top2);
+          for (int j = 0; j < kHalf; j += 4) {
+            float2 a = make_float2(__int_as_float(v[j]), __int_as_float(v[j + 1]));
+            float2 b = make_float2(__int_as_float(v[j + 2]), __int_as_float(v[j + 3]));
+            if constexpr (kExact) {
+              // the scores, in place of the codes' products; the largest of score + exponent of the value's scale
+              const ulonglong2 ks = factors(0, j), km = factors(1, j), ev = factors(2, j);
+              const uint64_t xa = fma2(pack2(a.x, a.y), ks.x, mul2(km.x, rb2));
+              const uint64_t xb = fma2(pack2(b.x, b.y), ks.y, mul2(km.y, rb2));
+              a = unpack2(xa);
+              b = unpack2(xb);
+              v[j] = __float_as_int(a.x); v[j + 1] = __float_as_int(a.y);
+              v[j + 2] = __float_as_int(b.x); v[j + 3] = __float_as_int(b.y);
+              a = unpack2(fma2(xa, ra2, ev.x));
+              b = unpack2(fma2(xb, ra2, ev.y));
+            }
+            top = max3(seen(j, a.x), seen(j + 1, a.y), top);
+            top2 = max3(seen(j + 2, b.x), seen(j + 3, b.y), top2);
           }
         };
         if (whole) largest(std::true_type());
         else largest(std::false_type());
         top = fmaxf(top, top2);
-        const float m_new = top == -INFINITY ? -INFINITY : top * ra;
+        const float m_new = kExact || top == -INFINITY ? top : top * ra;
         const bool grow = m_new > m_ref + kGrowth || (m_ref == -INFINITY && m_new > -INFINITY);
         if (__any_sync(0xffffffffu, grow)) {
           // nothing was seen before: nothing to rescale, the sum and O are 0
@@ -462,6 +528,7 @@ kv4_attention_tc_kernel(const Kv4Attention p) {
           const float alpha = rescale ? exp2_fast(m_ref - m_new) : 1.0f;
           if (grow) m_ref = m_new;
           l2 = mul2(l2, pack2(alpha, alpha));
+          if (kExact) s2 = mul2(s2, pack2(alpha, alpha));
           if (__any_sync(0xffffffffu, rescale)) {
             // O may be rewritten once the products of the step before are in it; those of two steps before
             // are, this step's scores were multiplied behind them
@@ -480,27 +547,43 @@ kv4_attention_tc_kernel(const Kv4Attention p) {
             }
           }
         }
-        // ---- weights, in place of the scores: two fp16 a column; a hidden key's score of -inf gives 0
-        const float ref = m_ref == -INFINITY ? 0.0f : kRoom - m_ref;
+        // ---- weights, in place of the scores: two fp16 a column; a hidden key's score of -inf gives 0.  kExact: times
+        // the scales of the values, the rounded numbers first, what the rounding left behind them
+        const float ref = m_ref == -INFINITY ? 0.0f : kRoom<kExact> - m_ref;
         const uint64_t ref2 = pack2(ref, ref);
-        uint32_t w[kHalf / 2];
+        uint32_t w[kHalf / 2], rest[kExact ? kHalf / 2 : 16];
         auto weigh = [&](auto all) {
+          ulonglong2 vs = {}, vm = {};
 #pragma unroll
           for (int j = 0; j < kHalf; j += 2) {
+            if (kExact && j % 4 == 0) { vs = factors(3, j); vm = factors(4, j); }
             float2 a = unpack2(fma2(pack2(__int_as_float(v[j]), __int_as_float(v[j + 1])), ra2, ref2));
             if (!decltype(all)::value) {
               if (!(vis[j >> 5] >> (j & 31) & 1u)) a.x = -INFINITY;
               if (!(vis[j >> 5] >> (j & 31) & 2u)) a.y = -INFINITY;
             }
             const float2 e = make_float2(exp2_fast(a.x), exp2_fast(a.y));
-            l2 = add2(l2, pack2(e.x, e.y));
-            w[j / 2] = half_pair(e.x, e.y);
+            const uint64_t e2 = pack2(e.x, e.y);
+            l2 = add2(l2, e2);
+            if constexpr (kExact) {
+              s2 = fma2(e2, j % 4 == 0 ? vm.x : vm.y, s2);
+              const float2 q = unpack2(mul2(e2, j % 4 == 0 ? vs.x : vs.y));
+              w[j / 2] = half_pair(q.x, q.y);
+              const float2 f = half_values(w[j / 2]);
+              rest[j / 2] = half_pair(q.x - f.x, q.y - f.y);
+            } else {
+              w[j / 2] = half_pair(e.x, e.y);
+            }
           }
         };
         if (whole) weigh(std::true_type());
         else weigh(std::false_type());
         tc_st16(t_sh, reinterpret_cast<uint32_t(&)[16]>(w[0]));
         tc_st16(t_sh + 16, reinterpret_cast<uint32_t(&)[16]>(w[16]));
+        if constexpr (kExact) {
+          tc_st16(t_sh + 32, reinterpret_cast<uint32_t(&)[16]>(rest[0]));
+          tc_st16(t_sh + 48, reinterpret_cast<uint32_t(&)[16]>(rest[16]));
+        }
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -508,6 +591,8 @@ kv4_attention_tc_kernel(const Kv4Attention p) {
       }
       const float2 lp = unpack2(l2);
       float l = lp.x + lp.y;
+      const float2 sp = unpack2(s2);
+      const float minima = sp.x + sp.y;
       if (poisoned) l = __int_as_float(0x7fc00000);
       if (ok && tiles > 0) ok = mbar_wait(smem_u32(&bar_pv[g][1]), (uint32_t)(tiles - 1) & 1u, abort_flag);
       if (ok) {
@@ -534,7 +619,8 @@ kv4_attention_tc_kernel(const Kv4Attention p) {
 #pragma unroll
               for (int n = 0; n < 8; ++n) {
                 // a row that sees nothing has no weights, whatever its products are
-                const float x = __int_as_float(v[8 * w + (((n & 3) << 1) | (n >> 2))]) * inv;
+                const float y = __int_as_float(v[8 * w + (((n & 3) << 1) | (n >> 2))]);
+                const float x = (kExact ? y + minima : y) * inv;
                 o[n] = m_ref == -INFINITY && l == 0.0f ? 0.0f : x;
               }
               if (p.splits > 1) store_f32<float, 8>(p.part + at * D + c + 8 * w, o);
@@ -545,7 +631,7 @@ kv4_attention_tc_kernel(const Kv4Attention p) {
         if (p.splits > 1 && real) {
           float* lm = p.part + (int64_t)p.splits * p.rows * D;
           lm[at] = l;
-          lm[(int64_t)p.splits * p.rows + at] = m_ref == -INFINITY ? -INFINITY : m_ref - kRoom;
+          lm[(int64_t)p.splits * p.rows + at] = m_ref == -INFINITY ? -INFINITY : m_ref - kRoom<kExact>;
         }
       }
     }
@@ -581,12 +667,11 @@ int launch(const Kv4Attention& p, cudaStream_t s) {
 }  // namespace
 
 // From 41 rows per key head on (bf16, us, kv4_attention.cu : this kernel; 4 sequences of up to 8000 tokens, 8 key
-// heads: 24 rows 30 : 45, 32 rows 38 : 45, 48 rows 51 : 46; 64 of 8192 tokens, 32 rows 373 : 405).  In fp16 from 64:
-// keys, values and weights are rounded to fp16 here, once each, which leaves outputs off by 4 - 7e-4, two or three
-// times their own rounding, and the other kernel's are as exact as that (48 rows 59 : 40, 64 rows 72 : 42).  An
-// exact split of all three would double this kernel's products.
+// heads: 24 rows 30 : 45, 32 rows 38 : 45, 48 rows 51 : 46; 64 of 8192 tokens, 32 rows 373 : 405), in fp16 from 49 on
+// (the same: 40 rows 65 : 68, 48 rows 68 : 69, 52 rows 89 : 69, 64 rows 92 : 69; 64 of 8192 tokens, 40 rows 654 : 712,
+// 48 rows 767 : 711; 2 of 1500 tokens, 64 channels, 52 rows 12.5 : 16, 96 rows 16.7 : 18).
 bool kv4_tc_wanted(int rows, int dim, int dtype) {
-  return dtype != MODIFF_FP32 && dim <= 128 && rows > (dtype == MODIFF_BF16 ? 40 : 63);
+  return dtype != MODIFF_FP32 && dim <= 128 && rows > (dtype == MODIFF_BF16 ? 40 : 48);
 }
 int kv4_tc_rows() { return kRows; }
 

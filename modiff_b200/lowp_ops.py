@@ -3,8 +3,9 @@ scale per block of 128, norms of queries and keys with the rotation of their pos
 over a paged cache of keys and values held in 4 bits.
 
 Tensors are CUDA tensors of fp32, fp16 or bf16, all of a call on one device; a call is enqueued on that
-device's current stream.  Sums, statistics and softmax are fp32, the result is rounded once.  There is no
-backward pass: inputs that ask for gradients are refused while gradients are recorded.
+device's current stream.  Sums, statistics and softmax are fp32, the result is rounded once; what
+`kv4_attention` holds in fewer bits its docstring says.  There is no backward pass: inputs that ask for
+gradients are refused while gradients are recorded.
 """
 import struct
 from typing import NamedTuple
@@ -397,7 +398,12 @@ def kv4_attention(q, cache, table, lengths, scale=None, causal=True, window=0, s
     them and the first `sinks` of the sequence (tokens outside are not read).  causal=False: every query
     sees all lengths[b] tokens.  A row that sees nothing is 0.  A cached scale or minimum that is not finite
     (`kv4_append` writes NaN for a row that holds one) makes the rows that see its key NaN, those that see its
-    value not finite, and no others.  scale defaults to d ** -0.5."""
+    value not finite, and no others.  scale defaults to d ** -0.5.
+
+    fp32 and fp16: queries and weights count with 22 bits (of a row's largest element), codes exactly, the rest is
+    fp32.  bf16: weights are rounded to fp16, 2^-11 of each at most, and sums of query times code keep 17 bits; from
+    41 query rows per key head on (d <= 128) keys and values are rounded to fp16 as well, once each, so that a
+    score is off by up to scale 2^-11 sum |q k|."""
     name = "kv4_attention"
     device = _device(name, q, table, lengths, *cache)
     c, kv_heads, dim, table, lengths = _cache(name, cache, table, lengths)
