@@ -4,13 +4,15 @@ over a paged cache of keys and values held in 4 bits.
 
 Tensors are CUDA tensors of fp32, fp16 or bf16, all of a call on one device; a call is enqueued on that
 device's current stream.  Sums, statistics and softmax are fp32, the result is rounded once; what
-`kv4_attention` holds in fewer bits its docstring says.  There is no backward pass: inputs that ask for
-gradients are refused while gradients are recorded.
+`kv4_attention` holds in fewer bits its docstring says.  There is no backward pass and no
+forward-mode derivative: inputs that ask for gradients are refused while gradients are recorded, inputs with
+a tangent always.
 """
 import struct
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _lib
 from ._lib import ModiffError
@@ -25,7 +27,8 @@ _stream, _current = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
 def _device(name, *tensors):
-    """The device that all `tensors` (None allowed) are on; CUDA tensors, none of which needs gradients."""
+    """The device that all `tensors` (None allowed) are on; CUDA tensors, none of which needs gradients or
+    carries a tangent."""
     device, grad = -2, _grad_enabled()
     for t in tensors:
         if t is None:
@@ -41,6 +44,10 @@ def _device(name, *tensors):
             device = d
         if grad and t.requires_grad:
             raise ModiffError(f"{name} has no backward pass: call it under torch.no_grad() or detach its inputs")
+    if _forward_ad._current_level >= 0:                        # inside a dual_level or torch.func.jvp
+        for t in tensors:
+            if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+                raise ModiffError(f"{name} has no forward-mode derivative: an input carries a tangent")
     return device
 
 

@@ -1,12 +1,12 @@
 """Low-precision transformer operators: how far attention over the 4-bit cache is from 64 bits, as a norm over
-all outputs, whichever kernel serves a call; cached rows that are not finite."""
+all outputs, whichever kernel serves a call; cached rows that are not finite; and tangents."""
 import math
 
 import pytest
 import torch
 
 import lowp_reference as ref
-from modiff_b200 import ops
+from modiff_b200 import ModiffError, ops
 
 gpu = pytest.mark.gpu
 TYPES = [torch.float32, torch.float16, torch.bfloat16]
@@ -141,3 +141,30 @@ def test_kv4_attention_meets_cached_rows_that_are_not_finite(cuda, n, d, which, 
         for a, c in zip(rest, [clean[1], clean[0, :n - n // 2], clean[0, :, :2]]):
             assert torch.equal(a, c)
     assert torch.equal(ops.kv4_attention(q, cache, table, lens), clean)
+
+
+@gpu
+def test_tangents_are_refused(cuda):
+    """There is no forward-mode derivative either: a tangent is refused, not dropped."""
+    import torch.autograd.forward_ad as fwd
+    x = torch.randn(4, 256, device=cuda)
+    w, ws = ops.fp8_pack_weight(torch.randn(8, 256, device=cuda))
+    cos = torch.ones(4, 32, device=cuda)
+    q = torch.randn(1, 4, 2, 64, device=cuda)
+    cache = ops.kv4_cache(2, 2, 16, 64, cuda)
+    table, lens = torch.zeros(1, 1, dtype=torch.int32, device=cuda), torch.full((1,), 4, dtype=torch.int32, device=cuda)
+    calls = (lambda f: ops.fp8_quantize(f(x)), lambda f: ops.fp8_linear(f(x), w, ws),
+             lambda f: ops.fp8_linear(x, w, ws, f(torch.zeros(8, device=cuda))),
+             lambda f: ops.qk_norm_rope(f(q), None, None, None, cos, cos),
+             lambda f: ops.qk_norm_rope(q, None, None, None, f(cos), cos),
+             lambda f: ops.kv4_append(cache, q, f(q), table, lens),
+             lambda f: ops.kv4_attention(f(q), cache, table, lens))
+    with fwd.dual_level():
+        for call in calls:
+            with pytest.raises(ModiffError, match="tangent"):
+                call(lambda t: fwd.make_dual(t, torch.ones_like(t)))
+            call(lambda t: t)                              # nothing to refuse
+    for call in calls:
+        call(lambda t: t)
+    with pytest.raises(ModiffError, match="tangent"):
+        torch.func.jvp(lambda t: ops.fp8_linear(t, w, ws), (x,), (x,))
