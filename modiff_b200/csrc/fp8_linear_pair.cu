@@ -10,9 +10,9 @@
 // leave through shared memory as 128-byte rows of a bulk store, so that the warps are back at the next
 // tile's blocks at once.
 //
-// Bound: the epilogue warps, about 1000 cycles per block of which the tensor pipe works 512: 256 go to the
-// additions, the rest to waits and tensor-memory loads one after the other.  16384 x 5120 -> 5120, codes
-// to bf16: 376 us, 2.3 PFLOP/s.  What it took: cluster-scope release / acquire on the barriers between the
+// About 1000 cycles a block, of which the tensor pipe works 512 and the additions issue for 256: neither is the
+// limit, the epilogue warps' chain of waits and tensor-memory loads, one after the other, is.  16384 x 5120 -> 5120,
+// codes to bf16: 376 us, 2.3 PFLOP/s.  What it took: cluster-scope release / acquire on the barriers between the
 // two CTAs 1001 us, default scope 430 (nothing but tensor memory passes through them, which tcgen05's own
 // fences order); scales through shared memory, bulk store 407; eight warps of 128 columns with 224
 // registers, loads and additions overlapped 389, with the present ring and register split 376.  Not better: sixteen warps of 64 columns (407), four

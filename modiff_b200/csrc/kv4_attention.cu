@@ -8,9 +8,9 @@
 // Queries are brought to fp16 by a power of two per row (exact for 16-bit types; fp32 queries travel as two
 // fp16 planes, hi + lo, 22 bits).  p_t s_v is held in fp16 relative to the running maximum of (score +
 // exponent of s_v), so that it lies in [0, 2) 2^14 whatever the scales are: in two planes for fp32 and fp16,
-// whose outputs then are as exact as their rounding, in one (2^-12 of each weight at most) for bf16, whose
-// outputs are rounded eight times as coarsely.  The second plane costs 28 % on 64 x 8192 cached tokens of 8
-// heads (148 us for 116).  Sums, maxima and the output stay in fp32.
+// whose outputs then are as exact as their rounding, in one (2^-11 of each weight at most) for bf16, whose
+// outputs are rounded eight times as coarsely.  The second plane and codes that are not subnormal numbers (below)
+// cost 32 % on 64 x 8192 cached tokens of 8 heads (149 us for 113).  Sums, maxima and the output stay in fp32.
 //
 // mma.m16n8k16 with the tokens (scores) or the channels (output) as the 16 rows and eight query rows as
 // the columns: S^T = K Q^T, O^T = V^T P^T.  One step of a conversation has as many query rows per
@@ -148,7 +148,7 @@ kv4_attention_kernel(const Kv4Attention p) {
   const uint32_t* kp_lane = reinterpret_cast<const uint32_t*>(p.c.k_params) + g;
   const uint32_t* vp_lane = reinterpret_cast<const uint32_t*>(p.c.v_params) + g;
 
-  // Rows of the cache where the four pieces of 16 tokens of a tile begin; -1: not there.  Pages of whole
+  // Rows of the cache where the two pieces of 16 tokens of a tile begin; -1: not there.  Pages of whole
   // tiles are looked up once.
   const bool whole_pages = p.c.page_size % kTile == 0;
   auto place = [&](int t0, int64_t (&base)[kSub]) {

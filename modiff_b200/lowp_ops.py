@@ -313,7 +313,8 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6, i
 class KV4Cache(NamedTuple):
     """A paged cache of keys and values in 4 bits (`kv4_cache` makes an empty one): codes uint8 [pages,
     kv_heads, page_size, d / 2], channel 2i in the low half of byte i, and fp16 (scale, minimum) [pages,
-    kv_heads, page_size, 2].  A token's value of channel c is scale * code[c] + minimum."""
+    kv_heads, page_size, 2].  A token's value of channel c is scale * code[c] + minimum, with the scale
+    (largest - smallest value) / 15 (as a product with the fp32 number 1 / 15)."""
     k_codes: torch.Tensor
     k_params: torch.Tensor
     v_codes: torch.Tensor
